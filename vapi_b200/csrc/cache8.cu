@@ -1,0 +1,365 @@
+// A paged cache of keys and values in 8 bits: the write that quantises, the read that gives values back, and causal GQA
+// attention over it.
+//
+// A number is code * 2^e: the code is an e4m3 number (four exponent bits, three of the mantissa, largest 448), and every block
+// of 16 tokens of a head has one e, for keys and for values apart.  e is the smallest in -110 .. 119 with which the block's
+// largest magnitude fits 448.  Powers of two because
+//  * multiplying by one is exact, so a code is the same in every arithmetic that rounds to nearest even, and code * 2^e is a
+//    bfloat16 number;
+//  * a block is written over several steps, and when a later token needs a larger e the older codes move onto it exactly, but
+//    for those that fall below the smallest e4m3 numbers (2^-6 of a code; the largest is 448).
+// A finer scale would buy nothing: e4m3's rounding is relative to each number, not to the block's largest.
+//
+// Layout of a layer: codes [pages][2 (k, v)][nkv][page_size][d], e [pages][2][nkv][page_size / 16].  The 16 tokens of a block of
+// one head are 16 * d bytes in one piece.
+#include "cache8.cuh"
+#include "cache8_decode.cuh"
+
+using namespace vapi;
+
+// ---- the write ----------------------------------------------------------------------------------
+// One warp per (token, head) of a fused row [q heads | k heads | v heads]:
+//   q: norm (if qw) -> rotation (if cosr) -> q_out;
+//   k, v: a warp takes all the step's tokens of its block of 16, if its token is the first of them (slots that follow one
+//   another within a block), else it has nothing to do.  First pass: the largest magnitude (k normed, rotated and rounded to the
+//   activations' type, as an unquantised cache would hold it).  Then e, the older tokens of the block moved onto it if it
+//   grew, and a second pass over the same rows (they are in L1 by then) that writes the codes.
+// A new block's first token (place 0) starts its e afresh: what a page held before is never looked at.
+constexpr int W8_WARPS = 4;
+constexpr int W8_MAX_D = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(W8_WARPS * 32)
+write8_kernel(const T* __restrict__ qkv, const float* __restrict__ qw, const float* __restrict__ kw, float eps, const float* __restrict__ cosr,
+              const float* __restrict__ sinr, int rot, T* __restrict__ q_out, unsigned char* __restrict__ codes, signed char* __restrict__ exps,
+              const int* __restrict__ slots, int n, int nh, int nkv, int d, int page_size, int num_pages, int* __restrict__ status) {
+    __shared__ float sh[W8_WARPS][W8_MAX_D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = nh + 2 * nkv;
+    const long long item = (long long)blockIdx.x * W8_WARPS + warp;
+    pdl_trigger();
+    if (item >= (long long)n * heads) {
+        pdl_wait();
+        return;
+    }
+    const int t = (int)(item / heads), h = (int)(item - (long long)t * heads);
+    const bool is_q = h < nh, is_k = !is_q && h < nh + nkv;
+    // (slots are host-copied index data: safe before the wait)
+    int slot = 0, count = 1;
+    bool mine = true;
+    if (!is_q) {
+        slot = slots[t];
+        const int place = slot & (C8_BLOCK - 1);
+        mine = t == 0 || place == 0 || slot < 0 || slots[t - 1] != slot - 1;
+        const bool follows = lane < C8_BLOCK && place + lane < C8_BLOCK && t + lane < n && slots[min(t + lane, n - 1)] == slot + lane;
+        count = __ffs(~__ballot_sync(0xffffffffu, follows)) - 1;
+    }
+    pdl_wait();
+    if (!mine) return;
+
+    const float* w = is_q ? qw : (is_k ? kw : nullptr);
+    const bool rope = (is_q || is_k) && cosr != nullptr;
+    const int half = rot >> 1;
+    float* s = sh[warp];
+    // element i of token t + j, as the activations' type holds it
+    auto row = [&](int j) { return qkv + ((size_t)(t + j) * heads + h) * d; };
+    auto inv_norm = [&](int j) {
+        const T* src = row(j);
+        __syncwarp();
+        float ss = 0.f;
+        for (int i = lane; i < d; i += 32) {
+            const float v = to_f32(src[i]);
+            s[i] = v;
+            ss += v * v;
+        }
+        __syncwarp();
+        return w ? rsqrtf(warp_sum(ss) / (float)d + eps) : 1.f;
+    };
+    auto element = [&](int j, int i, float inv) {
+        float v = w ? s[i] * inv * w[i] : s[i];
+        if (rope && i < rot) {
+            const int jj = i < half ? i : i - half;
+            const int pi = i < half ? i + half : i - half;
+            const float pv = w ? s[pi] * inv * w[pi] : s[pi];
+            const float c = cosr[(size_t)(t + j) * half + jj], sn = sinr[(size_t)(t + j) * half + jj];
+            v = i < half ? v * c - pv * sn : v * c + pv * sn;
+        }
+        return round_to<T>(v);
+    };
+    if (is_q) {
+        const float inv = inv_norm(0);
+        for (int i = lane; i < d; i += 32) q_out[((size_t)t * nh + h) * d + i] = from_f32<T>(element(0, i, inv));
+        return;
+    }
+    const int page = slot / page_size, off = slot - page * page_size, place = off & (C8_BLOCK - 1);
+    if (slot < 0 || page >= num_pages) {
+        if (lane == 0 && status) atomicExch(status, 2);
+        return;
+    }
+    const int g = is_k ? h - nh : h - nh - nkv;
+    const size_t head = ((size_t)page * 2 + (is_k ? 0 : 1)) * nkv + g;
+    unsigned char* block = codes + (head * page_size + off - place) * d;
+    signed char* exp_at = exps + head * (page_size / C8_BLOCK) + off / C8_BLOCK;
+
+    float amax = 0.f;
+    for (int j = 0; j < count; ++j) {
+        const float inv = inv_norm(j);
+        for (int i = lane; i < d; i += 32) {
+            const float a = fabsf(element(j, i, inv));
+            if (a < INFINITY) amax = fmaxf(amax, a);              // (false for NaN too)
+        }
+    }
+    int e = c8_exponent(warp_max(amax));
+    if (place > 0) {
+        const int old = *exp_at;
+        e = max(e, old);
+        if (e > old) {                                             // the block's older tokens, four codes a lane (d is a multiple of 16)
+            unsigned* older = reinterpret_cast<unsigned*>(block);
+            const float f = c8_power(max(old - e, -126));          // (2^-126 of any code rounds to zero)
+            for (int i = lane; i < place * d / 4; i += 32) older[i] = c8_rescale(older[i], f);
+        }
+    }
+    __syncwarp();                                                  // every lane has read the old e
+    if (lane == 0) *exp_at = (signed char)e;
+    const float f = c8_power(-e);
+    for (int j = 0; j < count; ++j) {
+        const float inv = inv_norm(j);
+        for (int i = lane; i < d; i += 32) block[(size_t)(place + j) * d + i] = c8_code(element(j, i, inv) * f);
+    }
+}
+
+VAPI_EXPORT int vapi_qk_norm_rope_write8(const void* qkv, int dtype, const float* qw, const float* kw, float eps, const float* cosr,
+                                         const float* sinr, int rot, void* q_out, void* codes, void* exps, const int* slots, int n,
+                                         int nh, int nkv, int d, int page_size, int num_pages, int* status, cudaStream_t stream) {
+    if (n <= 0) return 0;
+    if (d < 16 || d > W8_MAX_D || d % 16 != 0) return fail(-1, "qk_norm_rope_write8: head_dim %d is not a multiple of 16 in 16..256", d);
+    if (nh <= 0 || nkv <= 0) return fail(-1, "qk_norm_rope_write8: no heads");
+    if (cosr && (rot <= 0 || rot > d || rot % 2 != 0)) return fail(-1, "qk_norm_rope_write8: rotation width %d does not fit head_dim %d", rot, d);
+    if (page_size <= 0 || page_size % C8_BLOCK != 0 || num_pages <= 0) return fail(-1, "qk_norm_rope_write8: page size %d is not a multiple of 16, or there are no pages", page_size);
+    const long long blocks = ((long long)n * (nh + 2 * nkv) + W8_WARPS - 1) / W8_WARPS;
+    if (blocks > 0x7fffffffLL) return fail(-1, "qk_norm_rope_write8: %d tokens exceed the grid", n);
+    cudaError_t e;
+    if (dtype == VAPI_F32)
+        e = launch(write8_kernel<float>, (unsigned)blocks, W8_WARPS * 32, 0, stream, (const float*)qkv, qw, kw, eps, cosr, sinr, rot, (float*)q_out,
+                   (unsigned char*)codes, (signed char*)exps, slots, n, nh, nkv, d, page_size, num_pages, status);
+    else if (dtype == VAPI_BF16)
+        e = launch(write8_kernel<__nv_bfloat16>, (unsigned)blocks, W8_WARPS * 32, 0, stream, (const __nv_bfloat16*)qkv, qw, kw, eps, cosr, sinr, rot,
+                   (__nv_bfloat16*)q_out, (unsigned char*)codes, (signed char*)exps, slots, n, nh, nkv, d, page_size, num_pages, status);
+    else
+        return fail(-2, "qk_norm_rope_write8: unsupported dtype %d", dtype);
+    return check_launch("qk_norm_rope_write8", e);
+}
+
+// ---- the read -----------------------------------------------------------------------------------
+// Whole pages as numbers, in the order of `pages`: 16 codes (one 16-byte load) a thread; a page id outside the pool leaves zeros
+// and a status.
+template <typename T>
+__global__ void read8_kernel(const unsigned char* __restrict__ codes, const signed char* __restrict__ exps, const int* __restrict__ pages,
+                             T* __restrict__ out, long long pieces, int per_page, int per_block, int num_pages, int* __restrict__ status) {
+    pdl_trigger();
+    pdl_wait();
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= pieces) return;
+    const int at = (int)(i / per_page), piece = (int)(i - (long long)at * per_page);
+    const int page = pages[at];
+    float v[16];
+    if (page < 0 || page >= num_pages) {
+        if (piece == 0 && status) atomicExch(status, 4);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = 0.f;
+    } else {
+        const uint4 c = reinterpret_cast<const uint4*>(codes)[(size_t)page * per_page + piece];
+        const float f = c8_power(exps[(size_t)page * (per_page / per_block) + piece / per_block]);
+        const unsigned w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 x = c8_floats(w[k]);
+            v[4 * k] = x.x * f; v[4 * k + 1] = x.y * f; v[4 * k + 2] = x.z * f; v[4 * k + 3] = x.w * f;
+        }
+    }
+    T* dst = out + 16 * i;
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) reinterpret_cast<float4*>(dst)[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    } else {
+        unsigned w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const unsigned*>(&b);
+        }
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+VAPI_EXPORT int vapi_cache8_read(const void* codes, const void* exps, const int* pages, void* out, int dtype, int count, int nkv, int d,
+                                 int page_size, int num_pages, int* status, cudaStream_t stream) {
+    if (count <= 0) return 0;
+    if (d < 16 || d > 256 || d % 16 != 0) return fail(-1, "cache8_read: head_dim %d is not a multiple of 16 in 16..256", d);
+    if (nkv <= 0 || page_size <= 0 || page_size % C8_BLOCK != 0 || num_pages <= 0) return fail(-1, "cache8_read: page size %d is not a multiple of 16, or there are no pages", page_size);
+    if (((uintptr_t)codes & 15) != 0 || ((uintptr_t)out & 15) != 0) return fail(-1, "cache8_read: the codes or the output are not 16-byte aligned");
+    const long long per_page = 2LL * nkv * page_size * (d / 16), pieces = per_page * count;
+    if (per_page > 0x7fffffffLL || (pieces + 255) / 256 > 0x7fffffffLL) return fail(-1, "cache8_read: %d pages exceed the grid", count);
+    const unsigned blocks = (unsigned)((pieces + 255) / 256);
+    cudaError_t e;
+    if (dtype == VAPI_F32)
+        e = launch(read8_kernel<float>, blocks, 256, 0, stream, (const unsigned char*)codes, (const signed char*)exps, pages, (float*)out, pieces,
+                   (int)per_page, d, num_pages, status);
+    else if (dtype == VAPI_BF16)
+        e = launch(read8_kernel<__nv_bfloat16>, blocks, 256, 0, stream, (const unsigned char*)codes, (const signed char*)exps, pages, (__nv_bfloat16*)out,
+                   pieces, (int)per_page, d, num_pages, status);
+    else
+        return fail(-2, "cache8_read: unsupported dtype %d", dtype);
+    return check_launch("cache8_read", e);
+}
+
+// ---- attention: the general kernel --------------------------------------------------------------
+// float32 activations, head sizes other than 64 and 128.  A block owns 16 rows (query token, q head of the group) of one (sequence,
+// kv head) and walks the keys 32 at a time; K and V of a tile stand in shared memory as floats, a warp owns four rows, a lane
+// one key of the scores and every 32nd element of the output.  One pass with a running maximum and sum per row, in float.
+constexpr int G8_ROWS = 16, G8_KEYS = 32, G8_WARPS = 4, G8_RPW = G8_ROWS / G8_WARPS;
+
+template <typename T, int DMAX>
+__global__ void __launch_bounds__(G8_WARPS * 32)
+attention8_kernel(const C8Params p, const T* __restrict__ q, T* __restrict__ out) {
+    extern __shared__ float g8_smem[];
+    const int d = p.d, pitch = d + 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* sQ = g8_smem;
+    float* sK = sQ + G8_ROWS * pitch;
+    float* sV = sK + G8_KEYS * pitch;
+    const int s = blockIdx.z, g = blockIdx.y, n_rep = p.nh / p.nkv;
+    pdl_trigger();
+    pdl_wait();
+    const int q0 = p.cu_q[s], qlen = p.cu_q[s + 1] - q0, klen = p.seqlens_k[s];
+    const int rows_total = qlen * n_rep, r0 = blockIdx.x * G8_ROWS;
+    if (r0 >= rows_total) return;
+    const int base = klen - qlen;
+    const int p_min = base + r0 / n_rep, p_max = base + (min(rows_total, r0 + G8_ROWS) - 1) / n_rep;
+    for (int i = threadIdx.x; i < G8_ROWS * d; i += blockDim.x) {
+        const int r = i / d, c = i - r * d, rr = r0 + r;
+        const int tok = rr / n_rep, head = g * n_rep + rr - tok * n_rep;
+        sQ[r * pitch + c] = rr < rows_total ? to_f32(q[(size_t)(q0 + tok) * p.q_row_stride + (size_t)head * d + c]) * p.scale_log2e : 0.f;
+    }
+    float m[G8_RPW], l[G8_RPW], o[G8_RPW][DMAX / 32];
+#pragma unroll
+    for (int r = 0; r < G8_RPW; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DMAX / 32; ++c) o[r][c] = 0.f;
+    }
+    const int lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
+    const int* bt = p.block_table + (size_t)s * p.table_stride;
+    for (int k0 = lo / G8_KEYS * G8_KEYS; k0 <= p_max; k0 += G8_KEYS) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * G8_KEYS * (d / 4); i += blockDim.x) {
+            const int kv = i / (G8_KEYS * (d / 4)), j = i - kv * G8_KEYS * (d / 4), r = j / (d / 4), c = j - r * (d / 4), key = k0 + r;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);            // keys behind the end may hold anything, and are not read
+            if (key < klen && key <= p_max && key >= lo) {
+                const int page = bt[key / p.page_size];
+                if (page < 0 || page >= p.num_pages) {
+                    if (p.status) atomicExch(p.status, 4);
+                } else {
+                    const size_t head = ((size_t)page * 2 + kv) * p.nkv + g;
+                    const int off = key % p.page_size;
+                    v = c8_floats(*reinterpret_cast<const unsigned*>(p.codes + (head * p.page_size + off) * d + 4 * c));
+                    const float f = c8_power(p.exps[head * (p.page_size / C8_BLOCK) + off / C8_BLOCK]);
+                    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                }
+            }
+            *reinterpret_cast<float4*>((kv ? sV : sK) + r * pitch + 4 * c) = v;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < G8_RPW; ++r) {
+            const int rr = r0 + warp * G8_RPW + r;
+            if (rr >= rows_total) break;
+            const int pos = base + rr / n_rep, key = k0 + lane;
+            const float* qr = sQ + (warp * G8_RPW + r) * pitch;
+            float x = 0.f;
+            for (int c = 0; c < d; c += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(qr + c), b = *reinterpret_cast<const float4*>(sK + lane * pitch + c);
+                x = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, x))));
+            }
+            const bool sees = key <= pos && key < klen && (p.window <= 0 || key > pos - p.window);
+            x = sees ? x : -INFINITY;
+            const unsigned seen = __ballot_sync(0xffffffffu, sees);
+            if (!seen) continue;
+            const float mx = fmaxf(m[r], warp_max(x)), use = mx == -INFINITY ? 0.f : mx;
+            const float alpha = exp2f(m[r] - use), w = sees ? exp2f(x - use) : 0.f;
+            m[r] = mx;
+            l[r] = l[r] * alpha + warp_sum(w);
+#pragma unroll
+            for (int c = 0; c < DMAX / 32; ++c) o[r][c] *= alpha;
+            for (int k = 0; k < G8_KEYS; ++k) {
+                if (!(seen >> k & 1)) continue;                     // (a NaN behind the mask stays there)
+                const float wk = __shfl_sync(0xffffffffu, w, k);
+#pragma unroll
+                for (int c = 0; c < DMAX / 32; ++c)
+                    if (c * 32 + lane < d) o[r][c] = fmaf(wk, sV[k * pitch + c * 32 + lane], o[r][c]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < G8_RPW; ++r) {
+        const int rr = r0 + warp * G8_RPW + r;
+        if (rr >= rows_total) break;
+        const int tok = rr / n_rep, head = g * n_rep + rr - tok * n_rep;
+        const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];          // a row that sees nothing: zeros
+#pragma unroll
+        for (int c = 0; c < DMAX / 32; ++c)
+            if (c * 32 + lane < d) out[((size_t)(q0 + tok) * p.nh + head) * d + c * 32 + lane] = from_f32<T>(o[r][c] * inv);
+    }
+}
+
+template <typename T, int DMAX>
+static int launch_attention8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, cudaStream_t stream) {
+    const long long tiles = ((long long)max_q * (p.nh / p.nkv) + G8_ROWS - 1) / G8_ROWS;
+    if (tiles > 0x7fffffffLL || p.nkv > 65535 || num_seqs > 65535)
+        return fail(-1, "paged_attention8: the step exceeds the grid (%lld row tiles, %d kv heads, %d sequences)", tiles, p.nkv, num_seqs);
+    const size_t smem = (size_t)(G8_ROWS + 2 * G8_KEYS) * (p.d + 4) * sizeof(float);
+    auto kern = attention8_kernel<T, DMAX>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    }
+    return check_launch("paged_attention8", launch(kern, dim3((unsigned)tiles, p.nkv, num_seqs), G8_WARPS * 32, smem, stream, p, (const T*)q, (T*)out));
+}
+
+// q: [n, *] with `q_row_stride` elements between tokens, head h at h * d; out: [n, nh * d].
+// impl: 0 = the fastest kernel that applies; 1 = the general kernel; 2 = the tensor-core kernel, or an error.
+VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, const void* codes, const void* exps, int dtype, const int* block_table,
+                                      int table_stride, const int* cu_q, const int* seqlens_k, void* out, int n, int num_seqs, int max_q,
+                                      int max_k, int nh, int nkv, int d, int page_size, int num_pages, float scale, int window, int splits,
+                                      int impl, int* status, cudaStream_t stream) {
+    if (n <= 0 || num_seqs <= 0 || max_q <= 0) return 0;
+    if (d < 16 || d > 256 || d % 16 != 0) return fail(-1, "paged_attention8: head_dim %d is not a multiple of 16 in 16..256", d);
+    if (nh <= 0 || nkv <= 0 || nh % nkv != 0) return fail(-1, "paged_attention8: %d heads are not a multiple of %d kv heads", nh, nkv);
+    if (page_size <= 0 || page_size % C8_BLOCK != 0 || num_pages <= 0)
+        return fail(-1, "paged_attention8: page size %d is not a multiple of 16, or there are no pages", page_size);
+    if (((uintptr_t)codes & 15) != 0) return fail(-1, "paged_attention8: the codes are not 16-byte aligned");
+    C8Params p;
+    p.q_row_stride = q_row_stride; p.codes = (const unsigned char*)codes; p.exps = (const signed char*)exps; p.block_table = block_table;
+    p.table_stride = table_stride; p.cu_q = cu_q; p.seqlens_k = seqlens_k; p.nh = nh; p.nkv = nkv; p.d = d; p.page_size = page_size;
+    p.num_pages = num_pages; p.scale_log2e = scale * 1.4426950408889634f; p.window = window; p.status = status;
+    const bool fast = dtype == VAPI_BF16 && (d == 64 || d == 128) && q_row_stride % 8 == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0;
+    if (impl == 2 && !fast)
+        return fail(-3, "paged_attention8: the tensor-core kernel needs bfloat16, head_dim 64 or 128 and 16-byte aligned rows (got dtype %d, head_dim %d)", dtype, d);
+    if (fast && impl != 1) {
+        if (d == 64) return launch_decode8<64>(p, q, out, num_seqs, max_q, splits, stream);
+        return launch_decode8<128>(p, q, out, num_seqs, max_q, splits, stream);
+    }
+#define VAPI_ATT8(T, DM) return launch_attention8<T, DM>(p, q, out, num_seqs, max_q, stream)
+    if (dtype == VAPI_F32) {
+        if (d <= 64) VAPI_ATT8(float, 64); else if (d <= 128) VAPI_ATT8(float, 128); else VAPI_ATT8(float, 256);
+    }
+    if (dtype == VAPI_BF16) {
+        if (d <= 64) VAPI_ATT8(__nv_bfloat16, 64); else if (d <= 128) VAPI_ATT8(__nv_bfloat16, 128); else VAPI_ATT8(__nv_bfloat16, 256);
+    }
+#undef VAPI_ATT8
+    return fail(-2, "paged_attention8: unsupported dtype %d", dtype);
+}
+
+VAPI_EXPORT int vapi_attention8_slots(int d) { return d == 64 ? decode8_slots<64>() : decode8_slots<128>(); }
+VAPI_EXPORT const char* vapi_last_error() { return error_buffer(); }

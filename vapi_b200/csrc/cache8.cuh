@@ -1,0 +1,64 @@
+// What the kernels over an 8-bit cache share: its numbers (cache8.cu says what they are) and the arguments of attention.
+#pragma once
+#include "common.cuh"
+
+namespace vapi {
+
+constexpr int C8_BLOCK = 16;                       // tokens of a head that share a scale
+constexpr int C8_MIN_EXP = -110, C8_MAX_EXP = 119; // 448 * 2^119 is the largest bfloat16 of this form; below 2^-119 nothing is kept
+
+struct C8Params {
+    long long q_row_stride;
+    const unsigned char* codes;
+    const signed char* exps;
+    const int* block_table; int table_stride;
+    const int* cu_q; const int* seqlens_k;
+    int nh, nkv, d, page_size, num_pages;
+    float scale_log2e;
+    int window;
+    int* status;
+};
+
+// 2^e for e in -126 .. 127
+__device__ __forceinline__ float c8_power(int e) { return __int_as_float((e + 127) << 23); }
+
+// The smallest e with amax <= 448 * 2^e, within the limits, for a finite amax >= 0: amax = m * 2^x with 1 <= m < 2, 448 = 1.75 * 2^8.
+__device__ __forceinline__ int c8_exponent(float amax) {
+    const unsigned u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, C8_MIN_EXP), C8_MAX_EXP);
+}
+
+// The nearest e4m3 number (ties to even), magnitudes above 448 as 448; NaN for what is not finite, so that it is seen again.
+__device__ __forceinline__ unsigned char c8_code(float x) {
+    unsigned short c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.f), "f"(x));
+    return fabsf(x) < INFINITY ? (unsigned char)(c & 0xff) : (unsigned char)0x7f;
+}
+
+// Two codes (16 bits) as two halves, exactly; the low byte in the low half.
+__device__ __forceinline__ unsigned c8_halves(unsigned short c) {
+    unsigned h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
+    return h;
+}
+__device__ __forceinline__ float c8_half_lo(unsigned h) {
+    float f;
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %1;\ncvt.f32.f16 %0, a;\n}" : "=f"(f) : "r"(h));
+    return f;
+}
+__device__ __forceinline__ float c8_half_hi(unsigned h) { return c8_half_lo(h >> 16); }
+
+// Four codes as floats.
+__device__ __forceinline__ float4 c8_floats(unsigned c) {
+    const unsigned lo = c8_halves((unsigned short)(c & 0xffffu)), hi = c8_halves((unsigned short)(c >> 16));
+    return make_float4(c8_half_lo(lo), c8_half_hi(lo), c8_half_lo(hi), c8_half_hi(hi));
+}
+
+// Four codes times f, rounded again.
+__device__ __forceinline__ unsigned c8_rescale(unsigned c, float f) {
+    const float4 v = c8_floats(c);
+    return (unsigned)c8_code(v.x * f) | (unsigned)c8_code(v.y * f) << 8 | (unsigned)c8_code(v.z * f) << 16 | (unsigned)c8_code(v.w * f) << 24;
+}
+
+}  // namespace vapi

@@ -172,6 +172,14 @@ def _cuda(*ts: Optional[torch.Tensor]) -> None:
             raise KernelError("vapi_b200 kernels run on CUDA tensors only; there is no CPU fallback")
 
 
+def _here(*ts: Optional[torch.Tensor]) -> None:
+    """Tensors that a kernel launched now can follow: all on the current device."""
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -2299,3 +2307,8 @@ def fixed_decay_memory(qkv: torch.Tensor, powers: torch.Tensor, state: torch.Ten
         1 if act == "silu" else 0, _p(state), ctypes.c_longlong(state.stride(0)), _p(state_slots), _p(cu_q), _p(positions), _p(out),
         S, nh, dk, dv, state.shape[0], max_q, _p(scratch), chunks, int(least), _p(status), _stream()), launches)
     return out
+
+
+# operators of serving in fewer bits, each in a file of its own
+from .cache8 import (CACHE8_BLOCK, Cache8, attention8_splits, cache8_empty, cache8_read, paged_attention8,  # noqa: E402
+                     qk_norm_rope_write8)

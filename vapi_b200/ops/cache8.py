@@ -1,0 +1,152 @@
+"""A paged cache of keys and values in 8 bits: the write, the read, and attention over it (csrc/cache8.cu)."""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import (KernelError, _check, _contig, _cuda, _dt, _f32, _here, _i32, _least, _lib, _p, _stream, sm_count)
+
+#: tokens of a head that share a scale
+CACHE8_BLOCK = 16
+
+
+class Cache8(NamedTuple):
+    """A layer's keys and values in 8 bits.  ``codes`` [pages, 2, nkv, page_size, d] are e4m3 numbers, ``exps``
+    [pages, 2, nkv, page_size / 16] int8 the powers of two that blocks of 16 tokens of a head are scaled by: a number is
+    ``code * 2^exp``.  A block's exponent is the smallest in -110..119 with which its largest magnitude fits 448."""
+
+    codes: torch.Tensor
+    exps: torch.Tensor
+
+
+def cache8_empty(pages: int, nkv: int, page_size: int, d: int, device="cuda") -> Cache8:
+    """Memory for a layer's cache (its contents undefined)."""
+    if page_size <= 0 or page_size % CACHE8_BLOCK:
+        raise KernelError(f"page size {page_size} must be a positive multiple of {CACHE8_BLOCK}")
+    return Cache8(torch.empty((pages, 2, nkv, page_size, d), dtype=torch.float8_e4m3fn, device=device),
+                  torch.empty((pages, 2, nkv, page_size // CACHE8_BLOCK), dtype=torch.int8, device=device))
+
+
+def _cache8(cache: Cache8, nkv: int, d: int):
+    """(pages, page size) of a cache, checked."""
+    codes, exps = cache
+    if codes.dtype != torch.float8_e4m3fn or codes.dim() != 5 or codes.shape[1] != 2 or codes.shape[2] != nkv or codes.shape[4] != d:
+        raise KernelError(f"the codes must be [pages, 2, {nkv}, page_size, {d}] of float8_e4m3fn, got {tuple(codes.shape)} of {codes.dtype}")
+    pages, page_size = codes.shape[0], codes.shape[3]
+    if page_size % CACHE8_BLOCK or page_size == 0 or pages == 0:
+        raise KernelError(f"a cache of {pages} pages of {page_size} tokens: pages must hold a positive multiple of {CACHE8_BLOCK}")
+    if exps.dtype != torch.int8 or tuple(exps.shape) != (pages, 2, nkv, page_size // CACHE8_BLOCK):
+        raise KernelError(f"the exponents must be {(pages, 2, nkv, page_size // CACHE8_BLOCK)} of int8, got {tuple(exps.shape)} of {exps.dtype}")
+    _contig(codes, "codes")
+    _contig(exps, "exponents")
+    return pages, page_size
+
+
+def qk_norm_rope_write8(qkv: torch.Tensor, nh: int, nkv: int, d: int, q_weight: Optional[torch.Tensor],
+                        k_weight: Optional[torch.Tensor], eps: float, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                        rot: int, cache: Cache8, slot_mapping: torch.Tensor, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`qk_norm_rope_write` for a cache in 8 bits: per-head RMSNorm and rotate-half RoPE of q and k in a fused ``qkv``
+    [n, (nh+2nkv)*d], which is left as it was; returns q [n, nh*d], and writes the keys (normed, rotated, rounded to the
+    activations' type) and the values to ``cache`` at ``slot_mapping``.
+
+    Tokens of one block of 16 must follow one another in the step, as a request's do.  A block whose first token (place 0) is
+    among them begins afresh; the older tokens of another one are rounded again when a new token needs a larger scale.  What
+    is not finite is kept as NaN."""
+    _contig(qkv, "qkv")
+    for t, w in ((q_weight, "q norm weight"), (k_weight, "k norm weight"), (cos, "cos"), (sin, "sin")):
+        _f32(t, w)
+    _i32(slot_mapping, "slot mapping")
+    _contig(slot_mapping, "slot mapping")
+    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * d:
+        raise KernelError(f"qkv is {tuple(qkv.shape)}, expected {(nh + 2 * nkv) * d} columns")
+    n = qkv.shape[0]
+    pages, page_size = _cache8(cache, nkv, d)
+    _least(slot_mapping, n, "slot mapping")
+    for t, w in ((q_weight, "q norm weight"), (k_weight, "k norm weight")):
+        if t is not None and t.numel() != d:
+            raise KernelError(f"the {w} must be [head_dim]")
+    if (cos is None) != (sin is None) or (cos is not None and (tuple(cos.shape) != (n, rot // 2) or sin.shape != cos.shape)):
+        raise KernelError("cos/sin must be [n, rot/2]")
+    _cuda(qkv, q_weight, k_weight, cos, sin, cache.codes, cache.exps, slot_mapping)
+    _here(qkv, q_weight, k_weight, cos, sin, cache.codes, cache.exps, slot_mapping)
+    q = torch.empty((n, nh * d), dtype=qkv.dtype, device=qkv.device)
+    lib = _lib("cache8")
+    _check(lib, lib.vapi_qk_norm_rope_write8(_p(qkv), _dt(qkv), _p(q_weight), _p(k_weight), eps, _p(cos), _p(sin), rot, _p(q),
+                                             _p(cache.codes), _p(cache.exps), _p(slot_mapping), n, nh, nkv, d, page_size, pages,
+                                             _p(status), _stream()), launches=int(n > 0))
+    return q
+
+
+def cache8_read(cache: Cache8, pages: torch.Tensor, dtype: torch.dtype, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What whole pages of a cache hold, [len(pages), 2, nkv, page_size, d] in ``dtype`` (bfloat16 holds every number of the
+    cache exactly, and so does float32): to move a request's tokens to another cache, or to look at them."""
+    _i32(pages, "pages")
+    _contig(pages, "pages")
+    nkv, d = (cache.codes.shape[2], cache.codes.shape[4]) if cache.codes.dim() == 5 else (0, 0)
+    num_pages, page_size = _cache8(cache, nkv, d)
+    _cuda(cache.codes, cache.exps, pages)
+    _here(cache.codes, cache.exps, pages)
+    out = torch.empty((pages.numel(), 2, nkv, page_size, d), dtype=dtype, device=cache.codes.device)
+    lib = _lib("cache8")
+    _check(lib, lib.vapi_cache8_read(_p(cache.codes), _p(cache.exps), _p(pages), _p(out), _dt(out), pages.numel(), nkv, d, page_size,
+                                     num_pages, _p(status), _stream()), launches=int(pages.numel() > 0))
+    return out
+
+
+_slots = {}
+
+
+def attention8_splits(num_seqs: int, max_q: int, max_k: int, nh: int, nkv: int, d: int) -> int:
+    """How many blocks (of eight warps) share the keys of one (sequence, kv head, tile of rows) in :func:`paged_attention8`: a power of
+    two up to a cluster's 16, while all blocks are on the device at once and each warp still has two blocks of 16 tokens."""
+    rows = max_q * (nh // nkv)
+    blocks = num_seqs * nkv * -(-rows // (8 if rows <= 8 else 16))
+    key = (torch.cuda.current_device(), d)
+    slots = _slots.get(key)
+    if slots is None:
+        slots = _slots[key] = int(_lib("cache8").vapi_attention8_slots(d)) or 2 * sm_count()
+    splits = 1
+    while splits < 16 and 2 * splits * blocks <= slots and 2 * splits * 256 <= max_k:
+        splits *= 2
+    return splits
+
+
+_IMPL8 = {"auto": 0, "general": 1, "tensor_core": 2}
+
+
+def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_table: torch.Tensor, cu_q: torch.Tensor,
+                     seqlens_k: torch.Tensor, n: int, num_seqs: int, max_q: int, max_k: int, nh: int, nkv: int, d: int,
+                     scale: float, window: int = 0, splits: Optional[int] = None, status: Optional[torch.Tensor] = None,
+                     impl: str = "auto") -> torch.Tensor:
+    """:func:`paged_attention` over a cache in 8 bits; returns [n, nh*d].  Arguments as there; the numbers of the cache are taken
+    exactly, scores, softmax and sums are float32.  A query without a visible key gets zeros.
+
+    ``impl``: "tensor_core" forces the kernels for bfloat16 and head size 64 or 128, "general" the one that takes every type,
+    head size (a multiple of 16 up to 256) and page size (a multiple of 16); "auto" picks."""
+    for t, w in ((block_table, "block table"), (cu_q, "cu_q"), (seqlens_k, "seqlens_k")):
+        _i32(t, w)
+    if impl not in _IMPL8:
+        raise KernelError(f"impl `{impl}` is not one of {', '.join(_IMPL8)}")
+    if nh <= 0 or nkv <= 0 or nh % nkv:
+        raise KernelError(f"{nh} heads are not a multiple of {nkv} kv heads")
+    if block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] < num_seqs:
+        raise KernelError("block table must be [S, width] with unit inner stride")
+    _contig(cu_q, "cu_q")
+    _contig(seqlens_k, "seqlens_k")
+    _least(cu_q, num_seqs + 1, "cu_q")
+    _least(seqlens_k, num_seqs, "seqlens_k")
+    if q.stride(-1) != 1 or q_row_stride < nh * d or (n > 0 and q.untyped_storage().nbytes() < (q.storage_offset() + (n - 1) * q_row_stride + nh * d) * q.element_size()):
+        raise KernelError(f"q {tuple(q.shape)} does not hold {n} rows of {nh * d} at a stride of {q_row_stride}")
+    pages, page_size = _cache8(cache, nkv, d)
+    _cuda(q, cache.codes, cache.exps, block_table, cu_q, seqlens_k)
+    _here(q, cache.codes, cache.exps, block_table, cu_q, seqlens_k)
+    if splits is None:
+        splits = attention8_splits(num_seqs, max_q, max_k, nh, nkv, d)
+    out = torch.empty((n, nh * d), dtype=q.dtype, device=q.device)
+    lib = _lib("cache8")
+    _check(lib, lib.vapi_paged_attention8(_p(q), q_row_stride, _p(cache.codes), _p(cache.exps), _dt(q), _p(block_table), block_table.stride(0),
+                                          _p(cu_q), _p(seqlens_k), _p(out), n, num_seqs, max_q, max_k, nh, nkv, d, page_size, pages,
+                                          scale, window, splits, _IMPL8[impl], _p(status), _stream()), launches=int(n > 0))
+    return out
