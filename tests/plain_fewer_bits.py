@@ -113,3 +113,14 @@ def attention8_splits(num_seqs, max_q, max_k, nh, nkv, d):
 
 
 OPS = ["qk_norm_rope_write8", "paged_attention8", "attention8_splits"]
+
+
+def token_logprobs(logits, tokens, top=0, status=None, slices=0):
+    from vapi_b200 import ops
+    lp = torch.log_softmax(logits.double(), 1)
+    ids = torch.argsort(-logits.double(), dim=1, stable=True)[:, :top]
+    return ops.TokenLogprobs(lp.gather(1, tokens.long()[:, None])[:, 0].float(), -torch.where(lp > -math.inf, lp.exp() * lp, 0.0).sum(1).float(),
+                             ids.to(torch.int32), lp.gather(1, ids).float())
+
+
+OPS += ["token_logprobs"]

@@ -20,6 +20,7 @@
 // sequence did write, though a row may not see it, can reach that row through 0 * NaN; the step that wrote it was lost.)
 #pragma once
 #include "cache8.cuh"
+#include "cluster.cuh"
 #include "tcgen05.cuh"           // mbarriers with bounded waits
 
 namespace vapi {
@@ -59,25 +60,6 @@ __device__ __forceinline__ uint2 d8_lds8(unsigned addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ void d8_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ unsigned d8_peer(const void* local, unsigned rank) {      // this address in the shared memory of block `rank`
-    unsigned remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
-    return remote;
-}
-__device__ __forceinline__ float d8_peer_f32(unsigned addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 d8_peer_f32x4(unsigned addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-
 // WIDE: tiles of 16 rows; else of 8 (the lower half of every fragment is then zero and is not worked out).
 template <int HD, bool WIDE>
 __global__ void __launch_bounds__(D8_WARPS * 32, 2)
@@ -360,22 +342,22 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         }
     }
     if (splits > 1) {
-        d8_cluster_sync();                                                  // every block's result is in place
+        cluster_sync();                                                  // every block's result is in place
         for (int i = threadIdx.x * splits + rank; i < ROWS * HD / 4; i += D8_WARPS * 32 * splits) {
             const int r = i / (HD / 4), c = i % (HD / 4) * 4;
             float mx = -INFINITY, sum = 0.f;
-            for (int j = 0; j < splits; ++j) mx = fmaxf(mx, d8_peer_f32(d8_peer(&xM[r], (unsigned)j)));
+            for (int j = 0; j < splits; ++j) mx = fmaxf(mx, cluster_f32(cluster_peer(&xM[r], (unsigned)j)));
             const float mu = mx == -INFINITY ? 0.f : mx;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int j = 0; j < splits; ++j) {
-                const float a = d8_ex2(d8_peer_f32(d8_peer(&xM[r], (unsigned)j)) - mu);
-                const float4 y = d8_peer_f32x4(d8_peer(&xO[r][c], (unsigned)j));
-                sum = fmaf(d8_peer_f32(d8_peer(&xL[r], (unsigned)j)), a, sum);
+                const float a = d8_ex2(cluster_f32(cluster_peer(&xM[r], (unsigned)j)) - mu);
+                const float4 y = cluster_f32x4(cluster_peer(&xO[r][c], (unsigned)j));
+                sum = fmaf(cluster_f32(cluster_peer(&xL[r], (unsigned)j)), a, sum);
                 x.x = fmaf(y.x, a, x.x); x.y = fmaf(y.y, a, x.y); x.z = fmaf(y.z, a, x.z); x.w = fmaf(y.w, a, x.w);
             }
             store(r, c, x, sum);
         }
-        d8_cluster_sync();                                                  // nobody reads this block's memory any more
+        cluster_sync();                                                  // nobody reads this block's memory any more
     }
     if (threadIdx.x == 0 && failed && p.status) atomicExch(p.status, 16);
 }

@@ -2312,3 +2312,4 @@ def fixed_decay_memory(qkv: torch.Tensor, powers: torch.Tensor, state: torch.Ten
 # operators of serving in fewer bits, each in a file of its own
 from .cache8 import (CACHE8_BLOCK, Cache8, attention8_splits, cache8_empty, cache8_read, paged_attention8,  # noqa: E402
                      qk_norm_rope_write8)
+from .logprobs import LOGPROBS_MAX_TOP, TokenLogprobs, token_logprobs  # noqa: E402
