@@ -124,3 +124,36 @@ def token_logprobs(logits, tokens, top=0, status=None, slices=0):
 
 
 OPS += ["token_logprobs"]
+
+
+def unpack(w):
+    """(codes, scales, zeros) of an Int4Weight, read from its words bit by bit (host)."""
+    words, pairs = w.codes.cpu(), w.scales.cpu()
+    tiles, chunks = words.shape[:2]
+    codes = torch.zeros(tiles, 2, 8, chunks, 2, 4, 2, 2, 2, dtype=torch.uint8)
+    lanes = words.view(tiles, chunks, 8, 4, 2, 2)
+    for h in range(2):
+        for p in range(2):
+            for e in range(2):
+                codes[:, h, :, :, :, :, :, p, e] = ((lanes >> (8 * p + 4 * h + 16 * e)) & 15).permute(0, 2, 1, 4, 3, 5).to(torch.uint8)
+    table = pairs.permute(0, 3, 2, 1).reshape(tiles * 16, -1)[:w.n]
+    number = lambda t: (t & 0xffff).to(torch.int16).view(torch.bfloat16)
+    return codes.reshape(tiles * 16, chunks * 64)[:w.n, :w.k], number(table), number(table >> 16) - 128
+
+
+def int4_numbers(w):
+    codes, scales, zeros = unpack(w)
+    return (codes.double() - zeros.double().repeat_interleave(w.group, 1)) * scales.double().repeat_interleave(w.group, 1)
+
+
+def int4_linear(x, w, bias=None, out_dtype=None):
+    y = x.double() @ int4_numbers(w).t()
+    return (y if bias is None else y + bias.double()).to(out_dtype or x.dtype)
+
+
+def int4_linear_swiglu(x, w, act="silu"):
+    import plain_ops
+    return plain_ops.swiglu(int4_linear(x, w, out_dtype=torch.float32), act).to(x.dtype)
+
+
+OPS += ["int4_linear", "int4_linear_swiglu"]

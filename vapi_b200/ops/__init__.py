@@ -714,7 +714,10 @@ PROMPT_SWIGLU_MIN_ROWS = int(os.environ.get("VAPI_PROMPT_SWIGLU_MIN_ROWS", "256"
 
 def linear_swiglu(x: torch.Tensor, weight: torch.Tensor, act: str = "silu") -> torch.Tensor:
     """``act(x @ Wg.T) * (x @ Wu.T)`` for ``weight = [Wg; Wu]`` (``act`` "silu" or "gelu_tanh"): one kernel with the gate as the
-    product's epilogue for prompt-sized bfloat16 steps, else the product followed by :func:`swiglu`."""
+    product's epilogue for prompt-sized bfloat16 steps, else the product followed by :func:`swiglu`.  A 4-bit weight goes to
+    :func:`int4_linear_swiglu`."""
+    if type(weight) is Int4Weight:
+        return int4_linear_swiglu(x, weight, act)
     rows = x.shape[0]
     if (x.dtype == torch.bfloat16 and 0 < PROMPT_SWIGLU_MIN_ROWS <= rows and rows > TC_MAX_ROWS and weight.is_cuda
             and weight.dtype == torch.bfloat16 and weight.dim() == 2 and weight.shape[1] % 8 == 0 and weight.shape[0] % 16 == 0
@@ -779,8 +782,9 @@ def prompt_linear(weight: torch.Tensor, *, act: Optional[torch.Tensor] = None, x
 
 def few_rows_applies(rows: int, weight: torch.Tensor) -> bool:
     """Whether one of this package's own products (with their fused prologues and epilogues)
-    takes a step of ``rows`` rows against ``weight``."""
-    return (skinny_applies(rows, weight) or tc_applies(rows, weight, max(TC_MAX_ROWS, STREAM_PROMPT_MAX_ROWS))
+    takes a step of ``rows`` rows against ``weight`` (not with a 4-bit one)."""
+    return type(weight) is not Int4Weight and (
+            skinny_applies(rows, weight) or tc_applies(rows, weight, max(TC_MAX_ROWS, STREAM_PROMPT_MAX_ROWS))
             or prompt_applies(rows, weight))
 
 
@@ -906,8 +910,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     this package's kernels, the others on the library.
 
     float32 runs without any reduced-precision mode (see :func:`strict_fp32`).  A weight kept
-    in float32 beside bfloat16 activations is multiplied in float32.
+    in float32 beside bfloat16 activations is multiplied in float32.  A 4-bit weight goes to :func:`int4_linear`.
     """
+    if type(weight) is Int4Weight:
+        return int4_linear(x, weight, bias, out_dtype)
     _cuda(x, weight)
     if bias is not None:
         vector = _bias_vector(bias, weight.shape[0])
@@ -2312,4 +2318,6 @@ def fixed_decay_memory(qkv: torch.Tensor, powers: torch.Tensor, state: torch.Ten
 # operators of serving in fewer bits, each in a file of its own
 from .cache8 import (CACHE8_BLOCK, Cache8, attention8_splits, cache8_empty, cache8_read, paged_attention8,  # noqa: E402
                      qk_norm_rope_write8)
+from .int4 import (INT4_GROUPS, INT4_MAX_ROWS, Int4Weight, int4_dequantize, int4_linear, int4_linear_swiglu, int4_pack,  # noqa: E402
+                   int4_quantize)
 from .logprobs import LOGPROBS_MAX_TOP, TokenLogprobs, token_logprobs  # noqa: E402
