@@ -12,7 +12,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # the heavy parts import torch and (on first use) build kernels: load them lazily
-    if name in ("LLM", "generate", "Completion"):
+    if name in ("LLM", "generate", "Completion", "TextScore"):
         from . import api
         return getattr(api, name)
     if name == "ModelRunner":
@@ -24,4 +24,4 @@ def __getattr__(name):
     raise AttributeError(name)
 
 
-__all__ = ["LLM", "generate", "Completion", "SamplingParams", "FinishReason", "ModelRunner", "RuntimeConfig"]
+__all__ = ["LLM", "generate", "Completion", "TextScore", "SamplingParams", "FinishReason", "ModelRunner", "RuntimeConfig"]

@@ -20,6 +20,7 @@ from .config.runtime import RuntimeConfig
 from .engine.engine import Engine
 from .engine.runner import ModelRunner
 from .engine.scheduler import SchedulerConfig
+from .engine.score import TextScore, score_texts
 from .sampling.params import SamplingParams
 
 
@@ -42,12 +43,17 @@ class LLM:
                  cuda_graphs: bool = True, max_concurrent_seqs: int = 64, max_batched_tokens: int = 8192,
                  prefill_chunk_tokens: int = 2048, watermark: float = 0.01, max_step_failures: int = 3,
                  random_weights: Optional[int] = None, config_json: Optional[Dict[str, Any]] = None,
-                 page_size: Optional[int] = None, validate: bool = False, run_ahead: Optional[bool] = None):
+                 page_size: Optional[int] = None, validate: bool = False, run_ahead: Optional[bool] = None,
+                 kv_cache_dtype: str = "auto", weight_dtype: str = "auto", weight_group: int = 64):
+        """``kv_cache_dtype`` "fp8" keeps keys and values in 8 bits with a scale for each 16 tokens of a head, ``weight_dtype`` "int4" the
+        layers' matrices in 4 bits with a scale and a zero for each ``weight_group`` (32, 64 or 128) columns of a row; "auto" is the
+        activations' type.  A model one of whose layers has no such form is refused.  :meth:`score` says what they cost."""
         dt = "float32" if str(dtype).lower() in ("f32", "fp32", "float32") else "bfloat16"
         kw = dict(dtype=dt, device=device, page_size=page_size or ModelRunner.default_page_size,
                   num_pages=num_blocks, max_requests=max_concurrent_seqs,
                   max_batched_tokens=max_batched_tokens, max_context=max_context, watermark=watermark,
-                  kv_cache_fraction=kv_cache_fraction, validate=validate)
+                  kv_cache_fraction=kv_cache_fraction, validate=validate, kv_cache_dtype=kv_cache_dtype,
+                  weight_dtype=weight_dtype, weight_group=weight_group)
         if random_weights is not None:
             if config_json is None:
                 raise ValueError("random weights need a config_json (the architecture's config.json keys)")
@@ -69,9 +75,19 @@ class LLM:
                   kv_cache_fraction=m.kv_cache_fraction, num_blocks=m.num_blocks, cuda_graphs=m.cuda_graphs,
                   max_concurrent_seqs=w.max_concurrent_seqs, max_batched_tokens=w.max_batched_tokens,
                   prefill_chunk_tokens=w.prefill_chunk_tokens, watermark=c.watermark,
-                  max_step_failures=w.max_step_failures)
+                  max_step_failures=w.max_step_failures, kv_cache_dtype=c.dtype, weight_dtype=m.weight_dtype,
+                  weight_group=m.weight_group)
         kw.update(overrides)
         return cls(**kw)
+
+    def score(self, texts: Sequence[Sequence[int]], top: int = 0) -> List[TextScore]:
+        """What the model says of each text (a list of token ids): for every token but the first its log probability given those
+        before it, the entropy of the distribution it was one of, and the ``top`` (0..20) most likely tokens there.  Nothing may
+        be in generation meanwhile.  (The reference reports log-probabilities of generated tokens only,
+        crates/vapi-engine/src/sampler.rs:114-153.)"""
+        if not self.engine.is_idle():
+            raise RuntimeError("texts are scored between generations, not during one")
+        return score_texts(self.runner, texts, top, self.engine.cfg.prefill_chunk_tokens)
 
     def generate(self, prompts: Sequence[Sequence[int]],
                  params: Union[SamplingParams, Sequence[SamplingParams], None] = None,

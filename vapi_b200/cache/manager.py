@@ -7,7 +7,8 @@ Call sites of the model's run order that own a cache are grouped by what they ne
   tensor ``[sites, pages, page_size * elements per token]`` and one block table per request.
   Inside a page the spec's buffers follow one another, each as ``[rows, page_size, width]``, so
   keys and values of ``n_kv`` heads lie as ``[2, n_kv, page_size, head_dim]``; the manager
-  itself only knows sizes.  A group with a window gives pages back as soon as the window has
+  itself only knows sizes.  Pages of 8-bit codes have a second tensor beside them, the exponents of
+  their blocks of 16 tokens.  A group with a window gives pages back as soon as the window has
   passed them.
 * a **state group** per distinct :class:`~vapi_b200.parts.base.StateSpec`: one device tensor
   ``[slots + 1, sites, *shape]``.  All state groups share one slot pool, so a request holds a
@@ -43,9 +44,11 @@ class PagedGroup:
     sites: List[int]
     pool: PagePool
     tensor: torch.Tensor            # [sites, pages, page_size * elements per token]
+    exps: Optional[torch.Tensor] = None      # of 8-bit codes: [sites, pages, page_size / 16 * exponents per block]
 
     def bytes_per_token(self) -> int:
-        return len(self.sites) * self.spec.elems_per_token() * self.tensor.element_size()
+        """(rounded up where 16 tokens share an exponent)"""
+        return -(-len(self.sites) * self.spec.page_bytes(16, self.tensor.element_size()) // 16)
 
 
 @dataclass
@@ -126,9 +129,11 @@ class CacheManager:
             raise ValueError(hostlib.last_error())
         for gi, (spec, ss) in enumerate(by_paged.items()):
             t = torch.empty((len(ss), sizes[gi][0], self.page_size * spec.elems_per_token()),
-                            dtype=dtype, device=self.device)
+                            dtype=torch.float8_e4m3fn if spec.eight_bit else dtype, device=self.device)
+            exps = torch.empty((len(ss), sizes[gi][0], self.page_size // 16 * spec.exps_per_block()), dtype=torch.int8,
+                               device=self.device) if spec.eight_bit else None
             pool = PagePool(borrowed=self._lib.vh_cache_group_pool(self._h, gi), owner=self)
-            self.paged.append(PagedGroup(spec, list(ss), pool, t))
+            self.paged.append(PagedGroup(spec, list(ss), pool, t, exps))
             for j, s in enumerate(ss):
                 self._site[s] = ("paged", gi, j)
         self.slots = SlotPool(borrowed=self._lib.vh_cache_slot_pool(self._h), owner=self)
@@ -178,6 +183,13 @@ class CacheManager:
         if kind == "paged":
             return self.paged[gi].tensor[j]
         return self.state[gi].tensor[:, j]
+
+    def site_exps(self, site: int) -> Optional[torch.Tensor]:
+        """The exponents beside a call site's pages of 8-bit codes (None: its pages hold numbers)."""
+        if site not in self._site or self._site[site][0] != "paged":
+            return None
+        _, gi, j = self._site[site]
+        return None if self.paged[gi].exps is None else self.paged[gi].exps[j]
 
     def site_buffers(self, site: int) -> Optional[Dict[str, torch.Tensor]]:
         """A paged call site's pages seen buffer by buffer: name -> [pages, rows, page_size, width]

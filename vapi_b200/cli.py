@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import sys
 from typing import List, Optional
 
@@ -28,6 +29,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--num-blocks", type=int)
     g.add_argument("--cuda-graphs", dest="cuda_graphs", action="store_true", default=None)
     g.add_argument("--no-cuda-graphs", dest="cuda_graphs", action="store_false")
+    g.add_argument("--weight-dtype", choices=["auto", "int4"], help="int4: the layers' matrices in 4 bits")
+    g.add_argument("--weight-group", type=int, choices=[32, 64, 128], help="columns of a 4-bit matrix that share a scale")
     g.add_argument("--random-weights", type=int, metavar="SEED",
                    help="draw random weights for --config-json instead of loading a folder")
     g.add_argument("--config-json", help="a config.json to use with --random-weights")
@@ -38,6 +41,7 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--max-step-failures", type=int)
     g = ap.add_argument_group("[cache]")
     g.add_argument("--watermark", type=float)
+    g.add_argument("--kv-cache-dtype", choices=["auto", "fp8"], help="fp8: keys and values in 8 bits ([cache] dtype)")
     g = ap.add_argument_group("sampling")
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--top-p", type=float, default=1.0)
@@ -55,6 +59,9 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--prompt-ids", action="append", default=[], metavar="ID,ID,...",
                    help="a prompt as comma-separated token ids (repeatable); without it, "
                         "JSON lists are read from standard input, one per line")
+    g.add_argument("--score", action="store_true",
+                   help="generate nothing: print each prompt's token log-probabilities, their entropies and its perplexity "
+                        "(--logprobs N: and the N most likely tokens at each place)")
     g.add_argument("--stats", action="store_true", help="print engine statistics to stderr at the end")
     return ap
 
@@ -67,13 +74,16 @@ def main(argv: Optional[List[str]] = None) -> int:
     except RuntimeConfigError as e:
         print(f"vapi_b200: {e}", file=sys.stderr)
         return 2
-    for sec, keys in (("model", ("path", "dtype", "max_context", "kv_cache_fraction", "num_blocks", "cuda_graphs")),
+    for sec, keys in (("model", ("path", "dtype", "max_context", "kv_cache_fraction", "num_blocks", "cuda_graphs",
+                                "weight_dtype", "weight_group")),
                       ("worker", ("max_concurrent_seqs", "max_batched_tokens", "prefill_chunk_tokens", "max_step_failures")),
                       ("cache", ("watermark",))):
         for k in keys:
             v = getattr(args, k)
             if v is not None:
                 setattr(getattr(cfg, sec), k, v)
+    if args.kv_cache_dtype is not None:
+        cfg.cache.dtype = args.kv_cache_dtype
     try:
         cfg.validate()
     except RuntimeConfigError as e:
@@ -101,7 +111,25 @@ def main(argv: Optional[List[str]] = None) -> int:
     elif not cfg.model.path:
         print("vapi_b200: no model: give [model] path, --path, or --random-weights with --config-json", file=sys.stderr)
         return 2
-    llm = LLM.from_config(cfg, **overrides)
+    try:
+        llm = LLM.from_config(cfg, **overrides)
+    except ValueError as e:
+        if cfg.model.weight_dtype == "auto" and cfg.cache.dtype == "auto":
+            raise
+        print(f"vapi_b200: {e}", file=sys.stderr)          # a model that has no such form
+        return 2
+    if args.score:
+        try:
+            scores = llm.score(prompts, args.logprobs or 0)
+        except ValueError as e:
+            print(f"vapi_b200: {e}", file=sys.stderr)
+            return 2
+        for i, s in enumerate(scores):
+            rec = {"request": i, "tokens": len(s.tokens), "perplexity": s.perplexity if math.isfinite(s.perplexity) else None, "logprobs": s.logprobs, "entropies": s.entropies}
+            if args.logprobs:
+                rec["top"] = s.top
+            print(json.dumps(rec), flush=True)
+        return 0
     params = SamplingParams(
         temperature=args.temperature, top_p=args.top_p, top_k=args.top_k, min_p=args.min_p,
         repetition_penalty=args.repetition_penalty, frequency_penalty=args.frequency_penalty,

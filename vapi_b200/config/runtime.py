@@ -14,6 +14,8 @@ errors, as with the reference's ``deny_unknown_fields``.  Precedence of the file
     kv_cache_fraction = 0.85   # of free device memory, when num_blocks is not given
     num_blocks = 2048          # cache pages; the reference's name for them
     cuda_graphs = false
+    weight_dtype = "auto"      # auto | int4   (the layers' matrices in 4 bits)
+    weight_group = 64          # columns that share a scale: 32 | 64 | 128
 
     [worker]
     max_concurrent_seqs = 64
@@ -23,6 +25,9 @@ errors, as with the reference's ``deny_unknown_fields``.  Precedence of the file
 
     [cache]
     watermark = 0.01
+    dtype = "auto"             # auto | fp8    (keys and values in 8 bits)
+
+The last three keys, ``weight_dtype``, ``weight_group`` and ``[cache] dtype``, are this engine's own.
 """
 from __future__ import annotations
 
@@ -44,6 +49,8 @@ class ModelSection:
     kv_cache_fraction: float = 0.85
     num_blocks: Optional[int] = None
     cuda_graphs: bool = False
+    weight_dtype: str = "auto"
+    weight_group: int = 64
 
 
 @dataclass
@@ -57,6 +64,7 @@ class WorkerSection:
 @dataclass
 class CacheSection:
     watermark: float = 0.01
+    dtype: str = "auto"
 
 
 @dataclass
@@ -113,6 +121,12 @@ class RuntimeConfig:
             raise RuntimeConfigError("model.max_context must be at least 2")
         if not 0.0 <= float(c.watermark) < 1.0:
             raise RuntimeConfigError("cache.watermark must be in [0, 1)")
+        if m.weight_dtype not in ("auto", "int4"):
+            raise RuntimeConfigError(f"model.weight_dtype `{m.weight_dtype}` is not one of auto, int4")
+        if m.weight_group not in (32, 64, 128):
+            raise RuntimeConfigError(f"model.weight_group {m.weight_group} is not one of 32, 64, 128")
+        if c.dtype not in ("auto", "fp8"):
+            raise RuntimeConfigError(f"cache.dtype `{c.dtype}` is not one of auto, fp8")
 
     def resolved_dtype(self) -> str:
         return "float32" if self.model.dtype in ("f32", "float32") else "bfloat16"

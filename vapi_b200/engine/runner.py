@@ -42,6 +42,17 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype `{name}` is not one of {sorted(DTYPES)}")
 
 
+def check_fewer_bits(kv_cache_dtype, weight_dtype, weight_group):
+    """(kv_cache_dtype, weight_dtype) of a program's options, refused where there is no such form."""
+    if kv_cache_dtype not in ("auto", "fp8"):
+        raise ValueError(f"kv_cache_dtype `{kv_cache_dtype}` is not one of auto, fp8")
+    if weight_dtype not in ("auto", "int4"):
+        raise ValueError(f"weight_dtype `{weight_dtype}` is not one of auto, int4")
+    if weight_group not in ops.INT4_GROUPS:
+        raise ValueError(f"weight_group {weight_group} is not one of {', '.join(map(str, ops.INT4_GROUPS))}")
+    return kv_cache_dtype, weight_dtype
+
+
 class ModelRunner:
     #: tokens per cache page (the reference's block is 32 tokens, crates/vapi-core/src/config.rs:15;
     #: 64 keeps a page of one kv head at 8 KB for head_dim 64 in bfloat16)
@@ -50,11 +61,20 @@ class ModelRunner:
     def __init__(self, plan: ModelPlan, tensors: Dict[str, torch.Tensor], *, dtype, device="cuda",
                  page_size: int = default_page_size, num_pages: Optional[int] = None, max_requests: int = 64,
                  max_batched_tokens: int = 8192, max_context: Optional[int] = None,
-                 watermark: float = 0.0, kv_cache_fraction: float = 0.85, validate: bool = True):
+                 watermark: float = 0.0, kv_cache_fraction: float = 0.85, validate: bool = True, kv_cache_dtype: str = "auto",
+                 weight_dtype: str = "auto", weight_group: int = 64):
         self.plan, self.dtype, self.device = plan, parse_dtype(dtype), torch.device(device)
         if self.device.type == "cuda":
             ops.strict_fp32()
+        #: keys and values "auto": in the activations' type; "fp8": e4m3 codes, a scale for each 16 tokens of a head.  The layers'
+        #: matrices "auto": in the activations' type; "int4": 4-bit codes, a scale and a zero for each ``weight_group`` columns of a row
+        self.kv_cache_dtype, self.weight_dtype = check_fewer_bits(kv_cache_dtype, weight_dtype, weight_group)
+        if self.kv_cache_dtype == "fp8":
+            for blk in plan.layers:
+                blk.mixer.use_cache8()
         plan.bind(tensors, self.dtype)
+        if self.weight_dtype == "int4":
+            plan.quantize4(int(weight_group))
         self.vocab_size = plan.vocab_size
         self.max_context = min(int(max_context or plan.max_positions), plan.max_positions)
         if num_pages is not None:            # no request can hold more tokens than the pool has
@@ -100,7 +120,9 @@ class ModelRunner:
         self._site_buffers = {s: self.cache.site_buffers(s) for s in set(flat)}
         #: whether every block has the stream form that steps of few rows run (blocks without it hand
         #: their output on in another shape than a plain delta, so such a model takes the ordinary path)
-        self._stream_form = all(hasattr(b, "forward_stream") for b in plan.layers) and not plan.stream_parts
+        #: (nor do 4-bit products take norms and adds along)
+        self._stream_form = (all(hasattr(b, "forward_stream") for b in plan.layers) and not plan.stream_parts
+                             and self.weight_dtype != "int4")
         #: numbers in the matrices of a layer, on average
         self._layer_numbers = sum(math.prod(s.shape) for b in plan.layers for s in b.tensor_specs("") if s.role == "matrix") // max(1, len(plan.layers))
         self._keep_embedding = any(getattr(p, "needs_embedding_output", False) for p in plan.stream_parts.values())
@@ -140,7 +162,7 @@ class ModelRunner:
         (crates/vapi-backend-candle/src/backend.rs:385-400) with the state slots taken off first."""
         from ..parts.base import PagedSpec, StateSpec
         esize = 4 if self.dtype == torch.float32 else 2
-        per_token = sum(s.elems_per_token() for _, s in sites if isinstance(s, PagedSpec)) * esize
+        per_page = sum(s.page_bytes(page_size, esize) for _, s in sites if isinstance(s, PagedSpec))
         per_req = 0
         for _, s in sites:
             if isinstance(s, StateSpec):
@@ -152,7 +174,7 @@ class ModelRunner:
             raise ValueError("num_pages must be given when the device is not CUDA")
         free, _ = torch.cuda.mem_get_info(self.device)
         budget = int(free * fraction) - per_req * (max_requests + 1)
-        pages = budget // max(per_token * page_size, 1) if per_token else max_requests
+        pages = budget // max(per_page, 1) if per_page else max_requests
         # never more than every request at full context could use
         cap = max_requests * -(-self.max_context // page_size)
         pages = min(int(pages), cap)
@@ -168,7 +190,7 @@ class ModelRunner:
             kind, gi = self.cache.site_kind(site)
             return CacheView(kind, self.cache.site_tensor(site), ctx.groups[gi] if kind == "paged" else None,
                              write=write, buffers=self._site_buffers[site] if kind == "paged" else None,
-                             spec=self.cache.site_spec(site))
+                             spec=self.cache.site_spec(site), exps=self.cache.site_exps(site))
 
         out = []
         for i, call in enumerate(self.plan.order):

@@ -103,6 +103,21 @@ class ModelPlan:
         for part in self.stream_parts.values():
             part.bind(tensors, "", dtype)
 
+    def quantize4(self, group: int) -> None:
+        """Take the layers' (bound) matrices as 4-bit ones with a scale and a zero for each ``group`` columns of a row; embedding and
+        output head stay as they are.  Refused, before anything is changed, by a model one of whose layers has no such form."""
+        for blk, pre in zip(self.layers, self.layer_prefixes):
+            if type(blk).quantize4 is Part.quantize4:
+                raise ValueError(f"{type(blk).__name__} ({pre or 'a layer'}) has no form with 4-bit weights")
+            for _, part in blk._parts():
+                if type(part).quantize4 is Part.quantize4:
+                    part.quantize4(group)            # (nothing to do, or its refusal)
+            for s in blk.tensor_specs(pre):
+                if s.role == "matrix" and s.shape[1] % group:
+                    raise ValueError(f"the {s.shape[1]} columns of {s.name} do not fall into groups of {group}")
+        for blk in self.layers:
+            blk.quantize4(group)
+
     # ---- caches --------------------------------------------------------------------
     def cache_sites(self) -> List[Tuple[object, object]]:
         """(site, spec) of every cache that a call site owns.  A site is the call site's index in the run

@@ -40,8 +40,11 @@ class GQAttention(Mixer):
     is normalised over the keys) and ``score_bias`` (a stored number per head is added to the score behind the cap).
     Any of these but the suffixes sends the mixer to the general kernels
     (``ops.qk_norm_rope_write_split``, ``ops.masked_attention``); the plain form keeps the
-    specialised ones.
+    specialised ones, and can keep its cache in 8 bits (:meth:`use_cache8`).
     """
+
+    #: whether keys and values are kept in 8 bits
+    cache8 = False
 
     def __init__(self, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int, *,
                  qk_norm_eps: Optional[float] = None, pos: Optional[str] = "rope",
@@ -106,7 +109,15 @@ class GQAttention(Mixer):
         # (for equal widths this is PagedSpec.kv: keys [nkv, page, d], then values [nkv, page, dv])
         # (kept first tokens are read for as long as the request lives: nothing is given back early)
         return PagedSpec((PagedBuffer("k", self.nkv, self.d), PagedBuffer("v", self.nkv, self.dv)),
-                         0 if self.keep_first > 0 else self.window)
+                         0 if self.keep_first > 0 else self.window, self.cache8)
+
+    def use_cache8(self):
+        if self.general:
+            raise ValueError("attention with unlike widths, a chunk, a sink, gates or another of its options has no form with a cache in 8 bits")
+        self.cache8 = True
+
+    def quantize4(self, group):
+        self.w_qkv, self.w_o = ops.int4_quantize(self.w_qkv, group), ops.int4_quantize(self.w_o, group)
 
     def tensor_specs(self, prefix: str) -> List[TensorSpec]:
         n, (h, nh, nkv, d), x = self.names, (self.hidden, self.nh, self.nkv, self.d), self.sfx
@@ -167,6 +178,8 @@ class GQAttention(Mixer):
             if self.chunk > 0:
                 keys = min(keys, self.chunk)
             return ops.masked_attention_splits(batch, 1, keys, self.nh, self.nkv)
+        if self.cache8:
+            return ops.attention8_splits(batch, 1, keys, self.nh, self.nkv, self.d)
         dec = ops.decode_attention_applies(dtype, self.d, page_size, self.nh // self.nkv)
         return ops.attention_splits(batch, 1, keys, self.nh, self.nkv, dec)
 
@@ -206,11 +219,22 @@ class GQAttention(Mixer):
         if self.general:
             return self._attend_general(qkv, ctx, cache, cos, sin)
         n_rep = nh // nkv
-        kv = cache.stacked() if cache.tensor is not None else None      # [pages, 2, n_kv, page_size, head_dim]
+        kv = None                                                       # [pages, 2, n_kv, page_size, head_dim]
+        if cache.tensor is not None:
+            kv = cache.stacked8() if self.cache8 else cache.stacked()
         splits = grp.splits if getattr(grp, "splits", None) is not None else ctx.attention_splits
         max_k = getattr(grp, "max_k", None) or ctx.max_k
         if self.window > 0:
             max_k = min(max_k, self.window + ctx.max_q - 1)      # a query reads at most `window` keys
+        eps = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0
+        if self.cache8:
+            if cache.write:
+                q = ops.qk_norm_rope_write8(qkv, nh, nkv, d, self.q_w, self.k_w, eps, cos, sin, self.rot_dim, kv, grp.slot_mapping, ctx.status)
+            else:
+                ops.qk_norm_rope_write(qkv, nh, nkv, d, self.q_w, self.k_w, eps, cos, sin, self.rot_dim, None, grp.slot_mapping, ctx.status)
+                q = qkv
+            return ops.paged_attention8(q, q.stride(0), kv, grp.block_table, ctx.cu_q, ctx.seqlens_k, ctx.n, ctx.num_seqs, ctx.max_q,
+                                        max_k, nh, nkv, d, self.scale, self.window, splits, ctx.status)
         if (ops.FUSED_DECODE_ROPE and qkv.is_cuda and kv is not None
                 and ops.decode_attention_fused_applies(qkv.dtype, d, kv.shape[3], ctx.max_q * n_rep,
                                                        self.rot_dim if cos is not None else None)

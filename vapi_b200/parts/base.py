@@ -71,10 +71,14 @@ class PagedSpec:
     ``window`` = 0 keeps every position; ``window`` = W > 0 means positions more than W
     behind the newest are never read again, so the manager may give their pages back.
     Layers with equal specs share one group: one pool of pages, one block table a request.
+
+    ``eight_bit``: the pages hold 8-bit codes, and beside them one exponent a row and block of 16 tokens
+    (:class:`vapi_b200.ops.Cache8`).
     """
 
     buffers: Tuple[PagedBuffer, ...]
     window: int = 0
+    eight_bit: bool = False
 
     @classmethod
     def kv(cls, n_kv: int, head_dim: int, window: int = 0) -> "PagedSpec":
@@ -88,6 +92,14 @@ class PagedSpec:
 
     def elems_per_token(self) -> int:
         return sum(b.rows * b.width for b in self.buffers)
+
+    def exps_per_block(self) -> int:
+        """Exponents that a block of 16 tokens has beside its codes."""
+        return sum(b.rows for b in self.buffers) if self.eight_bit else 0
+
+    def page_bytes(self, page_size: int, elem_size: int) -> int:
+        """Bytes of a page, whose elements have ``elem_size`` bytes unless they are codes."""
+        return page_size * self.elems_per_token() * (1 if self.eight_bit else elem_size) + page_size // 16 * self.exps_per_block()
 
     def uniform(self) -> bool:
         """Whether all buffers have one shape (so that they can be read as one stacked tensor)."""
@@ -133,6 +145,7 @@ class CacheView:
     spec: Any = None
     parts: Optional[List["CacheView"]] = None
     block: Optional["CacheView"] = None
+    exps: Optional[torch.Tensor] = None       # of pages of 8-bit codes: [pages, page_size / 16 * exponents per block]
 
     def stacked(self) -> torch.Tensor:
         """Buffers of one shape as a single tensor [pages, n_buffers, rows, page_size, width]."""
@@ -144,6 +157,12 @@ class CacheView:
         pages = self.tensor.shape[0]
         page_size = self.tensor.shape[1] // self.spec.elems_per_token()
         return self.tensor.view(pages, len(self.spec.buffers), b.rows, page_size, b.width)
+
+    def stacked8(self) -> "Any":
+        """Keys and values in 8 bits as the kernels take them, a :class:`vapi_b200.ops.Cache8`."""
+        from ..ops import Cache8
+        codes = self.stacked()
+        return Cache8(codes, self.exps.view(codes.shape[0], codes.shape[1], codes.shape[2], codes.shape[3] // 16))
 
 
 @dataclass
@@ -227,6 +246,12 @@ class Part:
         the embedding as ``cache``."""
         return None
 
+    def quantize4(self, group: int) -> None:
+        """Take the (bound) part's matrices as 4-bit ones with a scale and a zero for each ``group`` columns of a row.  A part
+        without matrices has nothing to do; one that has no such form refuses."""
+        if any(s.role == "matrix" for s in self.tensor_specs("")):
+            raise ValueError(f"{type(self).__name__} has no form with 4-bit weights")
+
 
 class Norm(Part):
     """A norm over the last dimension that also folds in the pending residual add."""
@@ -282,6 +307,13 @@ class Mixer(Part):
         fixed-shape (captured) decode step, whose kernels cannot follow the batch's real lengths;
         the answer comes back to the mixer as ``cache.group.splits``.  1: no cutting."""
         return 1
+
+    def use_cache8(self) -> None:
+        """Keep what the mixer caches per token in 8 bits (asked before the cache is laid out).  A mixer without pages has nothing
+        to do; one whose pages have no such form refuses."""
+        spec = self.cache_spec()
+        if any(isinstance(s, PagedSpec) for s in (spec if isinstance(spec, tuple) else (spec,))):
+            raise ValueError(f"{type(self).__name__} has no form with a cache in 8 bits")
 
     # A mixer of the form ``W_out inner(W_in a + b_in) + b_out`` may offer itself in pieces, so that a mixer made of
     # several can run all in-projections as one product and all out-projections as another:

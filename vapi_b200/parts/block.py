@@ -47,6 +47,10 @@ class PreNormBlock(Part):
         for key, part in self._parts():
             part.bind(tensors, prefix + self.sub[key], dtype)
 
+    def quantize4(self, group):
+        for _, part in self._parts():
+            part.quantize4(group)
+
     def forward(self, x: torch.Tensor, delta: Optional[torch.Tensor], ctx: Any,
                 cache: CacheView) -> torch.Tensor:
         a = self.mixer_norm.apply(x, delta, ctx.dtype)

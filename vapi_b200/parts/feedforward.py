@@ -50,6 +50,9 @@ class SwiGLU(FeedForward):
             self.b_gate_up = torch.cat([tensors[f"{prefix}{n['gate']}{self.bsfx}"], tensors[f"{prefix}{n['up']}{self.bsfx}"]], 0).contiguous()
             self.b_down = tensors[f"{prefix}{n['down']}{self.bsfx}"].contiguous()
 
+    def quantize4(self, group):
+        self.w_gate_up, self.w_down = ops.int4_quantize(self.w_gate_up, group), ops.int4_quantize(self.w_down, group)
+
     def forward(self, f: torch.Tensor, ctx: Any) -> torch.Tensor:
         if self.bias:
             return ops.linear(ops.swiglu(ops.linear(f, self.w_gate_up, self.b_gate_up), act=self.act), self.w_down, self.b_down)

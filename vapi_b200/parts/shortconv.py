@@ -57,6 +57,9 @@ class ShortConv(Mixer):
             self.b_conv = tensors[f"{prefix}{n['conv']}.bias"].contiguous()
             self.b_out = tensors[f"{prefix}{n['out']}.bias"].contiguous()
 
+    def quantize4(self, group):
+        self.w_in, self.w_out = ops.int4_quantize(self.w_in, group), ops.int4_quantize(self.w_out, group)
+
     def forward(self, a: torch.Tensor, ctx: Any, cache: CacheView) -> torch.Tensor:
         h3 = ops.linear(a, self.w_in)          # the in_proj bias is applied inside the kernel
         y = ops.shortconv(h3, self.b_in, self.taps, self.b_conv, cache.tensor, ctx.state_slots,

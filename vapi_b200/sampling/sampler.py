@@ -97,6 +97,7 @@ class TokenLogprobs:
     token: int
     logprob: float
     top: List[Tuple[int, float]]        # the k most likely tokens, most likely first, ties by lower id
+    entropy: Optional[float] = None     # of that distribution, in nats
 
 
 def row_logprobs(logits: np.ndarray, k: int):
@@ -113,6 +114,20 @@ def row_logprobs(logits: np.ndarray, k: int):
         order = np.lexsort((cand, -row[cand]))[:k]
         top = [(int(cand[i]), float(row[cand[i]]) - lse) for i in order]
     return lse, top
+
+
+def host_logprobs(logits: torch.Tensor, tokens: Sequence[int], k: int):
+    """What ``ops.token_logprobs`` gives, for rows on the host."""
+    chosen, entropies, ids, tops = [], [], [], []
+    for row, tok in zip(logits.to(torch.float32).numpy(), tokens):
+        lse, top = row_logprobs(row, k)
+        lp = row.astype(np.float64) - lse
+        chosen.append(float(row[tok]) - lse)
+        entropies.append(float(-(np.exp(lp[lp > -np.inf]) * lp[lp > -np.inf]).sum()))
+        ids.append([t for t, _ in top])
+        tops.append([v for _, v in top])
+    return (torch.tensor(chosen, dtype=torch.float64), torch.tensor(entropies, dtype=torch.float64), torch.tensor(ids, dtype=torch.int32),
+            torch.tensor(tops, dtype=torch.float64))
 
 
 @dataclass
@@ -146,8 +161,8 @@ class Sampler:
     @staticmethod
     def device_only(p: SamplingParams) -> bool:
         """Whether the host has nothing to do for a row with these parameters but read the
-        result: no penalties (their counts are uploaded each step) and no logprobs (the raw row
-        is read back)."""
+        result: no penalties (their counts are uploaded each step) and no logprobs (they are read
+        back beside the tokens)."""
         return not p.has_penalties and p.logprobs is None
 
     def _ring_entry(self, out: torch.Tensor):
@@ -243,20 +258,20 @@ class Sampler:
 
     def sample(self, logits: torch.Tensor, rows: Sequence[Tuple[SamplingParams, SamplerState]],
                out: Optional[torch.Tensor] = None, status_block: Optional[torch.Tensor] = None) -> List[int]:
-        """Tokens for the rows of a step, waiting for them: raw rows are read back for requests
-        that report logprobs, penalties are applied on the device, and every row is then decided
+        """Tokens for the rows of a step, waiting for them: for requests that report logprobs the
+        raw rows' are worked out on the device, penalties are applied on the device, and every row is then decided
         as :meth:`launch` decides it (logits on the host: by the host restatement).  ``out`` and
         ``status_block`` as for :meth:`launch`; the status word read is left in ``last_status``."""
         R = len(rows)
         assert logits.shape[0] >= R
         dev = logits.device
-        # rows that report log-probabilities: their raw logits, before any penalty touches them
-        raw: Dict[int, Tuple[float, List[Tuple[int, float]], np.ndarray]] = {}
-        for r, (p, _) in enumerate(rows):
-            if p.logprobs is not None:
-                row = logits[r].to(torch.float32).cpu().numpy()
-                lse, top = row_logprobs(row, p.logprobs)
-                raw[r] = (lse, top, row)
+        # rows that report log-probabilities: of the raw logits, before any penalty touches them
+        asked = [r for r, (p, _) in enumerate(rows) if p.logprobs is not None]
+        raw = None
+        if asked:
+            raw = logits[:R]
+            if any(p.has_penalties and st.counts for p, st in rows):
+                raw = raw.clone()
         extra_h2d = self._penalise(logits, rows, dev)
         if logits.is_cuda:
             if out is None or out.numel() < R:
@@ -264,13 +279,21 @@ class Sampler:
                     self._out = torch.zeros(max(self.max_rows, R), dtype=torch.int32, device=dev)
                 out, status_block = self._out, None
             pending = self.launch(logits, rows, out, status_block)
+            if asked:
+                lp = ops.token_logprobs(raw, out[:R], min(max(rows[r][0].logprobs for r in asked), raw.shape[1]))
             toks = self.finish(pending)
             self.last_status = pending.status
             self.h2d_bytes_last += extra_h2d
         else:
             toks = self._choose_on_host(logits, rows)
-        self.last_logprobs = [TokenLogprobs(toks[r], float(raw[r][2][toks[r]]) - raw[r][0], raw[r][1]) if r in raw else None
-                              for r in range(R)]
+            if asked:
+                lp = host_logprobs(raw, toks, max(rows[r][0].logprobs for r in asked))
+        self.last_logprobs = [None] * R
+        if asked:
+            chosen, entropy, ids, tops = (t.tolist() for t in lp)
+            for r in asked:
+                k = rows[r][0].logprobs
+                self.last_logprobs[r] = TokenLogprobs(toks[r], chosen[r], list(zip(ids[r][:k], tops[r][:k])), entropy[r])
         return toks
 
     def _penalise(self, logits: torch.Tensor, rows, dev) -> int:
