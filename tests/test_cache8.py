@@ -270,7 +270,7 @@ def _check_attention(c, got, scale, window=0, tensor_cores=True):
 
 
 LENGTHS = [([1], [1]), ([16, 17, 15], [1, 1, 1]), ([63, 64, 65, 1], [1, 1, 1, 1]), ([300, 5, 129], [1, 3, 2]), ([700], [1]), ([40, 33], [17, 33]),
-           ([200, 90, 1], [70, 0, 1])]
+           ([200, 90, 1], [70, 0, 1])]              # (forced onto the mma.sync kernel, portions too)
 
 
 @gpu
@@ -279,7 +279,36 @@ LENGTHS = [([1], [1]), ([16, 17, 15], [1, 1, 1]), ([63, 64, 65, 1], [1, 1, 1, 1]
 @pytest.mark.parametrize("window", [0, 1, 37])
 def test_attention_on_the_tensor_cores(lens, news, nh, nkv, d, page, window):
     c = _attention_case(lens, news, nh, nkv, d, page, torch.bfloat16, 7 * d + len(lens) + page)
-    _check_attention(c, _run_attention(c, d ** -0.5, window), d ** -0.5, window)
+    _check_attention(c, _run_attention(c, d ** -0.5, window, impl="tensor_core"), d ** -0.5, window)
+
+
+def _portion_check(c, got, scale, window):
+    """The tcgen05 kernel's P is bfloat16 (half a step 2^-8, once in the product and once against the sum of unrounded weights: twice)
+    and its values code * 2^e are exact; the rest as for the mma.sync kernel."""
+    want, spread, most = plain.attention(c["q"][:, :c["nh"] * c["d"]], plain.values(c["codes"], c["exps"]), c["table"], c["cu"], c["kl"], c["nh"], c["nkv"], c["d"],
+                                         scale, window)
+    weight = 2 * (most * (c["d"] / 16 + 6) * 2.0 ** -22 + 2.0 ** -20) + 2.0 ** -7
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    over = (got - want).abs() - (2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * weight * spread)
+    assert (over <= 0).all(), float(over.max())
+    # (and on average far nearer: rounding errors of both signs; a value left out or taken twice would not be)
+    assert (got - want).norm() <= 2.0 ** -7 * want.norm()
+
+
+PORTIONS = [([1], [1]), ([64], [64]), ([65], [65]), ([300], [129]), ([40, 33, 100], [17, 33, 1]), ([1000, 90, 700], [70, 0, 512]), ([190], [2])]
+
+
+@gpu
+@pytest.mark.parametrize("lens,news", PORTIONS)
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 64), (4, 4, 64, 16), (6, 2, 128, 64), (32, 2, 64, 48), (4, 1, 128, 16), (3, 1, 64, 128)])
+@pytest.mark.parametrize("window", [0, 1, 37])
+def test_portions_on_tcgen05(lens, news, nh, nkv, d, page, window):
+    c = _attention_case(lens, news, nh, nkv, d, page, torch.bfloat16, 11 * d + len(lens) + page)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _portion_check(c, _run_attention(c, d ** -0.5, window, impl="tcgen05", status=status), d ** -0.5, window)
+    _portion_check(c, _run_attention(c, d ** -0.5, window, status=status), d ** -0.5, window)
+    assert int(status) == 0
 
 
 @gpu
@@ -322,12 +351,15 @@ def test_queries_at_any_stride_and_place():
 
 @gpu
 def test_a_query_without_keys_gets_zeros_and_a_bad_page_a_status():
-    for d, impl in ((64, "auto"), (64, "general")):
+    for d, impl in ((64, "auto"), (64, "general"), (64, "tcgen05"), (128, "tcgen05")):
         c = _attention_case([40, 16, 20], [1, 1, 2], 4, 2, d, 16, torch.bfloat16, 1)
         c["kl"] = torch.tensor([40, 0, 1], dtype=torch.int32)           # the third request's first query lies before position 0
         got = _run_attention(c, 0.125, impl=impl)
         assert not got[1].any() and not got[2].any()
-        _check_attention(c, got, 0.125, tensor_cores=impl == "auto")
+        if impl == "tcgen05":
+            _portion_check(c, got, 0.125, 0)
+        else:
+            _check_attention(c, got, 0.125, tensor_cores=impl == "auto")
         status = torch.zeros(1, dtype=torch.int32, device="cuda")
         c["table"][0, 1] = 10 ** 6
         _run_attention(c, 0.125, impl=impl, status=status)

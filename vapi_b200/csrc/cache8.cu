@@ -14,6 +14,7 @@
 // one head are 16 * d bytes in one piece.
 #include "cache8.cuh"
 #include "cache8_decode.cuh"
+#include "cache8_prompt.cuh"
 
 using namespace vapi;
 
@@ -328,7 +329,11 @@ static int launch_attention8(const C8Params& p, const void* q, void* out, int nu
 }
 
 // q: [n, *] with `q_row_stride` elements between tokens, head h at h * d; out: [n, nh * d].
-// impl: 0 = the fastest kernel that applies; 1 = the general kernel; 2 = the tensor-core kernel, or an error.
+// impl: 0 = the fastest kernel that applies: for bfloat16 and head size 64 or 128 the tcgen05 kernel for steps with a portion of at least
+// P8_AUTO_MAX_Q tokens (in a step of several sequences for those of at least P8_MIN_Q, beside the mma.sync kernel for the others), the mma.sync
+// kernel for shorter ones; the general kernel for everything else.  1 = the general kernel; 2 = the mma.sync kernel, or an error;
+// 3 = the tcgen05 kernel for every sequence, or an error.
+constexpr int P8_AUTO_MAX_Q = 32;
 VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, const void* codes, const void* exps, int dtype, const int* block_table,
                                       int table_stride, const int* cu_q, const int* seqlens_k, void* out, int n, int num_seqs, int max_q,
                                       int max_k, int nh, int nkv, int d, int page_size, int num_pages, float scale, int window, int splits,
@@ -344,11 +349,21 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
     p.table_stride = table_stride; p.cu_q = cu_q; p.seqlens_k = seqlens_k; p.nh = nh; p.nkv = nkv; p.d = d; p.page_size = page_size;
     p.num_pages = num_pages; p.scale_log2e = scale * 1.4426950408889634f; p.window = window; p.status = status;
     const bool fast = dtype == VAPI_BF16 && (d == 64 || d == 128) && q_row_stride % 8 == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0;
-    if (impl == 2 && !fast)
-        return fail(-3, "paged_attention8: the tensor-core kernel needs bfloat16, head_dim 64 or 128 and 16-byte aligned rows (got dtype %d, head_dim %d)", dtype, d);
+    if (impl >= 2 && (!fast || (impl == 3 && !(scale > 0.f))))
+        return fail(-3, "paged_attention8: the tensor-core kernels need bfloat16, head_dim 64 or 128, 16-byte aligned rows and, for portions, a "
+                        "positive scale (got dtype %d, head_dim %d, scale %g)", dtype, d, (double)scale);
     if (fast && impl != 1) {
-        if (d == 64) return launch_decode8<64>(p, q, out, num_seqs, max_q, splits, stream);
-        return launch_decode8<128>(p, q, out, num_seqs, max_q, splits, stream);
+        if ((long long)num_pages * 2 * nkv * (page_size / C8_BLOCK) > 0x7fffffffLL)
+            return fail(-1, "paged_attention8: %d pages of %d tokens and %d kv heads are more blocks than an index holds", num_pages, page_size, nkv);
+        int rc = 0, most_q = 0x7fffffff;
+        if (impl == 3 || (impl == 0 && max_q >= P8_AUTO_MAX_Q && scale > 0.f)) {
+            const int min_q = impl == 3 || num_seqs == 1 ? 1 : P8_MIN_Q;
+            rc = d == 64 ? launch_prompt8<64>(p, q, out, n, num_seqs, max_q, min_q, stream) : launch_prompt8<128>(p, q, out, n, num_seqs, max_q, min_q, stream);
+            if (rc != 0 || min_q == 1) return rc;
+            most_q = min_q - 1;
+        }
+        return d == 64 ? launch_decode8<64>(p, q, out, num_seqs, max_q, splits, most_q, stream)
+                       : launch_decode8<128>(p, q, out, num_seqs, max_q, splits, most_q, stream);
     }
 #define VAPI_ATT8(T, DM) return launch_attention8<T, DM>(p, q, out, num_seqs, max_q, stream)
     if (dtype == VAPI_F32) {

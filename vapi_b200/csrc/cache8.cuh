@@ -19,6 +19,13 @@ struct C8Params {
     int* status;
 };
 
+// The exponents of the block of keys at `where` and of its values, a byte each.  (From L2: the line may have been read before the
+// kernel that wrote this step's blocks had ended.)
+__device__ __forceinline__ int c8_scales(const C8Params& p, int where, int per_head) {
+    const unsigned char* e = reinterpret_cast<const unsigned char*>(p.exps);
+    return (int)__ldcg(e + where) | (int)__ldcg(e + where + p.nkv * per_head) << 8;
+}
+
 // 2^e for e in -126 .. 127
 __device__ __forceinline__ float c8_power(int e) { return __int_as_float((e + 127) << 23); }
 

@@ -63,7 +63,7 @@ __device__ __forceinline__ uint2 d8_lds8(unsigned addr) {
 // WIDE: tiles of 16 rows; else of 8 (the lower half of every fragment is then zero and is not worked out).
 template <int HD, bool WIDE>
 __global__ void __launch_bounds__(D8_WARPS * 32, 2)
-decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int splits) {
+decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int splits, const int most_q) {
     constexpr int ROWS = WIDE ? 16 : 8, H = WIDE ? 2 : 1, STAGES = D8_STAGES<HD>, CHUNK = D8_CHUNK<HD>;
     constexpr int KS = HD / 16, NT = HD / 8, Q64 = HD / 64;                 // k-steps of S, column tiles of O, runs of 64 elements
     extern __shared__ __align__(128) unsigned char d8_smem[];
@@ -79,7 +79,7 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     // index data was copied from the host before the step's first kernel: safe before the wait
     const int q0 = p.cu_q[s], qlen = p.cu_q[s + 1] - q0, klen = p.seqlens_k[s];
     const int n_rep = p.nh / p.nkv, rows_total = qlen * n_rep, r0 = tile * ROWS;
-    if (r0 >= rows_total) {                                                 // (the same for the whole cluster)
+    if (r0 >= rows_total || qlen > most_q) {                                // longer portions are another kernel's (the same for the whole cluster)
         pdl_wait();
         return;
     }
@@ -115,7 +115,7 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             page = 0;
         }
         where = (page * 2 * p.nkv + g) * per_head + key % p.page_size / C8_BLOCK;
-        scales_next = (unsigned char)p.exps[where] | (int)(unsigned char)p.exps[where + p.nkv * per_head] << 8;
+        scales_next = c8_scales(p, where, per_head);
     };
     auto bring = [&](int it) {                                              // chunk begin + it into its place of the ring
         if ((it & 31) == 0) look_up(it);
@@ -389,7 +389,7 @@ static int decode8_slots() {
 }
 
 template <int HD, bool WIDE>
-static int launch_decode8_of(const C8Params& p, const void* q, void* out, int num_seqs, long long rows, int splits, cudaStream_t stream) {
+static int launch_decode8_of(const C8Params& p, const void* q, void* out, int num_seqs, long long rows, int splits, int most_q, cudaStream_t stream) {
     const int rc = decode8_ready<HD, WIDE>();
     if (rc != 0) return rc;
     const long long tiles = (rows + (WIDE ? 15 : 7)) / (WIDE ? 16 : 8);
@@ -408,18 +408,17 @@ static int launch_decode8_of(const C8Params& p, const void* q, void* out, int nu
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return check_launch("paged_attention8", cudaLaunchKernelEx(&cfg, decode8_kernel<HD, WIDE>, p, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, splits));
+    return check_launch("paged_attention8", cudaLaunchKernelEx(&cfg, decode8_kernel<HD, WIDE>, p, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, splits, most_q));
 }
 
 template <int HD>
-static int launch_decode8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int splits, cudaStream_t stream) {
+// sequences that bring more than `most_q` tokens are left alone
+static int launch_decode8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int splits, int most_q, cudaStream_t stream) {
     if (splits < 1) splits = 1;
     if (splits > D8_MAX_CLUSTER) return fail(-1, "paged_attention8: %d splits are more than %d", splits, D8_MAX_CLUSTER);
-    if ((long long)p.num_pages * 2 * p.nkv * (p.page_size / C8_BLOCK) > 0x7fffffffLL)
-        return fail(-1, "paged_attention8: %d pages of %d tokens and %d kv heads are more blocks than an index holds", p.num_pages, p.page_size, p.nkv);
-    const long long rows = (long long)max_q * (p.nh / p.nkv);
-    if (rows <= 8) return launch_decode8_of<HD, false>(p, q, out, num_seqs, rows, splits, stream);
-    return launch_decode8_of<HD, true>(p, q, out, num_seqs, rows, splits, stream);
+    const long long rows = (long long)(max_q < most_q ? max_q : most_q) * (p.nh / p.nkv);
+    if (rows <= 8) return launch_decode8_of<HD, false>(p, q, out, num_seqs, rows, splits, most_q, stream);
+    return launch_decode8_of<HD, true>(p, q, out, num_seqs, rows, splits, most_q, stream);
 }
 
 }  // namespace vapi

@@ -1,0 +1,406 @@
+// Attention of prompt portions over an 8-bit cache on the fifth-generation tensor cores (tcgen05): bfloat16 queries, head size 64
+// or 128, sequences that bring at least `min_q` tokens to the step (shorter ones are decode8_kernel's).
+//
+// A block owns 128 rows (query token, q head of the group) of one (sequence, kv head) and walks the key tiles, 64 keys each, that any
+// of them can see:
+//   warp 0 (one lane)  issues S = Q K^T into one of two tensor-memory buffers and O += P V into a third; owns the allocation;
+//   warps 1..3         bring the codes of a tile into registers while the tile before is worked on, and write it to a ring of
+//                      shared-memory stages as 16-bit numbers;
+//   warps 4..7         softmax, one row a thread, as the 16-bit kernel does it (attention_tc.cuh): the running maximum only moves
+//                      when a tile exceeds it by more than 2^8, so O is rescaled a few times a row.
+//
+//   K: a code is an f16 number; Q's rows are f16 too, each scaled by a power of two so that its largest element is near 2^14 (as in
+//      cache8_decode.cuh).  The scale of a block of 16 keys multiplies 16 columns of S, where a score is multiplied by something
+//      anyway: it costs nothing.
+//   V: O is one sum over all tiles, so V must be on one scale; code * 2^e is a bfloat16 number exactly, and P is bfloat16 as in
+//      the 16-bit kernel.
+//
+// Keys behind the last that a row of the block sees are masked by selection, and their values written as zeros.  Every wait is bounded; a role that
+// gives up records status 16 and the block drains (tensor memory is released on every path).
+#pragma once
+#include "cache8.cuh"
+#include "attention_tc.cuh"        // ft_tile
+
+namespace vapi {
+
+constexpr int P8_ROWS = 128, P8_KEYS = 64, P8_THREADS = 256, P8_LOADERS = 96;
+constexpr int P8_MIN_Q = 32;                       // in a step of several sequences, those with fewer tokens go to decode8_kernel
+template <int HD> constexpr int P8_STAGES = HD == 64 ? 3 : 2;
+template <int HD> constexpr int P8_TILE = P8_KEYS * HD * 2;                                  // bytes of K (or V) of a tile
+template <int HD> constexpr size_t P8_SMEM = 1024 + P8_ROWS * HD * 2 + 2 * P8_ROWS * P8_KEYS * 2 + (size_t)P8_STAGES<HD> * 2 * P8_TILE<HD> + 512;
+constexpr int P8_TMEM_COLS = 256;                  // S0 | S1 | O, 64 + 64 + HD columns
+
+// 16 codes as 16 halves
+__device__ __forceinline__ void p8_halves(const uint4& c, uint4& lo, uint4& hi) {
+    const unsigned w[4] = {c.x, c.y, c.z, c.w};
+    unsigned h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[2 * i] = c8_halves((unsigned short)(w[i] & 0xffffu));
+        h[2 * i + 1] = c8_halves((unsigned short)(w[i] >> 16));
+    }
+    lo = make_uint4(h[0], h[1], h[2], h[3]);
+    hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+// 16 codes times f as 16 bfloat16
+__device__ __forceinline__ void p8_numbers(const uint4& c, float f, uint4& lo, uint4& hi) {
+    const unsigned w[4] = {c.x, c.y, c.z, c.w};
+    unsigned h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 v = c8_floats(w[i]);
+        h[2 * i] = pack_bf16(v.x * f, v.y * f);
+        h[2 * i + 1] = pack_bf16(v.z * f, v.w * f);
+    }
+    lo = make_uint4(h[0], h[1], h[2], h[3]);
+    hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(P8_THREADS, HD == 64 ? 2 : 1)
+prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int num_seqs, const int min_q) {
+    constexpr int STAGES = P8_STAGES<HD>, TILE = P8_TILE<HD>, ATOMS = HD / 64, ATOM = P8_KEYS * 128;     // 64 elements of 64 keys
+    extern __shared__ unsigned char p8_smem[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p8_smem) + 1023) & ~(uintptr_t)1023);
+    unsigned char* sQ = base;                                   // [atom][128 rows][128 B], 128-byte swizzle
+    unsigned char* sP = base + P8_ROWS * HD * 2;                // two buffers [128 rows][128 B]
+    unsigned char* sKV = sP + 2 * P8_ROWS * P8_KEYS * 2;        // [stage][K | V][atom][64 keys][128 B]
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sKV + (size_t)STAGES * 2 * TILE);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 16);
+    int* flags = reinterpret_cast<int*>(tmem_slot + 1);
+    float* sE = reinterpret_cast<float*>(tmem_slot + 4);        // [stage][4]: the scales of the tile's blocks of keys
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = (int)blockIdx.x % p.nkv, n_rep = p.nh / p.nkv;
+    pdl_trigger();
+    // index data was copied from the host before the step's first kernel: safe before the wait
+    int s = 0, tile = 0;
+    if (!ft_tile(p.cu_q, num_seqs, min_q, n_rep, P8_ROWS, (int)blockIdx.x / p.nkv, s, tile)) {
+        pdl_wait();
+        return;
+    }
+    const int q0 = p.cu_q[s], qlen = p.cu_q[s + 1] - q0, klen = p.seqlens_k[s];
+    const int rows_total = qlen * n_rep, tile_start = tile * P8_ROWS;
+    const int last_row = min(rows_total, tile_start + P8_ROWS) - 1;
+    const int base_pos = klen - qlen;
+    const int p_min = base_pos + tile_start / n_rep, p_max = base_pos + last_row / n_rep;
+    const int key_lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
+    const int kt_lo = key_lo / P8_KEYS;
+    const int nt = p_max < key_lo ? 0 : p_max / P8_KEYS - kt_lo + 1;
+
+    const unsigned kv_full = smem_u32(bars), kv_empty = smem_u32(bars + STAGES);
+    const unsigned s_full = smem_u32(bars + 2 * STAGES), s_free = smem_u32(bars + 2 * STAGES + 2);
+    const unsigned p_ready = smem_u32(bars + 2 * STAGES + 4), pv_done = smem_u32(bars + 2 * STAGES + 6);
+    const unsigned q_ready = smem_u32(bars + 2 * STAGES + 8);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(kv_full + 8 * i, P8_LOADERS); mbar_init(kv_empty + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(s_free + 8 * i, 128);
+            mbar_init(p_ready + 8 * i, 128);
+            mbar_init(pv_done + 8 * i, 1);
+        }
+        mbar_init(q_ready, 128);
+        flags[0] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((unsigned)P8_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const unsigned tmem_base = *tmem_slot, tS0 = tmem_base, tO = tmem_base + 128;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // instruction descriptors: float accumulate, N = 64, M = 128; f16 x f16, both K-major, and bf16 x bf16 with V's
+            // contiguous dimension N
+            const unsigned shape = (1u << 4) | ((unsigned)(P8_KEYS >> 3) << 17) | ((unsigned)(P8_ROWS >> 4) << 24);
+            const unsigned idesc_s = shape, idesc_o = shape | (1u << 7) | (1u << 10) | (1u << 16);
+            bool ok = true;
+            auto pv = [&](int j) {          // O += P(j) . V(j)
+                if (!ok) return;
+                if (!mbar_wait(p_ready + 8 * (j & 1), (j >> 1) & 1)) { ok = false; return; }
+                tc5_fence_after();
+                const int stage = j % STAGES;
+                const unsigned pa = smem_u32(sP + (j & 1) * P8_ROWS * P8_KEYS * 2);
+                const unsigned vb = smem_u32(sKV + (size_t)stage * 2 * TILE) + TILE;
+#pragma unroll
+                for (int a = 0; a < ATOMS; ++a)
+#pragma unroll
+                    for (int k = 0; k < P8_KEYS / 16; ++k)
+                        umma_f16(tO + a * 64, umma_desc(pa + k * 32), umma_desc_mn(vb + a * ATOM + k * 16 * 128), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                umma_commit(pv_done + 8 * (j & 1));
+                umma_commit(kv_empty + 8 * stage);
+            };
+            for (int i = 0; i < nt && ok; ++i) {
+                const int stage = i % STAGES, sb = i & 1;
+                if (!mbar_wait(kv_full + 8 * stage, (i / STAGES) & 1)) { ok = false; break; }
+                if (i >= 2 && !mbar_wait(s_free + 8 * sb, ((i >> 1) - 1) & 1)) { ok = false; break; }
+                if (i == 0 && !mbar_wait(q_ready, 0)) { ok = false; break; }
+                tc5_fence_after();
+                const unsigned qa = smem_u32(sQ), kb = smem_u32(sKV + (size_t)stage * 2 * TILE);
+#pragma unroll
+                for (int a = 0; a < ATOMS; ++a)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_f16(tS0 + sb * 64, umma_desc(qa + a * P8_ROWS * 128 + k * 32), umma_desc(kb + a * ATOM + k * 32), idesc_s, (a > 0 || k > 0) ? 1u : 0u);
+                umma_commit(s_full + 8 * sb);
+                if (i >= 1) pv(i - 1);
+            }
+            if (nt > 0) pv(nt - 1);
+            if (!ok) flags[0] = 1;
+        }
+    } else if (warp < 4) {
+        // ---- codes to numbers ----
+        const int t = threadIdx.x - 32;
+        constexpr int PER = 2 * P8_KEYS * HD / 16, EACH = (PER + P8_LOADERS - 1) / P8_LOADERS;       // 16-byte pieces of a tile, a thread
+        const int* bt = p.block_table + (size_t)s * p.table_stride;
+        const int per_head = p.page_size / C8_BLOCK;
+        bool waited = false;
+        // lane b < 4: where block b of a tile lies, and its scales
+        auto find = [&](int i) {
+            int at = 0;
+            if (lane < 4 && i < nt) {
+                const int key = (kt_lo + i) * P8_KEYS + lane * C8_BLOCK;
+                if (key <= p_max) {                             // (blocks behind the last key that is seen: the first block's place, and masked)
+                    int page = bt[key / p.page_size];
+                    if (page < 0 || page >= p.num_pages) {
+                        if (p.status) atomicExch(p.status, 4);
+                        page = 0;
+                    }
+                    at = (page * 2 * p.nkv + g) * per_head + key % p.page_size / C8_BLOCK;
+                }
+            }
+            return at;
+        };
+        uint4 codes[EACH];
+        int exps = 0;
+        auto load = [&](int i, int where) {                      // tile i, whose blocks lie at `where`
+            // a tile that reaches into this step's keys was written by the kernel before this one (and the block they begin in)
+            if (!waited && (kt_lo + i) * P8_KEYS + P8_KEYS > (base_pos < 0 ? 0 : base_pos / C8_BLOCK * C8_BLOCK)) { pdl_wait(); waited = true; }
+            if (lane < 4) exps = c8_scales(p, where, per_head);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                const int piece = t + j * P8_LOADERS;
+                const int kind = piece / (PER / 2), r = piece % (PER / 2) / (HD / 16), c = piece % (HD / 16);
+                const int block = __shfl_sync(0xffffffffu, where, r / C8_BLOCK);
+                if (piece < PER)
+                    codes[j] = __ldcg(reinterpret_cast<const uint4*>(p.codes + ((size_t)block + (kind ? (size_t)p.nkv * per_head : 0)) * C8_BLOCK * HD +
+                                                                    (r & (C8_BLOCK - 1)) * HD) + c);
+            }
+        };
+        int next = find(0), later = find(1);
+        if (nt > 0) load(0, next);
+        for (int i = 0; i < nt; ++i) {
+            const int stage = i % STAGES, k0 = (kt_lo + i) * P8_KEYS;
+            if (!__all_sync(0xffffffffu, i < STAGES || mbar_wait(kv_empty + 8 * stage, ((i / STAGES) - 1) & 1))) { flags[0] = 1; break; }
+            unsigned char* dst = sKV + (size_t)stage * 2 * TILE;
+            if (t < 4) sE[stage * 4 + t] = c8_power((int)(signed char)(exps & 0xff));
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                const int piece = t + j * P8_LOADERS;
+                const int kind = piece / (PER / 2), r = piece % (PER / 2) / (HD / 16), c = piece % (HD / 16);
+                const int e = (int)(signed char)(__shfl_sync(0xffffffffu, exps, r / C8_BLOCK) >> 8 & 0xff);
+                if (piece >= PER) continue;
+                uint4 lo, hi;
+                if (kind == 0) {
+                    p8_halves(codes[j], lo, hi);
+                } else if (k0 + r <= p_max) {                   // (what no row sees may be anything)
+                    p8_numbers(codes[j], c8_power(e), lo, hi);
+                } else {
+                    lo = hi = make_uint4(0u, 0u, 0u, 0u);
+                }
+                unsigned char* row = dst + kind * TILE + (c >> 2) * ATOM + r * 128;
+                const int ch = 2 * (c & 3);
+                *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = lo;
+                *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = hi;
+            }
+            fence_proxy_async();
+            mbar_arrive(kv_full + 8 * stage);
+            if (i + 1 < nt) {
+                next = later;
+                later = find(i + 2);
+                load(i + 1, next);
+            }
+        }
+        if (!waited) pdl_wait();
+    } else {
+        // ---- softmax and epilogue: one row per thread ----
+        const int quarter = warp & 3;                               // the tensor-memory lanes this warp may touch
+        const int row = quarter * 32 + lane;
+        const unsigned lane_addr = (unsigned)(quarter * 32) << 16;
+        const int rr = tile_start + row;
+        const bool row_ok = rr < rows_total;
+        const int tok = row_ok ? rr / n_rep : 0;
+        const int head = g * n_rep + (row_ok ? rr - tok * n_rep : 0);
+        const int pos = row_ok ? base_pos + tok : -1;               // -1: sees nothing
+        pdl_wait();                                                 // q comes from the kernel before this one
+        float row_f;
+        {
+            const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(q0 + tok) * p.q_row_stride + (size_t)head * HD);
+            float big = 0.f;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                const uint4 v = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+            }
+            const int x = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120);
+            const float up = c8_power(14 - x);
+            row_f = c8_power(x - 14) * p.scale_log2e;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                const uint4 v = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                unsigned h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = d8_half2(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
+                *reinterpret_cast<uint4*>(sQ + (c >> 3) * P8_ROWS * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            fence_proxy_async();
+            mbar_arrive(q_ready);
+        }
+        float m_run = -INFINITY, l_run = 0.f;
+        bool ok = true;
+        for (int i = 0; i < nt && ok; ++i) {
+            const int sb = i & 1, stage = i % STAGES;
+            const int k0 = (kt_lo + i) * P8_KEYS;
+            // (a wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide instructions)
+            if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, (i >> 1) & 1))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (i / STAGES) & 1))) { ok = false; break; }     // complete already: makes the scales visible here
+            tc5_fence_after();
+            float sv[P8_KEYS];
+            {
+                unsigned raw[P8_KEYS / 16][16];                     // all four loads in flight, one wait
+#pragma unroll
+                for (int j = 0; j < P8_KEYS / 16; ++j) tmem_ld16_nowait(tS0 + sb * 64 + lane_addr + j * 16, raw[j]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < P8_KEYS / 16; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sv[j * 16 + e] = __uint_as_float(raw[j][e]);
+            }
+            tc5_fence_before();
+            mbar_arrive(s_free + 8 * sb);                           // the scores are in registers
+            const float4 ek = *reinterpret_cast<const float4*>(sE + stage * 4);
+            // (kept above zero: a masked score is -inf before it is multiplied)
+            const float f[4] = {fmaxf(ek.x * row_f, 1.2e-38f), fmaxf(ek.y * row_f, 1.2e-38f), fmaxf(ek.z * row_f, 1.2e-38f), fmaxf(ek.w * row_f, 1.2e-38f)};
+
+            const bool need_mask = (k0 + P8_KEYS - 1 > p_min) || (p.window > 0 && k0 <= p_max - p.window);
+            if (need_mask) {
+#pragma unroll
+                for (int e = 0; e < P8_KEYS; ++e) {
+                    const int kj = k0 + e;
+                    const bool vis = kj <= pos && kj < klen && (p.window <= 0 || kj > pos - p.window);
+                    sv[e] = vis ? sv[e] : -INFINITY;
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {                           // (four chains: a single one would leave the warps waiting on latency)
+                float m4 = sv[16 * b];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) m4 = fmaxf(m4, sv[16 * b + e]);
+                mx = fmaxf(mx, m4 * f[b]);                          // (the scales are positive)
+            }
+            const bool grow = mx > m_run + FT_RAISE;                // also the first tile with a visible key
+            const float m_new = grow ? mx : m_run;
+            const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;         // m_run = -inf: 0
+            if (i >= 1 && __any_sync(0xffffffffu, grow)) {
+                // the accumulator must be at rest: P.V of the tile before this one has completed
+                if (!__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1))) { ok = false; break; }
+                tc5_fence_after();
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    float o16[16];
+                    tmem_ld16(tO + lane_addr + j * 16, o16);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o16[e] *= alpha;
+                    tmem_st16(tO + lane_addr + j * 16, o16);
+                }
+                tmem_st_wait();
+            }
+            l_run *= alpha;
+            m_run = m_new;
+            const float m_use = m_run == -INFINITY ? 0.f : m_run;
+            // this tile's P buffer was last read by P.V of the tile two before
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
+            const float2 mu2 = make_float2(-m_use, -m_use);
+            float rs4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                unsigned w[4];
+                const float2 f2 = make_float2(f[c >> 1], f[c >> 1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float2 x = __ffma2_rn(make_float2(sv[c * 8 + 2 * e], sv[c * 8 + 2 * e + 1]), f2, mu2);
+                    x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    rs4[e] += x.x + x.y;
+                    w[e] = pack_bf16(x.x, x.y);
+                }
+                *reinterpret_cast<uint4*>(sP + sb * P8_ROWS * P8_KEYS * 2 + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            l_run += (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
+            fence_proxy_async();
+            tc5_fence_before();
+            mbar_arrive(p_ready + 8 * sb);
+        }
+        if (ok && nt > 0 && !__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * ((nt - 1) & 1), ((nt - 1) >> 1) & 1))) ok = false;
+        tc5_fence_after();
+        if (ok) {                                                   // (uniform over the warp)
+            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;     // a row that sees nothing: zeros
+            __nv_bfloat16* o = out + ((size_t)(q0 + tok) * p.nh + head) * HD;
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+                float o16[16];
+                if (nt > 0) {
+                    tmem_ld16(tO + lane_addr + j * 16, o16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o16[e] = 0.f;
+                }
+                unsigned w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = inv == 0.f ? 0u : pack_bf16(o16[2 * e] * inv, o16[2 * e + 1] * inv);
+                if (row_ok) {
+                    *reinterpret_cast<uint4*>(o + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(o + j * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+            }
+        }
+        if (!ok) flags[0] = 1;
+    }
+    tc5_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && flags[0] && p.status) atomicExch(p.status, 16);
+    if (warp == 0) {
+        tc5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((unsigned)P8_TMEM_COLS) : "memory");
+    }
+}
+
+template <int HD>
+static int launch_prompt8(const C8Params& p, const void* q, void* out, int n, int num_seqs, int max_q, int min_q, cudaStream_t stream) {
+    static int ready[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "paged_attention8: cannot tell the current device");
+    if (!ready[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(prompt8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P8_SMEM<HD>);
+        if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", P8_SMEM<HD>, cudaGetErrorString(e));
+        ready[dev] = 1;
+    }
+    // tiles of all sequences together: at most those of n tokens in one piece and a ragged one a sequence of at least min_q tokens
+    const int n_rep = p.nh / p.nkv;
+    const long long longest = ((long long)max_q * n_rep + P8_ROWS - 1) / P8_ROWS, most = n / min_q < num_seqs ? n / min_q : num_seqs;
+    const long long whole = (long long)n * n_rep / P8_ROWS + most, tiles = longest * most < whole ? longest * most : whole;
+    if (tiles == 0) return 0;
+    if (tiles * p.nkv > 0x7fffffffLL) return fail(-1, "paged_attention8: the step exceeds the grid (%lld row tiles, %d kv heads)", tiles, p.nkv);
+    return check_launch("paged_attention8 (tcgen05)", launch(prompt8_kernel<HD>, dim3((unsigned)(tiles * p.nkv)), P8_THREADS, P8_SMEM<HD>, stream, p,
+                                                             (const __nv_bfloat16*)q, (__nv_bfloat16*)out, num_seqs, min_q));
+}
+
+}  // namespace vapi

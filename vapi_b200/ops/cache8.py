@@ -113,7 +113,9 @@ def attention8_splits(num_seqs: int, max_q: int, max_k: int, nh: int, nkv: int, 
     return splits
 
 
-_IMPL8 = {"auto": 0, "general": 1, "tensor_core": 2}
+_IMPL8 = {"auto": 0, "general": 1, "tensor_core": 2, "tcgen05": 3}
+#: steps whose longest portion has at least this many tokens go to the tcgen05 kernel (the library's own rule, restated)
+PORTION8_MIN_Q = 32
 
 
 def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_table: torch.Tensor, cu_q: torch.Tensor,
@@ -123,8 +125,10 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     """:func:`paged_attention` over a cache in 8 bits; returns [n, nh*d].  Arguments as there; the numbers of the cache are taken
     exactly, scores, softmax and sums are float32.  A query without a visible key gets zeros.
 
-    ``impl``: "tensor_core" forces the kernels for bfloat16 and head size 64 or 128, "general" the one that takes every type,
-    head size (a multiple of 16 up to 256) and page size (a multiple of 16); "auto" picks."""
+    ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions of 32 tokens or more, and the
+    mma.sync kernel, whose ``splits`` (up to 16) blocks share the keys as a cluster, for the others; the general kernel for every other
+    type, head size (a multiple of 16 up to 256) and alignment.  "tcgen05", "tensor_core" and "general" force one (the first two raise where
+    they do not apply)."""
     for t, w in ((block_table, "block table"), (cu_q, "cu_q"), (seqlens_k, "seqlens_k")):
         _i32(t, w)
     if impl not in _IMPL8:
@@ -142,11 +146,12 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     pages, page_size = _cache8(cache, nkv, d)
     _cuda(q, cache.codes, cache.exps, block_table, cu_q, seqlens_k)
     _here(q, cache.codes, cache.exps, block_table, cu_q, seqlens_k)
+    two = max_q >= PORTION8_MIN_Q and num_seqs > 1 and impl == "auto" and q.dtype == torch.bfloat16 and d in (64, 128)
     if splits is None:
-        splits = attention8_splits(num_seqs, max_q, max_k, nh, nkv, d)
+        splits = attention8_splits(num_seqs, 1 if two else max_q, max_k, nh, nkv, d)
     out = torch.empty((n, nh * d), dtype=q.dtype, device=q.device)
     lib = _lib("cache8")
     _check(lib, lib.vapi_paged_attention8(_p(q), q_row_stride, _p(cache.codes), _p(cache.exps), _dt(q), _p(block_table), block_table.stride(0),
                                           _p(cu_q), _p(seqlens_k), _p(out), n, num_seqs, max_q, max_k, nh, nkv, d, page_size, pages,
-                                          scale, window, splits, _IMPL8[impl], _p(status), _stream()), launches=int(n > 0))
+                                          scale, window, splits, _IMPL8[impl], _p(status), _stream()), launches=(2 if two else 1) if n > 0 else 0)
     return out
