@@ -328,11 +328,22 @@ static int launch_attention8(const C8Params& p, const void* q, void* out, int nu
     return check_launch("paged_attention8", launch(kern, dim3((unsigned)tiles, p.nkv, num_seqs), G8_WARPS * 32, smem, stream, p, (const T*)q, (T*)out));
 }
 
+// How many blocks of the mma.sync kernel share the keys of one (sequence, kv head, tile of rows): a power of two up to a cluster's 16, while all
+// blocks are on the device at once and each of a block's eight warps still has two blocks of 16 tokens.
+static int c8_splits(int num_seqs, int max_q, int max_k, int nh, int nkv, int d) {
+    if (num_seqs <= 0 || max_q <= 0 || nkv <= 0) return 1;
+    const long long rows = (long long)max_q * (nh / nkv), blocks = (long long)num_seqs * nkv * ((rows + (rows <= 8 ? 7 : 15)) / (rows <= 8 ? 8 : 16));
+    const long long slots = d == 64 ? decode8_slots<64>() : decode8_slots<128>();
+    int splits = 1;
+    while (splits < D8_MAX_CLUSTER && 2 * splits * blocks <= slots && 2LL * splits * 256 <= max_k) splits *= 2;
+    return splits;
+}
+
 // q: [n, *] with `q_row_stride` elements between tokens, head h at h * d; out: [n, nh * d].
 // impl: 0 = the fastest kernel that applies: for bfloat16 and head size 64 or 128 the tcgen05 kernel for steps with a portion of at least
 // P8_AUTO_MAX_Q tokens (in a step of several sequences for those of at least P8_MIN_Q, beside the mma.sync kernel for the others), the mma.sync
 // kernel for shorter ones; the general kernel for everything else.  1 = the general kernel; 2 = the mma.sync kernel, or an error;
-// 3 = the tcgen05 kernel for every sequence, or an error.
+// 3 = the tcgen05 kernel for every sequence, or an error.  splits 0: as many as pay (max_k: the most keys a sequence has).
 constexpr int P8_AUTO_MAX_Q = 32;
 VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, const void* codes, const void* exps, int dtype, const int* block_table,
                                       int table_stride, const int* cu_q, const int* seqlens_k, void* out, int n, int num_seqs, int max_q,
@@ -362,6 +373,7 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
             if (rc != 0 || min_q == 1) return rc;
             most_q = min_q - 1;
         }
+        if (splits <= 0) splits = c8_splits(num_seqs, most_q < max_q ? 1 : max_q, max_k, nh, nkv, d);      // (beside a portion: as for single tokens)
         return d == 64 ? launch_decode8<64>(p, q, out, num_seqs, max_q, splits, most_q, stream)
                        : launch_decode8<128>(p, q, out, num_seqs, max_q, splits, most_q, stream);
     }
@@ -376,5 +388,5 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
     return fail(-2, "paged_attention8: unsupported dtype %d", dtype);
 }
 
-VAPI_EXPORT int vapi_attention8_slots(int d) { return d == 64 ? decode8_slots<64>() : decode8_slots<128>(); }
+VAPI_EXPORT int vapi_attention8_splits(int num_seqs, int max_q, int max_k, int nh, int nkv, int d) { return c8_splits(num_seqs, max_q, max_k, nh, nkv, d); }
 VAPI_EXPORT const char* vapi_last_error() { return error_buffer(); }

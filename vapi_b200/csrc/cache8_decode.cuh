@@ -379,11 +379,12 @@ static int decode8_ready() {
 // blocks of the kernel that the device holds at a time
 template <int HD>
 static int decode8_slots() {
-    int per_sm = 0;
-    if (decode8_ready<HD, false>() != 0 ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode8_kernel<HD, false>, D8_WARPS * 32, D8_SMEM<HD>) != cudaSuccess) {
+    static int per_sm = 0;                         // (the same on every device that the kernel is built for)
+    if (per_sm == 0 && (decode8_ready<HD, false>() != 0 ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode8_kernel<HD, false>, D8_WARPS * 32, D8_SMEM<HD>) != cudaSuccess || per_sm <= 0)) {
         cudaGetLastError();
-        return 0;
+        per_sm = 0;
+        return 2 * sm_count();
     }
     return sm_count() * per_sm;
 }

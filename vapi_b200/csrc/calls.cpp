@@ -218,7 +218,209 @@ PyObject* shortconv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
+// ---- operators of serving in fewer bits ---------------------------------------------------------------
+// (`device`: the current one; all of a call's tensors are on it, or Python's steps say which is not)
+const at::Tensor& on(const at::Tensor& t, int device) {
+    if (t.get_device() != device) throw Bad{};
+    return t;
+}
+const at::Tensor* on(const at::Tensor* t, int device) {
+    if (t) on(*t, device);
+    return t;
+}
+const float* floats_on(PyObject* o, int64_t size, int device) {
+    on(tensor(o), device);
+    return floats(o, size, size);
+}
+const int* ints_on(PyObject* o, int64_t least, int device) {
+    on(tensor(o), device);
+    const int* p = ints(o, least);
+    if (!p) throw Bad{};
+    return p;
+}
+int type_code(const at::Tensor& t) {
+    if (t.scalar_type() == at::kBFloat16) return 1;
+    if (t.scalar_type() != at::kFloat) throw Bad{};
+    return 0;
+}
+struct Codes { const at::Tensor* codes; const at::Tensor* exps; int pages, nkv, page_size, d; };
+Codes cache8(PyObject* codes, PyObject* exps, int device) {
+    const at::Tensor& c = on(need(codes, at::kFloat8_e4m3fn, 5), device);
+    const at::Tensor& e = on(need(exps, at::kChar, 4), device);
+    if (c.size(1) != 2 || c.size(0) == 0 || c.size(3) == 0 || c.size(3) % 16 != 0 || e.size(0) != c.size(0) || e.size(1) != 2 || e.size(2) != c.size(2) ||
+        e.size(3) != c.size(3) / 16) throw Bad{};
+    return {&c, &e, size32(c.size(0)), size32(c.size(2)), size32(c.size(3)), size32(c.size(4))};
+}
+
+typedef int (*Write8Fn)(const void*, int, const float*, const float*, float, const float*, const float*, int, void*, void*, void*, const int*, int, int,
+                        int, int, int, int, int*, void*);
+
+// write8(fn, qkv, nh, nkv, d, q_weight, k_weight, eps, cos, sin, rot, codes, exps, slots, status, stream, device): ops.qk_norm_rope_write8
+PyObject* write8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    return guarded(nargs, 17, [&](bool& called) -> PyObject* {
+        const auto fn = reinterpret_cast<Write8Fn>(address(a[0]));
+        const int nh = integer(a[2]), nkv = integer(a[3]), d = integer(a[4]), rot = integer(a[10]), device = integer(a[16]);
+        const at::Tensor* x = on(tensor(a[1]), device);
+        if (!fn || !x || x->dim() != 2 || !x->is_contiguous() || nh <= 0 || nkv <= 0 || d <= 0 || x->size(1) != (nh + 2LL * nkv) * d) throw Bad{};
+        const int n = size32(x->size(0)), type = type_code(*x);
+        const Codes c = cache8(a[11], a[12], device);
+        if (c.nkv != nkv || c.d != d) throw Bad{};
+        const at::Tensor *cs = on(tensor(a[8]), device), *sn = on(tensor(a[9]), device);
+        if ((cs == nullptr) != (sn == nullptr)) throw Bad{};
+        for (const at::Tensor* t : {cs, sn})
+            if (t && (t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != n || t->size(1) != rot / 2 || !t->is_contiguous())) throw Bad{};
+        const float *qw = floats_on(a[5], d, device), *kw = floats_on(a[6], d, device);
+        const int* slots = ints_on(a[13], n, device);
+        const float eps = real(a[7]);
+        int* status = static_cast<int*>(address(a[14]));
+        void* stream = address(a[15]);
+        at::Tensor q = at::empty({n, (int64_t)nh * d}, x->options());
+        int rc;
+        called = true;
+        {
+            Unlocked unlocked;
+            rc = fn(x->data_ptr(), type, qw, kw, eps, cs ? static_cast<const float*>(cs->data_ptr()) : nullptr,
+                    sn ? static_cast<const float*>(sn->data_ptr()) : nullptr, rot, q.data_ptr(), c.codes->data_ptr(), c.exps->data_ptr(), slots, n, nh, nkv, d,
+                    c.page_size, c.pages, status, stream);
+        }
+        return rc != 0 ? PyLong_FromLong(rc) : wrap(q);
+    });
+}
+
+typedef int (*Read8Fn)(const void*, const void*, const int*, void*, int, int, int, int, int, int, int*, void*);
+
+// read8(fn, codes, exps, pages, float32 or not, status, stream, device): ops.cache8_read
+PyObject* read8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    return guarded(nargs, 8, [&](bool& called) -> PyObject* {
+        const auto fn = reinterpret_cast<Read8Fn>(address(a[0]));
+        const int f32 = integer(a[4]), device = integer(a[7]);
+        const Codes c = cache8(a[1], a[2], device);
+        const int* pages = ints_on(a[3], 0, device);
+        const int count = size32(tensor(a[3])->numel());
+        int* status = static_cast<int*>(address(a[5]));
+        void* stream = address(a[6]);
+        if (!fn) throw Bad{};
+        at::Tensor out = at::empty({count, 2, c.nkv, c.page_size, c.d}, c.codes->options().dtype(f32 ? at::kFloat : at::kBFloat16));
+        int rc;
+        called = true;
+        {
+            Unlocked unlocked;
+            rc = fn(c.codes->data_ptr(), c.exps->data_ptr(), pages, out.data_ptr(), f32 ? 0 : 1, count, c.nkv, c.d, c.page_size, c.pages, status, stream);
+        }
+        return rc != 0 ? PyLong_FromLong(rc) : wrap(out);
+    });
+}
+
+typedef int (*Attention8Fn)(const void*, long long, const void*, const void*, int, const int*, int, const int*, const int*, void*, int, int, int, int, int,
+                            int, int, int, int, float, int, int, int, int*, void*);
+
+// attention8(fn, q, q_row_stride, codes, exps, block_table, cu_q, seqlens_k, n, num_seqs, max_q, max_k, nh, nkv, d, scale, window, splits, impl, status,
+//            stream, device): ops.paged_attention8
+PyObject* attention8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    return guarded(nargs, 22, [&](bool& called) -> PyObject* {
+        const auto fn = reinterpret_cast<Attention8Fn>(address(a[0]));
+        const int device = integer(a[21]), n = integer(a[8]), seqs = integer(a[9]), max_q = integer(a[10]), max_k = integer(a[11]);
+        const int nh = integer(a[12]), nkv = integer(a[13]), d = integer(a[14]);
+        const int64_t stride = integer(a[2]);
+        const at::Tensor* q = on(tensor(a[1]), device);
+        if (!fn || !q || q->dim() < 1 || q->stride(-1) != 1 || n < 0 || seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || d <= 0 || stride < (int64_t)nh * d) throw Bad{};
+        const int type = type_code(*q);
+        if (n > 0 && (int64_t)q->storage().nbytes() < (q->storage_offset() + (n - 1) * stride + (int64_t)nh * d) * (int64_t)q->element_size()) throw Bad{};
+        const Codes c = cache8(a[3], a[4], device);
+        if (c.nkv != nkv || c.d != d) throw Bad{};
+        const at::Tensor* table = on(tensor(a[5]), device);
+        if (!table || table->scalar_type() != at::kInt || table->dim() != 2 || table->stride(1) != 1 || table->size(0) < seqs) throw Bad{};
+        const int *cu = ints_on(a[6], seqs + 1LL, device), *kl = ints_on(a[7], seqs, device);
+        const float scale = real(a[15]);
+        const int window = integer(a[16]), splits = integer(a[17]), impl = integer(a[18]), table_stride = size32(table->stride(0));
+        int* status = static_cast<int*>(address(a[19]));
+        void* stream = address(a[20]);
+        at::Tensor out = at::empty({n, (int64_t)nh * d}, q->options());
+        int rc;
+        called = true;
+        {
+            Unlocked unlocked;
+            rc = fn(q->data_ptr(), stride, c.codes->data_ptr(), c.exps->data_ptr(), type, static_cast<const int*>(table->data_ptr()), table_stride, cu, kl,
+                    out.data_ptr(), n, seqs, max_q, max_k, nh, nkv, d, c.page_size, c.pages, scale, window, splits, impl, status, stream);
+        }
+        return rc != 0 ? PyLong_FromLong(rc) : wrap(out);
+    });
+}
+
+typedef int (*Int4Fn)(const void*, const void*, int, int, int, const void*, int, const float*, void*, float*, int, int, void*);
+
+// int4(fn, codes, scales, n, k, group, x, bias, gated, act, float32 or not, stream, device): ops.int4_linear and int4_linear_swiglu of few rows.
+// (codes and scales are an Int4Weight's, laid out and checked by int4_pack)
+PyObject* int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    return guarded(nargs, 13, [&](bool& called) -> PyObject* {
+        const auto fn = reinterpret_cast<Int4Fn>(address(a[0]));
+        const int n = integer(a[3]), k = integer(a[4]), group = integer(a[5]), gated = integer(a[8]), act = integer(a[9]), f32 = integer(a[10]), device = integer(a[12]);
+        const at::Tensor& codes = on(need(a[1], at::kInt, 4), device);
+        const at::Tensor& scales = on(need(a[2], at::kInt, 4), device);
+        const at::Tensor& x = on(need(a[6], at::kBFloat16, 2), device);
+        if (!fn || x.size(1) != k || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0 || (gated && (f32 || a[7] != Py_None))) throw Bad{};
+        const int64_t tiles = (n + 15LL) / 16;
+        if (n <= 0 || k <= 0 || group <= 0 || codes.numel() != tiles * ((k + 63LL) / 64) * 128 || scales.numel() != tiles * (k / group) * 16) throw Bad{};
+        const int rows = size32(x.size(0));
+        const float* bias = floats_on(a[7], n, device);
+        void* stream = address(a[11]);
+        at::Tensor out = at::empty({rows, gated ? n / 2 : n}, f32 ? x.options().dtype(at::kFloat) : x.options());
+        int rc;
+        called = true;
+        {
+            Unlocked unlocked;
+            rc = fn(codes.data_ptr(), scales.data_ptr(), n, k, group, x.data_ptr(), rows, bias, f32 ? nullptr : out.data_ptr(),
+                    f32 ? static_cast<float*>(out.data_ptr()) : nullptr, gated, act, stream);
+        }
+        return rc != 0 ? PyLong_FromLong(rc) : wrap(out);
+    });
+}
+
+typedef int (*LogprobsFn)(const void*, int, int, int, long long, const int*, int, float*, float*, int*, float*, int, int*, void*);
+
+// logprobs(fn, logits, tokens, top, slices, status, stream, device): ops.token_logprobs, its four tensors as a tuple
+PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    return guarded(nargs, 8, [&](bool& called) -> PyObject* {
+        const auto fn = reinterpret_cast<LogprobsFn>(address(a[0]));
+        const int top = integer(a[3]), slices = integer(a[4]), device = integer(a[7]);
+        const at::Tensor* x = on(tensor(a[1]), device);
+        const at::Tensor& t = on(need(a[2], at::kInt, 1), device);
+        if (!fn || !x || x->dim() != 2 || (x->size(1) > 1 && x->stride(1) != 1) || t.size(0) != x->size(0)) throw Bad{};
+        const int64_t rows = size32(x->size(0)), vocab = size32(x->size(1));
+        if (top < 0 || top > 64 || top > vocab) throw Bad{};
+        const int type = type_code(*x);
+        int* status = static_cast<int*>(address(a[5]));
+        void* stream = address(a[6]);
+        // (one buffer: one allocation a call)
+        const auto options = x->options().dtype(at::kFloat);
+        at::Tensor buf = at::empty({rows * (2 + 2LL * top)}, options);
+        at::Tensor parts[4] = {buf.narrow(0, 0, rows), buf.narrow(0, rows, rows), buf.narrow(0, 2 * rows, rows * top).view(at::kInt).view({rows, (int64_t)top}),
+                               buf.narrow(0, (2 + top) * rows, rows * top).view({rows, (int64_t)top})};
+        float* p = static_cast<float*>(buf.data_ptr());
+        int rc;
+        called = true;
+        {
+            Unlocked unlocked;
+            rc = fn(x->data_ptr(), type, (int)rows, (int)vocab, x->stride(0), static_cast<const int*>(t.data_ptr()), top, p, p + rows,
+                    reinterpret_cast<int*>(p + 2 * rows), p + (2 + top) * rows, slices, status, stream);
+        }
+        if (rc != 0) return PyLong_FromLong(rc);
+        PyObject* all = PyTuple_New(4);
+        for (int i = 0; all && i < 4; ++i) {
+            PyObject* o = wrap(parts[i]);
+            if (!o) { Py_DECREF(all); return nullptr; }
+            PyTuple_SET_ITEM(all, i, o);
+        }
+        return all;
+    });
+}
+
 PyMethodDef methods[] = {
+    {"write8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write8)), METH_FASTCALL, "norm, rotation and the write to an 8-bit cache"},
+    {"read8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(read8)), METH_FASTCALL, "pages of an 8-bit cache as numbers"},
+    {"attention8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention8)), METH_FASTCALL, "attention over an 8-bit cache"},
+    {"int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(int4)), METH_FASTCALL, "a product of a few rows with a 4-bit weight"},
+    {"logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(logprobs)), METH_FASTCALL, "log probabilities of given tokens"},
     {"product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(product)), METH_FASTCALL, "a fused product of a few rows"},
     {"shortconv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(shortconv)), METH_FASTCALL, "the gated short convolution"},
     {nullptr, nullptr, 0, nullptr}};

@@ -124,7 +124,7 @@ class _NoCalls:
     def product(*_):
         return NotImplemented
 
-    shortconv = product
+    shortconv = write8 = read8 = attention8 = int4 = logprobs = product
 
 
 def _calls():
@@ -170,6 +170,16 @@ def _cuda(*ts: Optional[torch.Tensor]) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise KernelError("vapi_b200 kernels run on CUDA tensors only; there is no CPU fallback")
+
+
+def _native(name: str, lib: ctypes.CDLL, fn: str, *args):
+    """A call of csrc/calls.cpp on the current stream and device: its answer, or NotImplemented where the same steps in Python are to say
+    what is wrong (or to do it)."""
+    device = torch._C._cuda_getDevice()
+    stream = _held.stream
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(device)
+    return getattr(_calls_module or _calls(), name)(_address(lib, fn), *args, stream, device)
 
 
 def _here(*ts: Optional[torch.Tensor]) -> None:

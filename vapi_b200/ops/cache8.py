@@ -1,12 +1,11 @@
 """A paged cache of keys and values in 8 bits: the write, the read, and attention over it (csrc/cache8.cu)."""
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
 
-from . import (KernelError, _check, _contig, _cuda, _dt, _f32, _here, _i32, _least, _lib, _p, _stream, sm_count)
+from . import KernelError, _check, _contig, _cuda, _dt, _f32, _here, _i32, _least, _lib, _native, _p, _stream
 
 #: tokens of a head that share a scale
 CACHE8_BLOCK = 16
@@ -54,6 +53,13 @@ def qk_norm_rope_write8(qkv: torch.Tensor, nh: int, nkv: int, d: int, q_weight: 
     Tokens of one block of 16 must follow one another in the step, as a request's do.  A block whose first token (place 0) is
     among them begins afresh; the older tokens of another one are rounded again when a new token needs a larger scale.  What
     is not finite is kept as NaN."""
+    if qkv.is_cuda:
+        lib = _lib("cache8")
+        got = _native("write8", lib, "vapi_qk_norm_rope_write8", qkv, nh, nkv, d, q_weight, k_weight, eps, cos, sin, rot, cache[0], cache[1],
+                      slot_mapping, _p(status))
+        if got is not NotImplemented:
+            _check(lib, got if type(got) is int else 0, int(qkv.shape[0] > 0))
+            return got
     _contig(qkv, "qkv")
     for t, w in ((q_weight, "q norm weight"), (k_weight, "k norm weight"), (cos, "cos"), (sin, "sin")):
         _f32(t, w)
@@ -82,6 +88,12 @@ def qk_norm_rope_write8(qkv: torch.Tensor, nh: int, nkv: int, d: int, q_weight: 
 def cache8_read(cache: Cache8, pages: torch.Tensor, dtype: torch.dtype, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """What whole pages of a cache hold, [len(pages), 2, nkv, page_size, d] in ``dtype`` (bfloat16 holds every number of the
     cache exactly, and so does float32): to move a request's tokens to another cache, or to look at them."""
+    if pages.is_cuda and dtype in (torch.bfloat16, torch.float32):
+        lib = _lib("cache8")
+        got = _native("read8", lib, "vapi_cache8_read", cache[0], cache[1], pages, int(dtype == torch.float32), _p(status))
+        if got is not NotImplemented:
+            _check(lib, got if type(got) is int else 0, int(pages.numel() > 0))
+            return got
     _i32(pages, "pages")
     _contig(pages, "pages")
     nkv, d = (cache.codes.shape[2], cache.codes.shape[4]) if cache.codes.dim() == 5 else (0, 0)
@@ -95,22 +107,11 @@ def cache8_read(cache: Cache8, pages: torch.Tensor, dtype: torch.dtype, status: 
     return out
 
 
-_slots = {}
-
-
 def attention8_splits(num_seqs: int, max_q: int, max_k: int, nh: int, nkv: int, d: int) -> int:
-    """How many blocks (of eight warps) share the keys of one (sequence, kv head, tile of rows) in :func:`paged_attention8`: a power of
-    two up to a cluster's 16, while all blocks are on the device at once and each warp still has two blocks of 16 tokens."""
-    rows = max_q * (nh // nkv)
-    blocks = num_seqs * nkv * -(-rows // (8 if rows <= 8 else 16))
-    key = (torch.cuda.current_device(), d)
-    slots = _slots.get(key)
-    if slots is None:
-        slots = _slots[key] = int(_lib("cache8").vapi_attention8_slots(d)) or 2 * sm_count()
-    splits = 1
-    while splits < 16 and 2 * splits * blocks <= slots and 2 * splits * 256 <= max_k:
-        splits *= 2
-    return splits
+    """How many blocks (of eight warps) share the keys of one (sequence, kv head, tile of rows) in :func:`paged_attention8` when it is not
+    told (the library's own rule): a power of two up to a cluster's 16, while all blocks are on the device at once and each warp still
+    has two blocks of 16 tokens."""
+    return int(_lib("cache8").vapi_attention8_splits(num_seqs, max_q, max_k, nh, nkv, d))
 
 
 _IMPL8 = {"auto": 0, "general": 1, "tensor_core": 2, "tcgen05": 3}
@@ -129,6 +130,15 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     mma.sync kernel, whose ``splits`` (up to 16) blocks share the keys as a cluster, for the others; the general kernel for every other
     type, head size (a multiple of 16 up to 256) and alignment.  "tcgen05", "tensor_core" and "general" force one (the first two raise where
     they do not apply)."""
+    code = _IMPL8.get(impl)
+    two = max_q >= PORTION8_MIN_Q and num_seqs > 1 and code == 0 and q.dtype == torch.bfloat16 and d in (64, 128)
+    if q.is_cuda and code is not None:
+        lib = _lib("cache8")
+        got = _native("attention8", lib, "vapi_paged_attention8", q, q_row_stride, cache[0], cache[1], block_table, cu_q, seqlens_k, n, num_seqs,
+                      max_q, max_k, nh, nkv, d, scale, window, splits or 0, code, _p(status))
+        if got is not NotImplemented:
+            _check(lib, got if type(got) is int else 0, (2 if two else 1) if n > 0 else 0)
+            return got
     for t, w in ((block_table, "block table"), (cu_q, "cu_q"), (seqlens_k, "seqlens_k")):
         _i32(t, w)
     if impl not in _IMPL8:
@@ -146,12 +156,9 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     pages, page_size = _cache8(cache, nkv, d)
     _cuda(q, cache.codes, cache.exps, block_table, cu_q, seqlens_k)
     _here(q, cache.codes, cache.exps, block_table, cu_q, seqlens_k)
-    two = max_q >= PORTION8_MIN_Q and num_seqs > 1 and impl == "auto" and q.dtype == torch.bfloat16 and d in (64, 128)
-    if splits is None:
-        splits = attention8_splits(num_seqs, 1 if two else max_q, max_k, nh, nkv, d)
     out = torch.empty((n, nh * d), dtype=q.dtype, device=q.device)
     lib = _lib("cache8")
     _check(lib, lib.vapi_paged_attention8(_p(q), q_row_stride, _p(cache.codes), _p(cache.exps), _dt(q), _p(block_table), block_table.stride(0),
                                           _p(cu_q), _p(seqlens_k), _p(out), n, num_seqs, max_q, max_k, nh, nkv, d, page_size, pages,
-                                          scale, window, splits, _IMPL8[impl], _p(status), _stream()), launches=(2 if two else 1) if n > 0 else 0)
+                                          scale, window, splits or 0, code, _p(status), _stream()), launches=(2 if two else 1) if n > 0 else 0)
     return out

@@ -6,7 +6,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import BF16, KernelError, _bias, _check, _cuda, _glu, _here, _lib, _p, _stream, _DT
+from . import BF16, KernelError, _bias, _check, _cuda, _glu, _here, _lib, _native, _p, _stream, _DT
 from . import linear as _linear
 from . import linear_swiglu as _linear_swiglu
 from . import swiglu as _swiglu
@@ -140,6 +140,12 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
     Up to INT4_MAX_ROWS bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in
     float32, and the result is rounded once.  Larger steps, and float32 ones, take the weight as numbers of the type of ``x``
     (:func:`int4_dequantize`) through :func:`linear`."""
+    if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] <= INT4_MAX_ROWS and out_dtype in (None, torch.bfloat16, torch.float32):
+        lib = _lib("int4")
+        got = _native("int4", lib, "vapi_int4_linear", w.codes, w.scales, w.n, w.k, w.group, x, bias, 0, 0, int(out_dtype == torch.float32))
+        if got is not NotImplemented:
+            _check(lib, got if type(got) is int else 0, int(x.shape[0] > 0))
+            return got
     x = _operands(x, w)
     _bias(bias, w.n)
     if out_dtype not in (None, x.dtype, torch.float32):
@@ -151,6 +157,12 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
 
 def int4_linear_swiglu(x: torch.Tensor, w: Int4Weight, act: str = "silu") -> torch.Tensor:
     """:func:`linear_swiglu` with a 4-bit weight [Wg; Wu]: ``act(x @ Wg.T) * (x @ Wu.T)``, the gate in the product's epilogue."""
+    if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] <= INT4_MAX_ROWS and w.n % 32 == 0:
+        lib = _lib("int4")
+        got = _native("int4", lib, "vapi_int4_linear", w.codes, w.scales, w.n, w.k, w.group, x, None, 1, _glu(act), 0)
+        if got is not NotImplemented:
+            _check(lib, got if type(got) is int else 0, int(x.shape[0] > 0))
+            return got
     x = _operands(x, w)
     if w.n % 2:
         raise KernelError("a gated product needs an even number of features")

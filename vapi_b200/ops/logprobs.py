@@ -5,7 +5,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import KernelError, _check, _contig, _cuda, _dt, _here, _i32, _lib, _p, _stream
+from . import KernelError, _check, _contig, _cuda, _dt, _here, _i32, _lib, _native, _p, _stream
 
 #: alternatives that one call reports at most
 LOGPROBS_MAX_TOP = 64
@@ -30,6 +30,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sta
     ranking.  A row with a NaN or +inf, or of nothing but -inf, has NaN for its numbers (which tokens it then ranks is not said; -1 stands
     where there are none).  ``slices``: into how many blocks a row is cut (a power of two up to 16; 0: as many as pay); in another
     cut the sums are added in another order."""
+    if logits.is_cuda:
+        lib = _lib("logprobs")
+        got = _native("logprobs", lib, "vapi_token_logprobs", logits, tokens, top, slices, _p(status))
+        if got is not NotImplemented:
+            _check(lib, got if type(got) is int else 0, int(logits.shape[0] > 0))
+            return TokenLogprobs._make(got)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError("logits must be [R, V] with unit inner stride")
     dt = _dt(logits)
