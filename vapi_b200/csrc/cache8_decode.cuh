@@ -3,18 +3,21 @@
 //
 // A decode step reads every key and value of every live request once, so the kernel is built around that stream.  A cluster of
 // up to 16 blocks owns one (sequence, kv head, tile of 8 or 16 rows) and its eight warps each a run of chunks: the 16
-// tokens that share a scale, one piece of memory of 16 * head size bytes for K and one for V.  A warp brings its own chunks
-// in by bulk copies through a ring of its own, and no warp waits for another before the end, where their partial results are
-// joined: through shared memory in a block, through the cluster's among its blocks, always in the same order.
+// tokens that share a scale, one piece of memory of 16 * head size bytes for K and one for V.  A warp brings its own chunks,
+// two at a time, in by bulk copies through a ring of its own, and no warp waits for another before the end, where their partial
+// results are joined: through shared memory in a block, through the cluster's among its blocks, always in the same order.
 //
-//   S = Q K^T    A code is an f16 number exactly.  A row of Q is scaled by a power of two so that its largest element is near
-//                2^14: f16 then has three bits more than bfloat16 for it, and elements keep all of theirs down to 2^-28 of the
-//                largest.  A lane's 16 contiguous bytes of a key are its B operands of four k-steps: the order of the head's
-//                elements in the sum is free as long as Q follows it, and so no byte moves between lanes.
-//   O += P V     P = 2^(s - m_chunk) with the chunk's own row maximum, so that its largest is 1 whatever the other chunks hold;
-//                the chunk's product is added to O times 2^(m_chunk - m + e_V) in float.  (P times the scale in f16 would lose
-//                what a block of small values says beside one of large.)  The values of two tokens are paired by byte
-//                permutes; which token is which k is free too, as long as K's columns follow.
+//   S^T = K Q^T  16 tokens are a product's rows and 8 query rows its columns, so that four query heads a kv head leave half of it
+//                unused and not three quarters.  A code is an f16 number exactly.  A row of Q is scaled by a power of two so that
+//                its largest element is near 2^14: f16 then has three bits more than bfloat16 for it, and elements keep all of
+//                theirs down to 2^-28 of the largest.  A lane's 16 contiguous bytes of a key are its operands of four k-steps: the
+//                order of the head's elements in the sum is free as long as Q follows it, and so no byte moves between lanes.
+//   O^T += V^T P^T   P = 2^(s + e - M) with the values' scale 2^e in the exponent and M the largest s + e so far: the product of P and
+//                the codes is added up in the tensor core's accumulator as it is.  (One maximum for both would lose, in f16, what a
+//                block of large values says at a small weight, or the other way round.)  The sum of weights is taken of 2^(s - m), m
+//                the largest s so far.  m and M are only raised when a score passes them by more than 2^8 (f16 holds P up
+//                to 2^15, float the sums), which no lane has to ask its neighbours for: a vote a chunk, and a reduction a few times
+//                a row.  P is turned about by movmatrix; the values of two tokens are paired by byte permutes.
 //
 // Keys behind a sequence's end are masked by selection, and their values taken as zeros.  (A NaN among the keys and values that a
 // sequence did write, though a row may not see it, can reach that row through 0 * NaN; the step that wrote it was lost.)
@@ -27,14 +30,21 @@ namespace vapi {
 
 constexpr int D8_WARPS = 8;
 constexpr int D8_MAX_CLUSTER = 16;
-template <int HD> constexpr int D8_STAGES = HD == 64 ? 6 : 3;
+constexpr int D8_STAGES = 3;                                                           // of two chunks of K and of V
+constexpr float D8_RAISE = 8.f;                                                        // log2 units by which a score must pass a maximum to raise it
 template <int HD> constexpr int D8_CHUNK = C8_BLOCK * HD;                              // bytes of a chunk of K, or of V
-template <int HD> constexpr int D8_WARP_BYTES = D8_STAGES<HD> * 2 * D8_CHUNK<HD>;
+template <int HD> constexpr int D8_WARP_BYTES = D8_STAGES * 4 * D8_CHUNK<HD>;
 template <int HD> constexpr size_t D8_SMEM = (size_t)D8_WARPS * D8_WARP_BYTES<HD>;
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of 16-bit numbers, a row's pair of columns a lane, about its diagonal
+__device__ __forceinline__ unsigned d8_turned(unsigned x) {
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ unsigned d8_half2(float lo, float hi) {
     unsigned r;
@@ -60,16 +70,16 @@ __device__ __forceinline__ uint2 d8_lds8(unsigned addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
-// WIDE: tiles of 16 rows; else of 8 (the lower half of every fragment is then zero and is not worked out).
+// WIDE: tiles of 16 rows, else of 8.
 template <int HD, bool WIDE>
-__global__ void __launch_bounds__(D8_WARPS * 32, 2)
+__global__ void __launch_bounds__(D8_WARPS * 32, HD == 64 ? 2 : 1)
 decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int splits, const int most_q) {
-    constexpr int ROWS = WIDE ? 16 : 8, H = WIDE ? 2 : 1, STAGES = D8_STAGES<HD>, CHUNK = D8_CHUNK<HD>;
-    constexpr int KS = HD / 16, NT = HD / 8, Q64 = HD / 64;                 // k-steps of S, column tiles of O, runs of 64 elements
+    constexpr int ROWS = WIDE ? 16 : 8, H = WIDE ? 2 : 1, CHUNK = D8_CHUNK<HD>;
+    constexpr int KS = HD / 16, Q64 = HD / 64, VW = HD / 32;                // k-steps of S; runs of 64 elements; words of a token's values that a lane holds
     extern __shared__ __align__(128) unsigned char d8_smem[];
-    __shared__ __align__(8) unsigned long long bars[D8_WARPS * STAGES];
-    __shared__ float sM[D8_WARPS][ROWS], sL[D8_WARPS][ROWS];
-    __shared__ float xM[ROWS], xL[ROWS];
+    __shared__ __align__(8) unsigned long long bars[D8_WARPS * D8_STAGES];
+    __shared__ float sM[D8_WARPS][ROWS], sR[D8_WARPS][ROWS], sL[D8_WARPS][ROWS];
+    __shared__ float xM[ROWS], xR[ROWS], xL[ROWS];
     __shared__ __align__(16) float xO[ROWS][HD];
     __shared__ int failed;
 
@@ -89,11 +99,11 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     const int c_lo = key_lo / C8_BLOCK;
     const long long chunks = p_max < key_lo ? 0 : p_max / C8_BLOCK - c_lo + 1;
     const int units = splits * D8_WARPS, unit = rank * D8_WARPS + warp;
-    const int begin = c_lo + (int)(chunks * unit / units), end = c_lo + (int)(chunks * (unit + 1) / units), nt = end - begin;
+    const int begin = c_lo + (int)(chunks * unit / units), end = c_lo + (int)(chunks * (unit + 1) / units), nt = end - begin, pairs = (nt + 1) / 2;
 
-    const unsigned bar = smem_u32(bars + warp * STAGES), ring = smem_u32(d8_smem + (size_t)warp * D8_WARP_BYTES<HD>);
+    const unsigned bar = smem_u32(bars + warp * D8_STAGES), ring = smem_u32(d8_smem + (size_t)warp * D8_WARP_BYTES<HD>);
     if (lane == 0) {
-        for (int i = 0; i < STAGES; ++i) mbar_init(bar + 8 * i, 1);
+        for (int i = 0; i < D8_STAGES; ++i) mbar_init(bar + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x == 0) failed = 0;
@@ -117,34 +127,30 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         where = (page * 2 * p.nkv + g) * per_head + key % p.page_size / C8_BLOCK;
         scales_next = c8_scales(p, where, per_head);
     };
-    auto bring = [&](int it) {                                              // chunk begin + it into its place of the ring
-        if ((it & 31) == 0) look_up(it);
-        const int at = __shfl_sync(0xffffffffu, where, it & 31), stage = it % STAGES;
-        if (lane == 0) {
-            mbar_expect_tx(bar + 8 * stage, 2 * CHUNK);
-            const unsigned dst = ring + stage * 2 * CHUNK;
-            d8_copy(dst, p.codes + (size_t)at * CHUNK, CHUNK, bar + 8 * stage);
-            d8_copy(dst + CHUNK, p.codes + ((size_t)at + (size_t)p.nkv * per_head) * CHUNK, CHUNK, bar + 8 * stage);
-        }
+    const size_t to_values = (size_t)p.nkv * per_head * CHUNK;
+    auto bring = [&](int it, int stage) {                                   // chunks begin + 2 it and the next into a place of the ring: K, K, V, V
+        if ((it & 15) == 0) look_up(2 * it);
+        const int at = __shfl_sync(0xffffffffu, where, (2 * it + (lane & 1)) & 31);
+        const bool both = 2 * it + 1 < nt;
+        if (lane == 0) mbar_expect_tx(bar + 8 * stage, (both ? 4 : 2) * CHUNK);
+        __syncwarp();
+        if (lane < 4 && (both || !(lane & 1)))
+            d8_copy(ring + (stage * 4 + lane) * CHUNK, p.codes + (size_t)at * CHUNK + (lane & 2 ? to_values : 0), CHUNK, bar + 8 * stage);
     };
-    for (int it = 0; it < min(nt, STAGES); ++it) bring(it);
+    for (int it = 0; it < min(pairs, D8_STAGES); ++it) bring(it, it);
     scales = scales_next;
     if (!waited) { pdl_wait(); waited = true; }                             // q comes from the kernel before this one
 
-    int row_pos[H];
-    float row_f[H];
-    unsigned qf[KS][4];
+    // Q^T: a lane has row gq (and gq + 8), elements 16 tq .. + 15 of each 64; what it needs of the rows of its scores, 2 tq and
+    // 2 tq + 1 (and those + 8), comes from the lanes that have them
+    float row_f[H][2];
+    int row_pos[H][2];
+    unsigned qf[H][KS][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (h >= H) {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) qf[k][1] = qf[k][3] = 0u;
-            break;
-        }
+    for (int h = 0; h < H; ++h) {
         const int rr = r0 + gq + 8 * h;
         const bool ok = rr < rows_total;
         const int tok = ok ? rr / n_rep : 0, head = g * n_rep + (ok ? rr - tok * n_rep : 0);
-        row_pos[h] = ok ? base + tok : -1;                                  // -1: sees nothing
         const __nv_bfloat16* src = q + (size_t)(q0 + tok) * p.q_row_stride + (size_t)head * HD + tq * 16;
         unsigned raw[Q64][8];
         float big = 0.f;
@@ -163,133 +169,154 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         // largest element to [2^14, 2^15); the exponent kept where both factors are ordinary numbers
         const int x = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120);
-        const float up = c8_power(14 - x);
-        row_f[h] = c8_power(x - 14) * p.scale_log2e;
+        const float up = c8_power(14 - x), down = c8_power(x - 14) * p.scale_log2e;
+        const int pos = ok ? base + tok : -1;                               // -1: sees nothing
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            const unsigned a = raw[k / 4][2 * (k & 3)], b = raw[k / 4][2 * (k & 3) + 1];
-            qf[k][h] = d8_half2(__uint_as_float(a << 16) * up, __uint_as_float(a & 0xffff0000u) * up);
-            qf[k][2 + h] = d8_half2(__uint_as_float(b << 16) * up, __uint_as_float(b & 0xffff0000u) * up);
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned w = raw[k / 4][2 * (k & 3) + i];
+                qf[h][k][i] = d8_half2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+            }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            row_f[h][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * tq + i));
+            row_pos[h][i] = __shfl_sync(0xffffffffu, pos, 4 * (2 * tq + i));
         }
     }
 
-    float m[H], l[H], o[NT][2 * H];
+    float m[H][2], big[H][2], l[H][2], o[H][HD / 16][4];                    // of rows 2 tq and 2 tq + 1: m, M and the sum of weights
 #pragma unroll
-    for (int h = 0; h < H; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
+    for (int h = 0; h < H; ++h) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int i = 0; i < 2; ++i) { m[h][i] = big[h][i] = -INFINITY; l[h][i] = 0.f; }
 #pragma unroll
-        for (int i = 0; i < 2 * H; ++i) o[t][i] = 0.f;
+        for (int t = 0; t < HD / 16; ++t) o[h][t][0] = o[h][t][1] = o[h][t][2] = o[h][t][3] = 0.f;
+    }
     bool ok = true;
 
-    for (int it = 0; it < nt; ++it) {
-        const int stage = it % STAGES, k0 = (begin + it) * C8_BLOCK;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, (it / STAGES) & 1))) {
-            // given up: the copies that are still under way get one more bounded wait each, then the block leaves
-            for (int j = it; j < min(nt, it + STAGES); ++j) mbar_wait(bar + 8 * (j % STAGES), (j / STAGES) & 1);
-            ok = false;
-            break;
-        }
-        const unsigned kb = ring + stage * 2 * CHUNK, vb = kb + CHUNK;
-        // scores of tokens 8j + (column / 2) + 4 (column & 1), in tile j
-        float sc[2][4];
+    // Tokens of a chunk in the order of a product's rows: row r < 8 is token r / 2 + 4 (r & 1), row 8 + r the one 8 further on, so that
+    // the pairs of rows that a lane of V^T has (2 tq, 2 tq + 1) are tokens tq and 4 + tq.
+    const unsigned k_at = ((gq >> 1) + 4 * (gq & 1)) * HD + tq * 16, v_at = tq * HD + gq * (HD / 8);
+    const int token = (gq >> 1) + 4 * (gq & 1);
+    auto chunk_of = [&](unsigned kb, unsigned vb, int k0, int e) {
+        float sc[H][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-            const unsigned row = kb + (8 * j + (gq >> 1) + 4 * (gq & 1)) * HD + tq * 16;
+        for (int h = 0; h < H; ++h) sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
 #pragma unroll
-            for (int r = 0; r < Q64; ++r) {
-                const uint4 c = d8_lds16(row + r * 64);
-                const unsigned w[4] = {c.x, c.y, c.z, c.w};
+        for (int r = 0; r < Q64; ++r) {
+            const uint4 ca = d8_lds16(kb + k_at + r * 64), cb = d8_lds16(kb + k_at + 8 * HD + r * 64);
+            const unsigned wa[4] = {ca.x, ca.y, ca.z, ca.w}, wb[4] = {cb.x, cb.y, cb.z, cb.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    mma_f16_16816(sc[j], qf[4 * r + i][0], qf[4 * r + i][1], qf[4 * r + i][2], qf[4 * r + i][3],
-                                  c8_halves((unsigned short)(w[i] & 0xffffu)), c8_halves((unsigned short)(w[i] >> 16)));
+            for (int i = 0; i < 4; ++i) {
+                const unsigned a0 = c8_halves((unsigned short)(wa[i] & 0xffffu)), a1 = c8_halves((unsigned short)(wb[i] & 0xffffu));
+                const unsigned a2 = c8_halves((unsigned short)(wa[i] >> 16)), a3 = c8_halves((unsigned short)(wb[i] >> 16));
+#pragma unroll
+                for (int h = 0; h < H; ++h) mma_f16_16816(sc[h], a0, a1, a2, a3, qf[h][4 * r + i][0], qf[h][4 * r + i][1]);
             }
         }
+        const float ek = c8_power((int)(signed char)(e & 0xff)), ev = (float)(signed char)(e >> 8 & 0xff);
+        const bool edge = k0 + C8_BLOCK - 1 > p_min || (p.window > 0 && k0 <= p_max - p.window);
+        bool raise = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {                                   // row 2 tq + i: its scores of tokens `token` and 8 further on
+                float &x = sc[h][i], &y = sc[h][2 + i];
+                const float f = row_f[h][i] * ek;
+                x *= f;
+                y *= f;
+                if (edge) {
+                    const int pos = row_pos[h][i], kx = k0 + token, ky = kx + 8;
+                    x = kx <= pos && kx < klen && (p.window <= 0 || kx > pos - p.window) ? x : -INFINITY;
+                    y = ky <= pos && ky < klen && (p.window <= 0 || ky > pos - p.window) ? y : -INFINITY;
+                }
+                const float mx = fmaxf(x, y);
+                raise |= mx > m[h][i] + D8_RAISE || mx + ev > big[h][i] + D8_RAISE;
+            }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float mx = fmaxf(sc[h][i], sc[h][2 + i]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    if (mx > m[h][i]) {                                     // (m = -inf: the factor is 0, and the sum is 0)
+                        l[h][i] *= d8_ex2(m[h][i] - mx);
+                        m[h][i] = mx;
+                    }
+                    if (mx + ev > big[h][i]) {
+                        const float f = d8_ex2(big[h][i] - (mx + ev));
+#pragma unroll
+                        for (int t = 0; t < HD / 16; ++t) { o[h][t][i] *= f; o[h][t][2 + i] *= f; }
+                        big[h][i] = mx + ev;
+                    }
+                }
+        }
+        unsigned pt[H][2];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // (a row that has seen nothing: its scores are -inf, and stay so)
+                const float mu = m[h][i] == -INFINITY ? 0.f : m[h][i], up = m[h][i] == -INFINITY ? 0.f : ev - big[h][i];
+                w[i] = d8_ex2(sc[h][i] + up);
+                w[2 + i] = d8_ex2(sc[h][2 + i] + up);
+                l[h][i] += d8_ex2(sc[h][i] - mu) + d8_ex2(sc[h][2 + i] - mu);
+            }
+            pt[h][0] = d8_turned(d8_half2(w[0], w[1]));
+            pt[h][1] = d8_turned(d8_half2(w[2], w[3]));
+        }
         // the values of tokens tq, 4 + tq, 8 + tq, 12 + tq: HD / 8 elements from gq * (HD / 8) on
-        unsigned v[4][NT / 4];
+        unsigned v[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned at = vb + (4 * i + tq) * HD + gq * (HD / 8);
+            const unsigned at = vb + v_at + 4 * i * HD;
             if (HD == 64) {
                 const uint2 x = d8_lds8(at);
                 v[i][0] = x.x; v[i][1] = x.y;
             } else {
                 const uint4 x = d8_lds16(at);
-                v[i][0] = x.x; v[i][1] = x.y; v[i][NT / 4 - 2] = x.z; v[i][NT / 4 - 1] = x.w;
+                v[i][0] = x.x; v[i][1] = x.y; v[i][VW - 2] = x.z; v[i][VW - 1] = x.w;
             }
             if (k0 + C8_BLOCK > klen && k0 + 4 * i + tq >= klen) {
 #pragma unroll
-                for (int c = 0; c < NT / 4; ++c) v[i][c] = 0u;
+                for (int c = 0; c < VW; ++c) v[i][c] = 0u;
             }
         }
-        const int e = __shfl_sync(0xffffffffu, scales, it & 31);
+        // tile t of O^T: rows gq and 8 + gq are elements gq * (HD / 8) + 2t and + 1
+#pragma unroll
+        for (int c = 0; c < VW; ++c) {
+            const unsigned x01[2] = {__byte_perm(v[0][c], v[1][c], 0x5140), __byte_perm(v[0][c], v[1][c], 0x7362)};
+            const unsigned x23[2] = {__byte_perm(v[2][c], v[3][c], 0x5140), __byte_perm(v[2][c], v[3][c], 0x7362)};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned a0 = c8_halves((unsigned short)(x01[i] & 0xffffu)), a1 = c8_halves((unsigned short)(x01[i] >> 16));
+                const unsigned a2 = c8_halves((unsigned short)(x23[i] & 0xffffu)), a3 = c8_halves((unsigned short)(x23[i] >> 16));
+#pragma unroll
+                for (int h = 0; h < H; ++h) mma_f16_16816(o[h][2 * c + i], a0, a1, a2, a3, pt[h][0], pt[h][1]);
+            }
+        }
+    };
+    int stage = 0, parity = 0;
+    for (int it = 0; it < pairs; ++it) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
+            // given up: the copies that are still under way get one more bounded wait each, then the block leaves
+            for (int j = it; j < min(pairs, it + D8_STAGES); ++j) mbar_wait(bar + 8 * (j % D8_STAGES), (j / D8_STAGES) & 1);
+            ok = false;
+            break;
+        }
+        const unsigned kb = ring + stage * 4 * CHUNK;
+        const int k0 = (begin + 2 * it) * C8_BLOCK, e0 = __shfl_sync(0xffffffffu, scales, (2 * it) & 31), e1 = __shfl_sync(0xffffffffu, scales, (2 * it + 1) & 31);
+        chunk_of(kb, kb + 2 * CHUNK, k0, e0);
+        if (2 * it + 1 < nt) chunk_of(kb + CHUNK, kb + 3 * CHUNK, k0 + C8_BLOCK, e1);
         __syncwarp();                                                       // every lane has what it wants of this place
-        if (it + STAGES < nt) bring(it + STAGES);
-        if ((it & 31) == 31) scales = scales_next;                          // (the look-up of the next 32 is behind us: STAGES < 32)
-
-        const float ek = c8_power((int)(signed char)(e & 0xff)), ev = c8_power((int)(signed char)(e >> 8 & 0xff));
-        const bool edge = k0 + C8_BLOCK - 1 > p_min || (p.window > 0 && k0 <= p_max - p.window);
-        float add[H];
-        bool moved = false;
-        float keep[H];
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const float f = row_f[h] * ek;
-            float* x[4] = {&sc[0][2 * h], &sc[0][2 * h + 1], &sc[1][2 * h], &sc[1][2 * h + 1]};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                *x[i] *= f;
-                if (edge) {
-                    const int key = k0 + 4 * i + tq;                        // column 2 tq + (i & 1) of tile i >> 1
-                    const bool sees = key <= row_pos[h] && key < klen && (p.window <= 0 || key > row_pos[h] - p.window);
-                    *x[i] = sees ? *x[i] : -INFINITY;
-                }
-            }
-            float mx = fmaxf(fmaxf(*x[0], *x[1]), fmaxf(*x[2], *x[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mu = mx == -INFINITY ? 0.f : mx, mn = fmaxf(m[h], mx), mnu = mn == -INFINITY ? 0.f : mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                *x[i] = d8_ex2(*x[i] - mu);
-                sum += *x[i];
-            }
-            const float a = d8_ex2(m[h] - mnu), b = d8_ex2(mx - mnu);
-            l[h] = l[h] * a + sum * b;
-            m[h] = mn;
-            keep[h] = a;
-            add[h] = b * ev;
-            moved |= a != 1.f;
-        }
-        const unsigned a0 = d8_half2(sc[0][0], sc[0][1]), a2 = d8_half2(sc[1][0], sc[1][1]);
-        const unsigned a1 = WIDE ? d8_half2(sc[0][2], sc[0][3]) : 0u, a3 = WIDE ? d8_half2(sc[1][2], sc[1][3]) : 0u;
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 2 * H; ++i) o[t][i] *= keep[i >> 1];
-        }
-#pragma unroll
-        for (int c = 0; c < NT / 4; ++c) {
-            const unsigned lo01 = __byte_perm(v[0][c], v[1][c], 0x5140), hi01 = __byte_perm(v[0][c], v[1][c], 0x7362);
-            const unsigned lo23 = __byte_perm(v[2][c], v[3][c], 0x5140), hi23 = __byte_perm(v[2][c], v[3][c], 0x7362);
-            const unsigned w01[2] = {lo01, hi01}, w23[2] = {lo23, hi23};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned x = w01[i >> 1], y = w23[i >> 1];
-                float t4[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16_16816(t4, a0, a1, a2, a3, c8_halves((unsigned short)(i & 1 ? x >> 16 : x & 0xffffu)),
-                              c8_halves((unsigned short)(i & 1 ? y >> 16 : y & 0xffffu)));
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    o[4 * c + i][2 * h] = fmaf(t4[2 * h], add[h], o[4 * c + i][2 * h]);
-                    o[4 * c + i][2 * h + 1] = fmaf(t4[2 * h + 1], add[h], o[4 * c + i][2 * h + 1]);
-                }
-            }
-        }
+        if (it + D8_STAGES < pairs) bring(it + D8_STAGES, stage);
+        if ((it & 15) == 15) scales = scales_next;                          // (the look-up of the next 32 is behind us)
+        if (++stage == D8_STAGES) { stage = 0; parity ^= 1; }
     }
     if (!ok) failed = 1;
     __syncwarp();
@@ -297,67 +324,72 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     // ---- the warps' results, joined in warp order; a warp's own part of the ring holds its O (all its copies have arrived)
     float* wO = reinterpret_cast<float*>(d8_smem + (size_t)warp * D8_WARP_BYTES<HD>);
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        float sum = l[h];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (tq == 0) { sM[warp][gq + 8 * h] = m[h]; sL[warp][gq + 8 * h] = sum; }
-        // columns 2 tq and 2 tq + 1 of tile t are elements (2 tq) * NT + t and (2 tq + 1) * NT + t
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+            const int row = 8 * h + 2 * tq + i;
+            float sum = l[h][i];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            if (gq == 0) { sM[warp][row] = m[h][i]; sR[warp][row] = big[h][i]; sL[warp][row] = sum; }
 #pragma unroll
-            for (int t = 0; t < NT; t += 4)
-                *reinterpret_cast<float4*>(wO + (gq + 8 * h) * HD + (2 * tq + i) * NT + t) =
-                    make_float4(o[t][2 * h + i], o[t + 1][2 * h + i], o[t + 2][2 * h + i], o[t + 3][2 * h + i]);
-    }
+            for (int t = 0; t < HD / 16; t += 2)
+                *reinterpret_cast<float4*>(wO + row * HD + gq * (HD / 8) + 2 * t) =
+                    make_float4(o[h][t][i], o[h][t][2 + i], o[h][t + 1][i], o[h][t + 1][2 + i]);
+        }
     __syncthreads();
-    auto store = [&](int r, int c, float4 x, float sum) {
+    // a row's result is (O / l) 2^(M - m), the power in two halves so that neither leaves float's range
+    auto store = [&](int r, int c, float4 x, float sum, float up) {
         const int rr = r0 + r;
         if (rr >= rows_total || failed) return;
         const int tok = rr / n_rep, head = g * n_rep + rr - tok * n_rep;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;                     // a row that sees nothing: zeros
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv, x.y * inv), hi = __floats2bfloat162_rn(x.z * inv, x.w * inv);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum, f = sum == 0.f ? 0.f : d8_ex2(0.5f * up);        // a row that sees nothing: zeros
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * f * f, x.y * inv * f * f), hi = __floats2bfloat162_rn(x.z * inv * f * f, x.w * inv * f * f);
         *reinterpret_cast<uint2*>(out + ((size_t)(q0 + tok) * p.nh + head) * HD + c) =
             make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
     };
     for (int i = threadIdx.x; i < ROWS * HD / 4; i += D8_WARPS * 32) {
         const int r = i / (HD / 4), c = i % (HD / 4) * 4;
-        float mx = -INFINITY, sum = 0.f;
+        float mx = -INFINITY, rx = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < D8_WARPS; ++w) mx = fmaxf(mx, sM[w][r]);
-        const float mu = mx == -INFINITY ? 0.f : mx;
+        for (int w = 0; w < D8_WARPS; ++w) { mx = fmaxf(mx, sM[w][r]); rx = fmaxf(rx, sR[w][r]); }
+        const float mu = mx == -INFINITY ? 0.f : mx, ru = rx == -INFINITY ? 0.f : rx;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < D8_WARPS; ++w) {
-            const float a = d8_ex2(sM[w][r] - mu);
+            const float a = d8_ex2(sR[w][r] - ru);
             const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(d8_smem + (size_t)w * D8_WARP_BYTES<HD>) + r * HD + c);
-            sum = fmaf(sL[w][r], a, sum);
+            sum = fmaf(sL[w][r], d8_ex2(sM[w][r] - mu), sum);
             x.x = fmaf(y.x, a, x.x); x.y = fmaf(y.y, a, x.y); x.z = fmaf(y.z, a, x.z); x.w = fmaf(y.w, a, x.w);
         }
         if (splits == 1) {
-            store(r, c, x, sum);
+            store(r, c, x, sum, ru - mu);
         } else {
             *reinterpret_cast<float4*>(&xO[r][c]) = x;
-            if (c == 0) { xM[r] = mx; xL[r] = sum; }
+            if (c == 0) { xM[r] = mx; xR[r] = rx; xL[r] = sum; }
         }
     }
     if (splits > 1) {
-        cluster_sync();                                                  // every block's result is in place
+        cluster_sync();                                                     // every block's result is in place
         for (int i = threadIdx.x * splits + rank; i < ROWS * HD / 4; i += D8_WARPS * 32 * splits) {
             const int r = i / (HD / 4), c = i % (HD / 4) * 4;
-            float mx = -INFINITY, sum = 0.f;
-            for (int j = 0; j < splits; ++j) mx = fmaxf(mx, cluster_f32(cluster_peer(&xM[r], (unsigned)j)));
-            const float mu = mx == -INFINITY ? 0.f : mx;
+            float mx = -INFINITY, rx = -INFINITY, sum = 0.f;
+            for (int j = 0; j < splits; ++j) {
+                mx = fmaxf(mx, cluster_f32(cluster_peer(&xM[r], (unsigned)j)));
+                rx = fmaxf(rx, cluster_f32(cluster_peer(&xR[r], (unsigned)j)));
+            }
+            const float mu = mx == -INFINITY ? 0.f : mx, ru = rx == -INFINITY ? 0.f : rx;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int j = 0; j < splits; ++j) {
-                const float a = d8_ex2(cluster_f32(cluster_peer(&xM[r], (unsigned)j)) - mu);
+                const float a = d8_ex2(cluster_f32(cluster_peer(&xR[r], (unsigned)j)) - ru), b = d8_ex2(cluster_f32(cluster_peer(&xM[r], (unsigned)j)) - mu);
                 const float4 y = cluster_f32x4(cluster_peer(&xO[r][c], (unsigned)j));
-                sum = fmaf(cluster_f32(cluster_peer(&xL[r], (unsigned)j)), a, sum);
+                sum = fmaf(cluster_f32(cluster_peer(&xL[r], (unsigned)j)), b, sum);
                 x.x = fmaf(y.x, a, x.x); x.y = fmaf(y.y, a, x.y); x.z = fmaf(y.z, a, x.z); x.w = fmaf(y.w, a, x.w);
             }
-            store(r, c, x, sum);
+            store(r, c, x, sum, ru - mu);
         }
-        cluster_sync();                                                  // nobody reads this block's memory any more
+        cluster_sync();                                                     // nobody reads this block's memory any more
     }
     if (threadIdx.x == 0 && failed && p.status) atomicExch(p.status, 16);
 }
