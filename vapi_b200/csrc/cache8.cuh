@@ -43,11 +43,9 @@ __device__ __forceinline__ unsigned char c8_code(float x) {
     return fabsf(x) < INFINITY ? (unsigned char)(c & 0xff) : (unsigned char)0x7f;
 }
 
-// Two codes (16 bits) as two halves, exactly; the low byte in the low half.
-__device__ __forceinline__ unsigned c8_halves(unsigned short c) {
-    unsigned h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-    return h;
+// Four codes as two pairs of halves, exactly; the lowest byte in the low half of `lo`.
+__device__ __forceinline__ void c8_halves4(unsigned c, unsigned& lo, unsigned& hi) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(c));
 }
 __device__ __forceinline__ float c8_half_lo(unsigned h) {
     float f;
@@ -58,7 +56,8 @@ __device__ __forceinline__ float c8_half_hi(unsigned h) { return c8_half_lo(h >>
 
 // Four codes as floats.
 __device__ __forceinline__ float4 c8_floats(unsigned c) {
-    const unsigned lo = c8_halves((unsigned short)(c & 0xffffu)), hi = c8_halves((unsigned short)(c >> 16));
+    unsigned lo, hi;
+    c8_halves4(c, lo, hi);
     return make_float4(c8_half_lo(lo), c8_half_hi(lo), c8_half_lo(hi), c8_half_hi(hi));
 }
 

@@ -28,7 +28,10 @@
 
 namespace vapi {
 
-constexpr int D8_WARPS = 8;
+#ifndef D8_WARPS_N
+#define D8_WARPS_N 8
+#endif
+constexpr int D8_WARPS = D8_WARPS_N;
 constexpr int D8_MAX_CLUSTER = 16;
 constexpr int D8_STAGES = 3;                                                           // of two chunks of K and of V
 constexpr float D8_RAISE = 8.f;                                                        // log2 units by which a score must pass a maximum to raise it
@@ -37,7 +40,7 @@ template <int HD> constexpr int D8_WARP_BYTES = D8_STAGES * 4 * D8_CHUNK<HD>;
 template <int HD> constexpr size_t D8_SMEM = (size_t)D8_WARPS * D8_WARP_BYTES<HD>;
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // an 8 x 8 matrix of 16-bit numbers, a row's pair of columns a lane, about its diagonal
@@ -70,9 +73,11 @@ __device__ __forceinline__ uint2 d8_lds8(unsigned addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
+template <int V> struct Number { static constexpr int value = V; };
+
 // WIDE: tiles of 16 rows, else of 8.
 template <int HD, bool WIDE>
-__global__ void __launch_bounds__(D8_WARPS * 32, HD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(D8_WARPS * 32, (HD == 64 ? 16 : 8) / D8_WARPS)
 decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int splits, const int most_q) {
     constexpr int ROWS = WIDE ? 16 : 8, H = WIDE ? 2 : 1, CHUNK = D8_CHUNK<HD>;
     constexpr int KS = HD / 16, Q64 = HD / 64, VW = HD / 32;                // k-steps of S; runs of 64 elements; words of a token's values that a lane holds
@@ -199,105 +204,134 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     // the pairs of rows that a lane of V^T has (2 tq, 2 tq + 1) are tokens tq and 4 + tq.
     const unsigned k_at = ((gq >> 1) + 4 * (gq & 1)) * HD + tq * 16, v_at = tq * HD + gq * (HD / 8);
     const int token = (gq >> 1) + 4 * (gq & 1);
-    auto chunk_of = [&](unsigned kb, unsigned vb, int k0, int e) {
-        float sc[H][4];
-#pragma unroll
-        for (int h = 0; h < H; ++h) sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
-#pragma unroll
-        for (int r = 0; r < Q64; ++r) {
-            const uint4 ca = d8_lds16(kb + k_at + r * 64), cb = d8_lds16(kb + k_at + 8 * HD + r * 64);
-            const unsigned wa[4] = {ca.x, ca.y, ca.z, ca.w}, wb[4] = {cb.x, cb.y, cb.z, cb.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned a0 = c8_halves((unsigned short)(wa[i] & 0xffffu)), a1 = c8_halves((unsigned short)(wb[i] & 0xffffu));
-                const unsigned a2 = c8_halves((unsigned short)(wa[i] >> 16)), a3 = c8_halves((unsigned short)(wb[i] >> 16));
-#pragma unroll
-                for (int h = 0; h < H; ++h) mma_f16_16816(sc[h], a0, a1, a2, a3, qf[h][4 * r + i][0], qf[h][4 * r + i][1]);
-            }
-        }
-        const float ek = c8_power((int)(signed char)(e & 0xff)), ev = (float)(signed char)(e >> 8 & 0xff);
-        const bool edge = k0 + C8_BLOCK - 1 > p_min || (p.window > 0 && k0 <= p_max - p.window);
+    // N chunks at once (two, or the last one alone): their products do not wait for one another
+    auto work = [&](auto number, unsigned kb, int k0, const int (&e)[2]) {
+        constexpr int N = decltype(number)::value;
+        const unsigned vb = kb + 2 * CHUNK;
+        float sc[N][H][4], ev[N];
         bool raise = false;
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+        for (int j = 0; j < N; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {                                   // row 2 tq + i: its scores of tokens `token` and 8 further on
-                float &x = sc[h][i], &y = sc[h][2 + i];
-                const float f = row_f[h][i] * ek;
-                x *= f;
-                y *= f;
-                if (edge) {
-                    const int pos = row_pos[h][i], kx = k0 + token, ky = kx + 8;
-                    x = kx <= pos && kx < klen && (p.window <= 0 || kx > pos - p.window) ? x : -INFINITY;
-                    y = ky <= pos && ky < klen && (p.window <= 0 || ky > pos - p.window) ? y : -INFINITY;
+            for (int h = 0; h < H; ++h) sc[j][h][0] = sc[j][h][1] = sc[j][h][2] = sc[j][h][3] = 0.f;
+#pragma unroll
+        for (int r = 0; r < Q64; ++r)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint4 ca = d8_lds16(kb + j * CHUNK + k_at + r * 64), cb = d8_lds16(kb + j * CHUNK + k_at + 8 * HD + r * 64);
+                const unsigned wa[4] = {ca.x, ca.y, ca.z, ca.w}, wb[4] = {cb.x, cb.y, cb.z, cb.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned a0, a1, a2, a3;
+                    c8_halves4(wa[i], a0, a2);
+                    c8_halves4(wb[i], a1, a3);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) mma_f16_16816(sc[j][h], a0, a1, a2, a3, qf[h][4 * r + i][0], qf[h][4 * r + i][1]);
                 }
-                const float mx = fmaxf(x, y);
-                raise |= mx > m[h][i] + D8_RAISE || mx + ev > big[h][i] + D8_RAISE;
             }
+        const bool edge = k0 + N * C8_BLOCK - 1 > p_min || (p.window > 0 && k0 <= p_max - p.window);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float ek = c8_power((int)(signed char)(e[j] & 0xff));
+            ev[j] = (float)(signed char)(e[j] >> 8 & 0xff);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {                               // row 2 tq + i: its scores of tokens `token` and 8 further on
+                    float &x = sc[j][h][i], &y = sc[j][h][2 + i];
+                    const float f = row_f[h][i] * ek;
+                    x *= f;
+                    y *= f;
+                    if (edge) {
+                        const int pos = row_pos[h][i], kx = k0 + j * C8_BLOCK + token, ky = kx + 8;
+                        x = kx <= pos && kx < klen && (p.window <= 0 || kx > pos - p.window) ? x : -INFINITY;
+                        y = ky <= pos && ky < klen && (p.window <= 0 || ky > pos - p.window) ? y : -INFINITY;
+                    }
+                    const float mx = fmaxf(x, y);
+                    raise |= mx > m[h][i] + D8_RAISE || mx + ev[j] > big[h][i] + D8_RAISE;
+                }
+        }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float mx = fmaxf(sc[h][i], sc[h][2 + i]);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    float mx = -INFINITY, rx = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const float x = fmaxf(sc[j][h][i], sc[j][h][2 + i]);
+                        mx = fmaxf(mx, x);
+                        rx = fmaxf(rx, x + ev[j]);
+                    }
+#pragma unroll
+                    for (int k = 4; k < 32; k *= 2) {
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                        rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, k));
+                    }
                     if (mx > m[h][i]) {                                     // (m = -inf: the factor is 0, and the sum is 0)
                         l[h][i] *= d8_ex2(m[h][i] - mx);
                         m[h][i] = mx;
                     }
-                    if (mx + ev > big[h][i]) {
-                        const float f = d8_ex2(big[h][i] - (mx + ev));
+                    if (rx > big[h][i]) {
+                        const float f = d8_ex2(big[h][i] - rx);
 #pragma unroll
                         for (int t = 0; t < HD / 16; ++t) { o[h][t][i] *= f; o[h][t][2 + i] *= f; }
-                        big[h][i] = mx + ev;
+                        big[h][i] = rx;
                     }
                 }
         }
-        unsigned pt[H][2];
+        unsigned pt[N][H][2];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            float w[4];
+            // (a row that has seen nothing: its scores are -inf, and stay so)
+            const float mu[2] = {m[h][0] == -INFINITY ? 0.f : m[h][0], m[h][1] == -INFINITY ? 0.f : m[h][1]};
+            const float ru[2] = {m[h][0] == -INFINITY ? 0.f : big[h][0], m[h][1] == -INFINITY ? 0.f : big[h][1]};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                // (a row that has seen nothing: its scores are -inf, and stay so)
-                const float mu = m[h][i] == -INFINITY ? 0.f : m[h][i], up = m[h][i] == -INFINITY ? 0.f : ev - big[h][i];
-                w[i] = d8_ex2(sc[h][i] + up);
-                w[2 + i] = d8_ex2(sc[h][2 + i] + up);
-                l[h][i] += d8_ex2(sc[h][i] - mu) + d8_ex2(sc[h][2 + i] - mu);
-            }
-            pt[h][0] = d8_turned(d8_half2(w[0], w[1]));
-            pt[h][1] = d8_turned(d8_half2(w[2], w[3]));
-        }
-        // the values of tokens tq, 4 + tq, 8 + tq, 12 + tq: HD / 8 elements from gq * (HD / 8) on
-        unsigned v[4][VW];
+            for (int j = 0; j < N; ++j) {
+                float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned at = vb + v_at + 4 * i * HD;
-            if (HD == 64) {
-                const uint2 x = d8_lds8(at);
-                v[i][0] = x.x; v[i][1] = x.y;
-            } else {
-                const uint4 x = d8_lds16(at);
-                v[i][0] = x.x; v[i][1] = x.y; v[i][VW - 2] = x.z; v[i][VW - 1] = x.w;
-            }
-            if (k0 + C8_BLOCK > klen && k0 + 4 * i + tq >= klen) {
-#pragma unroll
-                for (int c = 0; c < VW; ++c) v[i][c] = 0u;
+                for (int i = 0; i < 2; ++i) {
+                    const float up = ev[j] - ru[i];
+                    w[i] = d8_ex2(sc[j][h][i] + up);
+                    w[2 + i] = d8_ex2(sc[j][h][2 + i] + up);
+                    l[h][i] += d8_ex2(sc[j][h][i] - mu[i]) + d8_ex2(sc[j][h][2 + i] - mu[i]);
+                }
+                pt[j][h][0] = d8_turned(d8_half2(w[0], w[1]));
+                pt[j][h][1] = d8_turned(d8_half2(w[2], w[3]));
             }
         }
-        // tile t of O^T: rows gq and 8 + gq are elements gq * (HD / 8) + 2t and + 1
 #pragma unroll
-        for (int c = 0; c < VW; ++c) {
-            const unsigned x01[2] = {__byte_perm(v[0][c], v[1][c], 0x5140), __byte_perm(v[0][c], v[1][c], 0x7362)};
-            const unsigned x23[2] = {__byte_perm(v[2][c], v[3][c], 0x5140), __byte_perm(v[2][c], v[3][c], 0x7362)};
+        for (int j = 0; j < N; ++j) {
+            // the values of tokens tq, 4 + tq, 8 + tq, 12 + tq: HD / 8 elements from gq * (HD / 8) on
+            unsigned v[4][VW];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const unsigned a0 = c8_halves((unsigned short)(x01[i] & 0xffffu)), a1 = c8_halves((unsigned short)(x01[i] >> 16));
-                const unsigned a2 = c8_halves((unsigned short)(x23[i] & 0xffffu)), a3 = c8_halves((unsigned short)(x23[i] >> 16));
+            for (int i = 0; i < 4; ++i) {
+                const unsigned at = vb + j * CHUNK + v_at + 4 * i * HD;
+                if (HD == 64) {
+                    const uint2 x = d8_lds8(at);
+                    v[i][0] = x.x; v[i][1] = x.y;
+                } else {
+                    const uint4 x = d8_lds16(at);
+                    v[i][0] = x.x; v[i][1] = x.y; v[i][VW - 2] = x.z; v[i][VW - 1] = x.w;
+                }
+                if (edge && k0 + j * C8_BLOCK + 4 * i + tq >= klen) {
 #pragma unroll
-                for (int h = 0; h < H; ++h) mma_f16_16816(o[h][2 * c + i], a0, a1, a2, a3, pt[h][0], pt[h][1]);
+                    for (int c = 0; c < VW; ++c) v[i][c] = 0u;
+                }
+            }
+            // tile t of O^T: rows gq and 8 + gq are elements gq * (HD / 8) + 2t and + 1
+#pragma unroll
+            for (int c = 0; c < VW; ++c) {
+                const unsigned x01[2] = {__byte_perm(v[0][c], v[1][c], 0x5140), __byte_perm(v[0][c], v[1][c], 0x7362)};
+                const unsigned x23[2] = {__byte_perm(v[2][c], v[3][c], 0x5140), __byte_perm(v[2][c], v[3][c], 0x7362)};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    unsigned a0, a1, a2, a3;
+                    c8_halves4(x01[i], a0, a1);
+                    c8_halves4(x23[i], a2, a3);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) mma_f16_16816(o[h][2 * c + i], a0, a1, a2, a3, pt[j][h][0], pt[j][h][1]);
+                }
             }
         }
     };
@@ -310,9 +344,10 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             break;
         }
         const unsigned kb = ring + stage * 4 * CHUNK;
-        const int k0 = (begin + 2 * it) * C8_BLOCK, e0 = __shfl_sync(0xffffffffu, scales, (2 * it) & 31), e1 = __shfl_sync(0xffffffffu, scales, (2 * it + 1) & 31);
-        chunk_of(kb, kb + 2 * CHUNK, k0, e0);
-        if (2 * it + 1 < nt) chunk_of(kb + CHUNK, kb + 3 * CHUNK, k0 + C8_BLOCK, e1);
+        const int k0 = (begin + 2 * it) * C8_BLOCK;
+        const int e[2] = {__shfl_sync(0xffffffffu, scales, (2 * it) & 31), __shfl_sync(0xffffffffu, scales, (2 * it + 1) & 31)};
+        if (2 * it + 1 < nt) work(Number<2>(), kb, k0, e);
+        else work(Number<1>(), kb, k0, e);
         __syncwarp();                                                       // every lane has what it wants of this place
         if (it + D8_STAGES < pairs) bring(it + D8_STAGES, stage);
         if ((it & 15) == 15) scales = scales_next;                          // (the look-up of the next 32 is behind us)

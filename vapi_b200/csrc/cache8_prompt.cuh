@@ -35,10 +35,7 @@ __device__ __forceinline__ void p8_halves(const uint4& c, uint4& lo, uint4& hi) 
     const unsigned w[4] = {c.x, c.y, c.z, c.w};
     unsigned h[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h[2 * i] = c8_halves((unsigned short)(w[i] & 0xffffu));
-        h[2 * i + 1] = c8_halves((unsigned short)(w[i] >> 16));
-    }
+    for (int i = 0; i < 4; ++i) c8_halves4(w[i], h[2 * i], h[2 * i + 1]);
     lo = make_uint4(h[0], h[1], h[2], h[3]);
     hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
