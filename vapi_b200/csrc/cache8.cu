@@ -19,7 +19,7 @@
 using namespace vapi;
 
 // ---- the write ----------------------------------------------------------------------------------
-// One warp per (token, head) of a fused row [q heads | k heads | v heads]:
+// The general kernel: one warp per (token, head) of a fused row [q heads | k heads | v heads]:
 //   q: norm (if qw) -> rotation (if cosr) -> q_out;
 //   k, v: a warp takes all the step's tokens of its block of 16, if its token is the first of them (slots that follow one
 //   another within a block), else it has nothing to do.  First pass: the largest magnitude (k normed, rotated and rounded to the
@@ -129,6 +129,176 @@ write8_kernel(const T* __restrict__ qkv, const float* __restrict__ qw, const flo
     }
 }
 
+// The same for bfloat16, head size 64 or 128 and a rotation over the whole head (or none), with 16-byte accesses and in one pass: D / 16
+// lanes take one (token, head), a lane 8 elements of the first half and their partners of the second.  The blocks before `q_blocks`
+// take the queries; a warp of the others one head's keys or values of `GROUP` tokens of the step, and of these the runs that begin
+// among them: 32 / (D / 16) tokens of a run at a time, all of whose loads are under way together, kept as bfloat16 until
+// the block's scale is known.  GROUP 16 for prompts (a run begins in every 16 tokens, but for the ends), 1 for decode steps, where
+// each token is a run and 16 of them in a row would be a warp's alone.
+template <int D>
+struct W8Row {                                     // 8 + 8 elements of a (token, head), normed, rotated and rounded
+    uint4 lo, hi;
+    __device__ __forceinline__ void load(const __nv_bfloat16* src, bool ok, const float* w, float eps, const float* cosr, const float* sinr, int e) {
+        constexpr int G = D / 16;
+        float a[8], b[8];
+        const uint4 ra = ok ? *reinterpret_cast<const uint4*>(src + e) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 rb = ok ? *reinterpret_cast<const uint4*>(src + D / 2 + e) : make_uint4(0u, 0u, 0u, 0u);
+        const unsigned wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[2 * i] = __uint_as_float(wa[i] << 16); a[2 * i + 1] = __uint_as_float(wa[i] & 0xffff0000u);
+            b[2 * i] = __uint_as_float(wb[i] << 16); b[2 * i + 1] = __uint_as_float(wb[i] & 0xffff0000u);
+        }
+        if (w) {                                   // (the same for the whole warp)
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = rsqrtf(ss / (float)D + eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] = a[i] * inv * w[e + i];
+                b[i] = b[i] * inv * w[D / 2 + e + i];
+            }
+        }
+        if (cosr && ok) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(cosr + e + i), s = *reinterpret_cast<const float4*>(sinr + e + i);
+                const float cc[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float x = a[i + k], y = b[i + k];
+                    a[i + k] = x * cc[k] - y * sn[k];
+                    b[i + k] = y * cc[k] + x * sn[k];
+                }
+            }
+        }
+        lo = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(a[4], a[5]), pack_bf16(a[6], a[7]));
+        hi = make_uint4(pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3]), pack_bf16(b[4], b[5]), pack_bf16(b[6], b[7]));
+    }
+    // the largest finite magnitude
+    __device__ __forceinline__ float largest() const {
+        const unsigned w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = fabsf(__uint_as_float(w[i] << 16)), y = fabsf(__uint_as_float(w[i] & 0xffff0000u));
+            m = x < INFINITY ? fmaxf(m, x) : m;
+            m = y < INFINITY ? fmaxf(m, y) : m;
+        }
+        return m;
+    }
+    static __device__ __forceinline__ uint2 codes(const uint4& v, float f) {
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+        unsigned c[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            c[i] = c8_codes4(__uint_as_float(w[2 * i] << 16) * f, __uint_as_float(w[2 * i] & 0xffff0000u) * f, __uint_as_float(w[2 * i + 1] << 16) * f,
+                             __uint_as_float(w[2 * i + 1] & 0xffff0000u) * f);
+        return make_uint2(c[0], c[1]);
+    }
+};
+
+template <int D, int GROUP>
+__global__ void __launch_bounds__(W8_WARPS * 32)
+write8_vec_kernel(const __nv_bfloat16* __restrict__ qkv, const float* __restrict__ qw, const float* __restrict__ kw, float eps, const float* __restrict__ cosr,
+                  const float* __restrict__ sinr, __nv_bfloat16* __restrict__ q_out, unsigned char* __restrict__ codes, signed char* __restrict__ exps,
+                  const int* __restrict__ slots, int n, int nh, int nkv, int page_size, int num_pages, int q_blocks, int* __restrict__ status) {
+    constexpr int G = D / 16, TOKENS = 32 / G, PASSES = C8_BLOCK / TOKENS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane / G, e = lane % G * 8;
+    const int heads = nh + 2 * nkv;
+    pdl_trigger();
+    if ((int)blockIdx.x < q_blocks) {
+        pdl_wait();
+        const long long item = ((long long)blockIdx.x * W8_WARPS + warp) * TOKENS + part;
+        const bool ok = item < (long long)n * nh;
+        const int t = ok ? (int)(item / nh) : 0, h = ok ? (int)(item - (long long)t * nh) : 0;
+        W8Row<D> r;
+        r.load(qkv + ((size_t)t * heads + h) * D, ok, qw, eps, cosr ? cosr + (size_t)t * (D / 2) : nullptr, sinr ? sinr + (size_t)t * (D / 2) : nullptr, e);
+        if (ok) {
+            __nv_bfloat16* dst = q_out + (size_t)item * D + e;
+            *reinterpret_cast<uint4*>(dst) = r.lo;
+            *reinterpret_cast<uint4*>(dst + D / 2) = r.hi;
+        }
+        return;
+    }
+    const long long item = (long long)(blockIdx.x - q_blocks) * W8_WARPS + warp;
+    const int t0 = (int)(item / (2 * nkv)) * GROUP, hk = (int)(item % (2 * nkv));
+    if (t0 >= n) {
+        pdl_wait();
+        return;
+    }
+    // where runs begin (slots are host-copied index data: safe before the wait)
+    const int at = min(t0 + lane, n - 1), mine = slots[at];
+    const bool first = lane < GROUP && t0 + lane < n && (at == 0 || (mine & (C8_BLOCK - 1)) == 0 || mine < 0 || slots[at - 1] != mine - 1);
+    unsigned runs = __ballot_sync(0xffffffffu, first);
+    pdl_wait();
+    const bool is_k = hk < nkv;
+    const int g = is_k ? hk : hk - nkv;
+    for (; runs; runs &= runs - 1) {
+        const int j0 = __ffs(runs) - 1, t = t0 + j0, slot = __shfl_sync(0xffffffffu, mine, j0);
+        const int page = slot / page_size, off = slot - page * page_size, place = off & (C8_BLOCK - 1);
+        const bool follows = lane < C8_BLOCK && place + lane < C8_BLOCK && t + lane < n && slots[min(t + lane, n - 1)] == slot + lane;
+        const int count = __ffs(~__ballot_sync(0xffffffffu, follows)) - 1;
+        if (slot < 0 || page >= num_pages) {
+            if (lane == 0 && status) atomicExch(status, 2);
+            continue;
+        }
+        W8Row<D> r[PASSES];
+        float amax = 0.f;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int j = p * TOKENS + part;
+            const bool ok = j < count;
+            const size_t row = ok ? t + j : t;
+            r[p].load(qkv + (row * heads + nh + hk) * D, ok, is_k ? kw : nullptr, eps, is_k && cosr ? cosr + row * (D / 2) : nullptr,
+                      is_k && sinr ? sinr + row * (D / 2) : nullptr, e);
+            amax = fmaxf(amax, r[p].largest());
+        }
+        int x = c8_exponent(warp_max(amax));
+        const size_t head = ((size_t)page * 2 + (is_k ? 0 : 1)) * nkv + g;
+        unsigned char* block = codes + (head * page_size + off - place) * D;
+        signed char* exp_at = exps + head * (page_size / C8_BLOCK) + off / C8_BLOCK;
+        if (place > 0) {
+            const int old = *exp_at;
+            x = max(x, old);
+            if (x > old) {                                         // the block's older tokens
+                unsigned* older = reinterpret_cast<unsigned*>(block);
+                const float f = c8_power(max(old - x, -126));
+                for (int i = lane; i < place * D / 4; i += 32) older[i] = c8_rescale(older[i], f);
+            }
+        }
+        __syncwarp();                                              // every lane has read the old exponent
+        if (lane == 0) *exp_at = (signed char)x;
+        const float f = c8_power(-x);
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int j = p * TOKENS + part;
+            if (j >= count) continue;
+            unsigned char* dst = block + (place + j) * D + e;
+            *reinterpret_cast<uint2*>(dst) = W8Row<D>::codes(r[p].lo, f);
+            *reinterpret_cast<uint2*>(dst + D / 2) = W8Row<D>::codes(r[p].hi, f);
+        }
+    }
+}
+
+// tokens of a step from which on a warp takes 16 of them
+constexpr int W8_GROUP_TOKENS = 512;
+
+template <int D>
+static int launch_write8_vec(const void* qkv, const float* qw, const float* kw, float eps, const float* cosr, const float* sinr, void* q_out, void* codes, void* exps,
+                             const int* slots, int n, int nh, int nkv, int page_size, int num_pages, int* status, cudaStream_t stream) {
+    const int group = n >= W8_GROUP_TOKENS ? C8_BLOCK : 1;
+    const long long per = (long long)W8_WARPS * (32 / (D / 16)), q_blocks = ((long long)n * nh + per - 1) / per;
+    const long long blocks = q_blocks + ((long long)((n + group - 1) / group) * 2 * nkv + W8_WARPS - 1) / W8_WARPS;
+    if (blocks > 0x7fffffffLL) return fail(-1, "qk_norm_rope_write8: %d tokens exceed the grid", n);
+    return check_launch("qk_norm_rope_write8", launch(group == 1 ? write8_vec_kernel<D, 1> : write8_vec_kernel<D, C8_BLOCK>, (unsigned)blocks, W8_WARPS * 32, 0, stream,
+                                                      (const __nv_bfloat16*)qkv, qw, kw, eps, cosr, sinr, (__nv_bfloat16*)q_out, (unsigned char*)codes,
+                                                      (signed char*)exps, slots, n, nh, nkv, page_size, num_pages, (int)q_blocks, status));
+}
+
 VAPI_EXPORT int vapi_qk_norm_rope_write8(const void* qkv, int dtype, const float* qw, const float* kw, float eps, const float* cosr,
                                          const float* sinr, int rot, void* q_out, void* codes, void* exps, const int* slots, int n,
                                          int nh, int nkv, int d, int page_size, int num_pages, int* status, cudaStream_t stream) {
@@ -137,6 +307,11 @@ VAPI_EXPORT int vapi_qk_norm_rope_write8(const void* qkv, int dtype, const float
     if (nh <= 0 || nkv <= 0) return fail(-1, "qk_norm_rope_write8: no heads");
     if (cosr && (rot <= 0 || rot > d || rot % 2 != 0)) return fail(-1, "qk_norm_rope_write8: rotation width %d does not fit head_dim %d", rot, d);
     if (page_size <= 0 || page_size % C8_BLOCK != 0 || num_pages <= 0) return fail(-1, "qk_norm_rope_write8: page size %d is not a multiple of 16, or there are no pages", page_size);
+    // (16-byte rows of everything that is read or written by the piece)
+    if (dtype == VAPI_BF16 && (d == 64 || d == 128) && (!cosr || rot == d) &&
+        (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)codes | (uintptr_t)cosr | (uintptr_t)sinr) & 15) == 0)
+        return d == 64 ? launch_write8_vec<64>(qkv, qw, kw, eps, cosr, sinr, q_out, codes, exps, slots, n, nh, nkv, page_size, num_pages, status, stream)
+                       : launch_write8_vec<128>(qkv, qw, kw, eps, cosr, sinr, q_out, codes, exps, slots, n, nh, nkv, page_size, num_pages, status, stream);
     const long long blocks = ((long long)n * (nh + 2 * nkv) + W8_WARPS - 1) / W8_WARPS;
     if (blocks > 0x7fffffffLL) return fail(-1, "qk_norm_rope_write8: %d tokens exceed the grid", n);
     cudaError_t e;

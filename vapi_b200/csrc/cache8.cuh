@@ -43,6 +43,17 @@ __device__ __forceinline__ unsigned char c8_code(float x) {
     return fabsf(x) < INFINITY ? (unsigned char)(c & 0xff) : (unsigned char)0x7f;
 }
 
+// Four codes, x the lowest byte.
+__device__ __forceinline__ unsigned c8_codes4(float x, float y, float z, float w) {
+    unsigned short lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y), "f"(x));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(w), "f"(z));
+    unsigned c = (unsigned)lo | (unsigned)hi << 16;
+    if (!(fmaxf(fmaxf(fabsf(x), fabsf(y)), fmaxf(fabsf(z), fabsf(w))) < INFINITY) || x != x || y != y || z != z || w != w)
+        c = (unsigned)c8_code(x) | (unsigned)c8_code(y) << 8 | (unsigned)c8_code(z) << 16 | (unsigned)c8_code(w) << 24;
+    return c;
+}
+
 // Four codes as two pairs of halves, exactly; the lowest byte in the low half of `lo`.
 __device__ __forceinline__ void c8_halves4(unsigned c, unsigned& lo, unsigned& hi) {
     asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(c));
