@@ -136,7 +136,7 @@ def unpack(w):
         for p in range(2):
             for e in range(2):
                 codes[:, h, :, :, :, :, :, p, e] = ((lanes >> (8 * p + 4 * h + 16 * e)) & 15).permute(0, 2, 1, 4, 3, 5).to(torch.uint8)
-    table = pairs.permute(0, 3, 2, 1).reshape(tiles * 16, -1)[:w.n]
+    table = pairs.permute(0, 3, 2, 1).reshape(tiles * 16, -1)[:w.n, :w.k // w.group]
     number = lambda t: (t & 0xffff).to(torch.int16).view(torch.bfloat16)
     return codes.reshape(tiles * 16, chunks * 64)[:w.n, :w.k], number(table), number(table >> 16) - 128
 

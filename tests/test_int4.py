@@ -103,7 +103,7 @@ SIZES = [(16, 32, 32), (1, 64, 64), (48, 128, 128), (33, 96, 32), (200, 512, 64)
 
 @gpu
 @pytest.mark.parametrize("n,k,group", SIZES)
-@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 24, 25, 32, 33, 64])
 def test_few_rows(n, k, group, rows):
     ops = _ops()
     w = ops.int4_pack(*_random(n, k, group, n + k))

@@ -360,7 +360,7 @@ PyObject* int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         const at::Tensor& x = on(need(a[6], at::kBFloat16, 2), device);
         if (!fn || x.size(1) != k || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0 || (gated && (f32 || a[7] != Py_None))) throw Bad{};
         const int64_t tiles = (n + 15LL) / 16;
-        if (n <= 0 || k <= 0 || group <= 0 || codes.numel() != tiles * ((k + 63LL) / 64) * 128 || scales.numel() != tiles * (k / group) * 16) throw Bad{};
+        if (n <= 0 || k <= 0 || group <= 0 || codes.numel() != tiles * ((k + 63LL) / 64) * 128 || scales.numel() != tiles * (group == 32 ? (k + 63LL) / 64 * 2 : k / group) * 16) throw Bad{};
         const int rows = size32(x.size(0));
         const float* bias = floats_on(a[7], n, device);
         void* stream = address(a[11]);

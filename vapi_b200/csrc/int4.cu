@@ -9,7 +9,7 @@
 // float sums and the result.  The order of 32 columns (the smallest group) is free as long as x follows it: a lane's 8 columns of
 // x are 16 bytes in one piece, its B operands of two k-steps.
 //
-// Scales: for each tile row and group 8 pairs of words, word = scale | (128 + zero) << 16 as two bfloat16, rows l/4 and l/4 + 8.
+// Scales: for each tile row and group (of 32: two for every 64 columns, the last perhaps of nothing) 8 pairs of words, word = scale | (128 + zero) << 16 as two bfloat16, rows l/4 and l/4 + 8.
 #include "cluster.cuh"
 #include "attention_mma.cuh"       // mma_bf16_16816
 
@@ -31,7 +31,8 @@ struct I4Params {
 
 // two codes, `shift` and 16 + shift bits up, less their row's zero
 __device__ __forceinline__ unsigned i4_pair(unsigned w, int shift, __nv_bfloat162 zero) {
-    const unsigned u = ((w >> shift) & 0x000f000fu) | 0x43004300u;
+    unsigned u;                                    // (one operation: the two constants in registers)
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w >> shift), "r"(0x000f000fu), "r"(0x43004300u));
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), zero);
     return *reinterpret_cast<const unsigned*>(&d);
 }
@@ -42,154 +43,214 @@ __device__ __forceinline__ __nv_bfloat162 i4_zero(unsigned w) {
 __device__ __forceinline__ float i4_scale(unsigned w) { return __uint_as_float(w << 16); }
 
 // ---- few rows -------------------------------------------------------------------------------------
-// A block owns RT tile rows (16 features each; a gated product's are one of the gate and one of up) and 8 NT rows of x; its
-// eight warps, and the blocks of a cluster, share out the columns, 64 at a time.  Weights go from memory to registers, AHEAD tiles of
-// each tile row under way; those that a warp asks for first do not wait for the kernel before (weights are nobody's output).
-// Partial results are added in warp order, then in block order.
-constexpr int I4_AHEAD = 4;
+// A block owns WN tile rows (16 features each; for a gated product half of them the gate's and half up's) and 8 NT rows of x; its eight
+// warps are WN tile rows x 8 / WN slices of the block's columns, and the blocks of a cluster share out the columns further.
+// Weights and scales go from memory to registers, AHEAD tiles of a warp under way; those that it asks for first do not wait for the
+// kernel before (weights are nobody's output).  x comes to shared memory once a block, a segment of columns at a time, for all its
+// warps: with 8 NT rows, x is NT / 4 times as many bytes a column as a tile row's weights, and read for every tile row alone it
+// would be most of the traffic.  Partial results are added in the order of slices, then of blocks.
+constexpr int I4_PART = 8 * 16;                    // rows of partial results: eight warps x 16 features
 
-template <int NT, int RT, int GS, bool GLU>        // GS: k-steps of 16 columns a group (2, 4, 8)
-__global__ void __launch_bounds__(I4_WARPS * 32, NT == 4 ? 1 : 2)
-int4_rows_kernel(const I4Params p, const int splits) {
-    __shared__ __align__(16) float part[I4_WARPS][RT][16][8 * NT + 1];
+template <int NT> constexpr int I4_SEG = NT >= 3 ? 16 : 32;              // tiles of columns of x that shared memory holds at most
+template <int NT> constexpr int I4_AHEAD = NT >= 3 ? 4 : 6;
+
+template <int NT, int GS, bool GLU>                // GS: k-steps of 16 columns a group (2, 4, 8)
+__global__ void __launch_bounds__(I4_WARPS * 32, 2)
+int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg) {
+    constexpr int AHEAD = I4_AHEAD<NT>, CPG = GS > 4 ? GS / 4 : 1, GPC = GS < 4 ? 4 / GS : 1;      // tiles a group; groups a tile
+    extern __shared__ __align__(16) unsigned char i4_smem[];
+    float (*part)[8 * NT + 1] = reinterpret_cast<float (*)[8 * NT + 1]>(i4_smem);
+    __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(i4_smem + ((I4_PART * (8 * NT + 1) * 4 + 15) & ~15));
+    constexpr int PITCH = I4_SEG<NT> * 64 + 32;    // (64 bytes more than whole tiles: two rows of a quarter of a warp are in unlike banks)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int rank = (int)blockIdx.x % splits, tile = (int)blockIdx.x / splits, r0 = blockIdx.y * 8 * NT;
-    const int tiles = (p.n + 15) / 16, groups = p.k / p.group;
+    const int rank = (int)blockIdx.x % splits, block = (int)blockIdx.x / splits, r0 = blockIdx.y * 8 * NT;
+    const int tiles = (p.n + 15) / 16, groups = GS < 4 ? p.chunks * GPC : p.k / p.group;
+    const int tn = warp % wn, tk = warp / wn, wk = I4_WARPS / wn;
     pdl_trigger();
-    int t[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) t[r] = GLU ? tile + r * (tiles / 2) : min(tile * RT + r, tiles - 1);
-    const int units = splits * I4_WARPS, unit = rank * I4_WARPS + warp;
-    // (a group's columns stay with one warp: groups of two tiles are handed out whole)
-    constexpr int CPG = GS > 4 ? GS / 4 : 1;       // tiles a group
+    // this warp's tile row: a gated block has wn / 2 of the gate and the same of up
+    const int half = wn / 2;
+    const int mine = GLU ? (tn < half ? block * half + tn : tiles / 2 + block * half + tn - half) : block * wn + tn;
+    const bool real = GLU ? block * half + tn % half < tiles / 2 : mine < tiles;
+    const int t = real ? mine : 0;
+    // (a group's columns stay with one warp)
     const int whole = (p.chunks + CPG - 1) / CPG;
-    const int begin = (int)((long long)whole * unit / units) * CPG, end = min(p.chunks, (int)((long long)whole * (unit + 1) / units) * CPG);
+    const int from = (int)((long long)whole * rank / splits) * CPG, upto = min(p.chunks, (int)((long long)whole * (rank + 1) / splits) * CPG);
 
-    uint4 w[I4_AHEAD][RT];
-    auto bring = [&](int ch, uint4 (&to)[RT]) {
+    float total[NT][4], sum[NT][4];
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-            to[r] = ch < end ? __ldg(reinterpret_cast<const uint4*>(p.codes) + ((size_t)t[r] * p.chunks + ch) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
-    };
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int i = 0; i < I4_AHEAD; ++i) bring(begin + i, w[i]);
-    float total[RT][NT][4], sum[RT][NT][4];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) total[r][n][i] = sum[r][n][i] = 0.f;
-    pdl_wait();
+        for (int i = 0; i < 4; ++i) total[n][i] = sum[n][i] = 0.f;
 
-    for (int base = begin; base < end; base += I4_AHEAD) {
+    const uint4* codes = reinterpret_cast<const uint4*>(p.codes) + (size_t)t * p.chunks * 32 + lane;
+    const uint2* scales = reinterpret_cast<const uint2*>(p.scales) + (size_t)t * groups * 8 + g;
+    bool waited = false;
+    for (int s0 = from; s0 < upto; s0 += seg) {
+        const int tiles_here = min(seg, upto - s0), groups_here = (tiles_here + CPG - 1) / CPG;
+        const int begin = s0 + groups_here * tk / wk * CPG, end = min(s0 + tiles_here, s0 + groups_here * (tk + 1) / wk * CPG);
+        uint4 w[AHEAD];
+        uint2 sc[AHEAD][GPC];
+        const uint4* wp = codes + (size_t)begin * 32;
+        const uint2* sp = scales + (size_t)(GS < 4 ? begin * GPC : begin / CPG) * 8;
+        auto bring = [&](int ch, uint4& to, uint2 (&ts)[GPC]) {            // tile after tile; nothing behind the last is used
+            if (ch < end) {
+                to = __ldg(wp);
 #pragma unroll
-        for (int i = 0; i < I4_AHEAD; ++i) {
-            const int ch = base + i;
-            if (ch >= end) break;
-            // x: 8 and 8 columns of rows g, 8 + g ..
-            uint4 xa[NT], xb[NT];
-            const int col = ch * 64 + c * 8;
+                for (int i = 0; i < GPC; ++i) ts[i] = __ldg(sp + 8 * i);
+            }
+            wp += 32;
+            if (CPG == 1 || (ch & 1)) sp += 8 * GPC;
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) bring(begin + i, w[i], sc[i]);
+        if (!waited) { pdl_wait(); waited = true; }
+        else __syncthreads();                      // (the segment before is read)
+        {
+            // a warp has every eighth row, a lane every 32nd 16 bytes of it
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int row = r0 + 8 * n + g;
-                const uint4* src = reinterpret_cast<const uint4*>(p.x + (size_t)row * p.k + col);
-                const bool ok = row < p.rows;
-                xa[n] = ok && col < p.k ? src[0] : make_uint4(0u, 0u, 0u, 0u);
-                xb[n] = ok && col + 32 < p.k ? src[4] : make_uint4(0u, 0u, 0u, 0u);
+                const int row = 8 * n + warp;
+                const bool ok = r0 + row < p.rows;
+                const __nv_bfloat16* src = p.x + (ok ? (size_t)(r0 + row) * p.k : 0) + s0 * 64;
+                for (int i = lane * 8; i < tiles_here * 64; i += 256) {
+                    const bool in = ok && s0 * 64 + i < p.k;
+                    cp_async_16(sx + row * PITCH + i, in ? src + i : p.x, in ? 16 : 0);
+                }
             }
+            cp_async_commit();
+            cp_async_wait<0>();
+        }
+        __syncthreads();
+        const __nv_bfloat16* xr = sx + g * PITCH + c * 8 + (begin - s0) * 64;
+        for (int base = begin; base < end; base += AHEAD) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const unsigned words[4] = {w[i][r].x, w[i][r].y, w[i][r].z, w[i][r].w};
+            for (int i = 0; i < AHEAD; ++i) {
+                const int ch = base + i;
+                if (ch >= end) break;
+                uint4 xa[NT], xb[NT];
 #pragma unroll
-                for (int part_of = 0; part_of < (GS < 4 ? 4 / GS : 1); ++part_of) {
-                    const int group = min(GS < 4 ? ch * 2 + part_of : ch / CPG, groups - 1);      // (columns behind the last: x is zero there)
-                    const uint2 sc = __ldg(reinterpret_cast<const uint2*>(p.scales) + ((size_t)t[r] * groups + group) * 8 + g);
-                    const __nv_bfloat162 z0 = i4_zero(sc.x), z1 = i4_zero(sc.y);
+                for (int n = 0; n < NT; ++n) {
+                    xa[n] = *reinterpret_cast<const uint4*>(xr + n * 8 * PITCH);
+                    xb[n] = *reinterpret_cast<const uint4*>(xr + n * 8 * PITCH + 32);
+                }
+                xr += 64;
+                const unsigned words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-                    for (int j = part_of * GS; j < (GS < 4 ? (part_of + 1) * GS : 4); ++j) {
+                for (int q = 0; q < GPC; ++q) {
+                    const uint2 s = sc[i][q];
+                    const __nv_bfloat162 z0 = i4_zero(s.x), z1 = i4_zero(s.y);
+#pragma unroll
+                    for (int j = q * (GPC == 1 ? 4 : GS); j < (q + 1) * (GPC == 1 ? 4 : GS); ++j) {
                         const unsigned a[4] = {i4_pair(words[j], 0, z0), i4_pair(words[j], 4, z1), i4_pair(words[j], 8, z0), i4_pair(words[j], 12, z1)};
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             const unsigned b[8] = {xa[n].x, xa[n].y, xa[n].z, xa[n].w, xb[n].x, xb[n].y, xb[n].z, xb[n].w};
-                            mma_bf16_16816(sum[r][n], a, b[2 * j], b[2 * j + 1]);
+                            mma_bf16_16816(sum[n], a, b[2 * j], b[2 * j + 1]);
                         }
                     }
                     // a group is complete: its sum on its scale
                     if (GS <= 4 || (ch + 1) % CPG == 0 || ch + 1 == end) {
-                        const float s0 = i4_scale(sc.x), s1 = i4_scale(sc.y);
+                        const float f0 = i4_scale(s.x), f1 = i4_scale(s.y);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            total[r][n][0] = fmaf(sum[r][n][0], s0, total[r][n][0]);
-                            total[r][n][1] = fmaf(sum[r][n][1], s0, total[r][n][1]);
-                            total[r][n][2] = fmaf(sum[r][n][2], s1, total[r][n][2]);
-                            total[r][n][3] = fmaf(sum[r][n][3], s1, total[r][n][3]);
-                            sum[r][n][0] = sum[r][n][1] = sum[r][n][2] = sum[r][n][3] = 0.f;
+                            total[n][0] = fmaf(sum[n][0], f0, total[n][0]);
+                            total[n][1] = fmaf(sum[n][1], f0, total[n][1]);
+                            total[n][2] = fmaf(sum[n][2], f1, total[n][2]);
+                            total[n][3] = fmaf(sum[n][3], f1, total[n][3]);
+                            sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
                         }
                     }
                 }
+                bring(ch + AHEAD, w[i], sc[i]);
             }
-            bring(ch + I4_AHEAD, w[i]);
         }
     }
+    if (!waited) pdl_wait();
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            part[warp][r][g][8 * n + 2 * c] = total[r][n][0];
-            part[warp][r][g][8 * n + 2 * c + 1] = total[r][n][1];
-            part[warp][r][g + 8][8 * n + 2 * c] = total[r][n][2];
-            part[warp][r][g + 8][8 * n + 2 * c + 1] = total[r][n][3];
-        }
+    for (int n = 0; n < NT; ++n) {
+        float* lo = part[(tk * wn + tn) * 16 + g], *hi = part[(tk * wn + tn) * 16 + g + 8];
+        lo[8 * n + 2 * c] = total[n][0];
+        lo[8 * n + 2 * c + 1] = total[n][1];
+        hi[8 * n + 2 * c] = total[n][2];
+        hi[8 * n + 2 * c + 1] = total[n][3];
+    }
     __syncthreads();
-    constexpr int ALL = RT * 16 * 8 * NT;
+    const int features = wn * 16;                  // of the block, with up's behind the gate's (a power of two)
     if (splits > 1) {
         // the block's own sum first, then the cluster's
-        for (int i = threadIdx.x; i < ALL; i += I4_WARPS * 32) {
-            const int r = i / (16 * 8 * NT), f = i / (8 * NT) % 16, n = i % (8 * NT);
-            float s = 0.f;
-#pragma unroll
-            for (int v = 0; v < I4_WARPS; ++v) s += part[v][r][f][n];
-            part[0][r][f][n] = s;
+        if (wk > 1) {
+            for (int i = threadIdx.x; i < features * 8 * NT; i += I4_WARPS * 32) {
+                const int f = i & (features - 1), n = i >> (31 - __clz(features));
+                float s = 0.f;
+                for (int k = 0; k < wk; ++k) s += part[k * features + f][n];
+                part[f][n] = s;
+            }
         }
         cluster_sync();
     }
     // one result (a pair for a gated product) a thread, features side by side
-    const int wide = GLU ? p.n / 2 : p.n;
-    for (int i = threadIdx.x * splits + rank; i < (GLU ? ALL / 2 : ALL); i += I4_WARPS * 32 * splits) {
-        const int n = i / ((GLU ? 1 : RT) * 16), f = i % ((GLU ? 1 : RT) * 16), row = r0 + n;
-        const int feature = (GLU ? tile : tile * RT) * 16 + f;
+    const int wide = GLU ? p.n / 2 : p.n, mine_f = GLU ? features / 2 : features, rows_here = min(8 * NT, p.rows - r0), shift = 31 - __clz(mine_f);
+    for (int i = threadIdx.x * splits + rank; i < mine_f * rows_here; i += I4_WARPS * 32 * splits) {
+        const int n = i >> shift, f = i & (mine_f - 1), feature = block * mine_f + f;
         float v[GLU ? 2 : 1];
 #pragma unroll
         for (int h = 0; h < (GLU ? 2 : 1); ++h) {
-            const int r = GLU ? h : f / 16;
+            const int at = f + h * mine_f;
             float s = 0.f;
             if (splits > 1) {
-                for (int j = 0; j < splits; ++j) s += cluster_f32(cluster_peer(&part[0][r][f % 16][n], (unsigned)j));
-            } else {
+                float peer[8];                     // (all under way together)
 #pragma unroll
-                for (int q = 0; q < I4_WARPS; ++q) s += part[q][r][f % 16][n];
+                for (int j = 0; j < 8; ++j) peer[j] = j < splits ? cluster_f32(cluster_peer(&part[at][n], (unsigned)j)) : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s += peer[j];
+            } else {
+                for (int k = 0; k < wk; ++k) s += part[k * features + at][n];
             }
             v[h] = s;
         }
-        if (row >= p.rows || feature >= wide) continue;
+        if (feature >= wide) continue;
+        const size_t to = (size_t)(r0 + n) * wide + feature;
         if (GLU) {
-            p.y[(size_t)row * wide + feature] = __float2bfloat16_rn(glu_gate_16(v[0], p.act) * v[GLU ? 1 : 0]);
+            p.y[to] = __float2bfloat16_rn(glu_gate_16(v[0], p.act) * v[GLU ? 1 : 0]);
         } else {
             const float s = v[0] + (p.bias ? p.bias[feature] : 0.f);
-            if (p.y32) p.y32[(size_t)row * wide + feature] = s;
-            else p.y[(size_t)row * wide + feature] = __float2bfloat16_rn(s);
+            if (p.y32) p.y32[to] = s;
+            else p.y[to] = __float2bfloat16_rn(s);
         }
     }
     if (splits > 1) cluster_sync();                // nobody reads this block's memory any more
 }
 
-template <int NT, int RT, int GS, bool GLU>
-static int launch_int4_rows(const I4Params& p, int splits, cudaStream_t stream) {
-    const int tiles = (p.n + 15) / 16, blocks = GLU ? tiles / 2 : (tiles + RT - 1) / RT;
+// How the work falls to blocks: as many tile rows a block (1, 2, 4 or 8) as leave about two blocks a multiprocessor, and at least NT, so that x is
+// not read more often than the weights; then, while there are fewer blocks, a cluster of up to 8 shares the columns as long as each
+// warp still has four tiles.
+static void int4_shape(int tiles, int chunks, int nt, bool glu, int& wn, int& splits) {
+    wn = glu ? 2 : 1;
+    while (wn < 8 && (wn < nt || (tiles + wn - 1) / wn > 2 * sm_count())) wn *= 2;
+    const long long blocks = (tiles + wn - 1) / wn;
+    splits = 1;
+    while (splits < 8 && 2 * splits * blocks <= 2LL * sm_count() && chunks / (2 * splits * (I4_WARPS / wn)) >= 4) splits *= 2;
+}
+
+template <int NT, int GS, bool GLU>
+static int launch_int4_rows(const I4Params& p, cudaStream_t stream) {
+    const int tiles = (p.n + 15) / 16;
+    int wn, splits;
+    int4_shape(tiles, p.chunks, NT, GLU, wn, splits);
+    const int each = (p.chunks + splits - 1) / splits + 1, seg = (each < I4_SEG<NT> ? each + (each & 1) : I4_SEG<NT>);
+    constexpr size_t smem = ((I4_PART * (8 * NT + 1) * 4 + 15) & ~15) + (size_t)8 * NT * (I4_SEG<NT> * 64 + 32) * 2;
+    static int ready[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "int4_linear: cannot tell the current device");
+    if (!ready[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(int4_rows_kernel<NT, GS, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return fail(-101, "int4_linear: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+        ready[dev] = 1;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(blocks * splits), (unsigned)((p.rows + 8 * NT - 1) / (8 * NT)));
+    cfg.gridDim = dim3((unsigned)((tiles + wn - 1) / wn * splits), (unsigned)((p.rows + 8 * NT - 1) / (8 * NT)));
     cfg.blockDim = dim3(I4_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -199,31 +260,15 @@ static int launch_int4_rows(const I4Params& p, int splits, cudaStream_t stream) 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return check_launch("int4_linear", cudaLaunchKernelEx(&cfg, int4_rows_kernel<NT, RT, GS, GLU>, p, splits));
-}
-
-// Blocks of a cluster that share the columns: a power of two up to 8, while there are fewer than two blocks a multiprocessor
-// and each warp still has four tiles.
-static int int4_splits(long long blocks, int chunks) {
-    int s = 1;
-    while (s < 8 && 2 * s * blocks <= 2LL * sm_count() && chunks / (2 * s * I4_WARPS) >= 4) s *= 2;
-    return s;
+    return check_launch("int4_linear", cudaLaunchKernelEx(&cfg, int4_rows_kernel<NT, GS, GLU>, p, splits, wn, seg));
 }
 
 template <int GS>
 static int int4_rows(const I4Params& p, bool glu, cudaStream_t stream) {
-    const int tiles = (p.n + 15) / 16;
-    // one tile row a block while there are few of them, else two, which halves what is read of x
-    const bool two = !glu && tiles >= 4 * sm_count();
-    const long long blocks = glu || two ? tiles / 2 : tiles;
-    const int splits = int4_splits(blocks, p.chunks);
-#define VAPI_I4(NT)                                                                       \
-    return glu ? launch_int4_rows<NT, 2, GS, true>(p, splits, stream)                     \
-               : two ? launch_int4_rows<NT, 2, GS, false>(p, splits, stream) : launch_int4_rows<NT, 1, GS, false>(p, splits, stream)
-    if (p.rows <= 8) VAPI_I4(1);
-    if (p.rows <= 16) VAPI_I4(2);
-    VAPI_I4(4);
-#undef VAPI_I4
+    if (p.rows <= 8) return glu ? launch_int4_rows<1, GS, true>(p, stream) : launch_int4_rows<1, GS, false>(p, stream);
+    if (p.rows <= 16) return glu ? launch_int4_rows<2, GS, true>(p, stream) : launch_int4_rows<2, GS, false>(p, stream);
+    if (p.rows <= 24) return glu ? launch_int4_rows<3, GS, true>(p, stream) : launch_int4_rows<3, GS, false>(p, stream);
+    return glu ? launch_int4_rows<4, GS, true>(p, stream) : launch_int4_rows<4, GS, false>(p, stream);
 }
 
 // x [rows][k] bfloat16 with 16-byte aligned rows.  gated: W is [gate; up], y [rows][n / 2] = act(gate) * up, n / 2 a multiple of 16.
@@ -260,7 +305,7 @@ __global__ void int4_numbers_kernel(const unsigned* __restrict__ codes, const un
     const int tile = (int)(i / 32 / chunks), ch = (int)(i / 32 % chunks);
     const uint4 w = __ldg(reinterpret_cast<const uint4*>(codes) + i);
     const unsigned words[4] = {w.x, w.y, w.z, w.w};
-    const int groups = k / group;
+    const int groups = group == 32 ? 2 * chunks : k / group;
     pdl_wait();                                    // (the weight is nobody's output, but `out` may still be read)
 #pragma unroll
     for (int a = 0; a < 2; ++a) {

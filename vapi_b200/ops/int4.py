@@ -74,7 +74,8 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.T
         words[at:at + m] = got.view(m, chunks, 32, 4)
     bits = lambda t: t.to(torch.bfloat16).view(torch.int16).to(torch.int32) & 0xffff
     pairs = bits(scales) | bits(zeros.to(torch.float32) + 128.0) << 16
-    pairs = torch.nn.functional.pad(pairs, (0, 0, 0, tiles * 16 - n)).view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+    wide = 2 * chunks if group == 32 else groups                   # (whole tiles of 64 columns)
+    pairs = torch.nn.functional.pad(pairs, (0, wide - groups, 0, tiles * 16 - n)).view(tiles, 2, 8, wide).permute(0, 3, 2, 1).contiguous()
     return Int4Weight(words, pairs, n, k, group)
 
 
