@@ -391,12 +391,17 @@ PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         const int type = type_code(*x);
         int* status = static_cast<int*>(address(a[5]));
         void* stream = address(a[6]);
-        // (one buffer: one allocation a call)
-        const auto options = x->options().dtype(at::kFloat);
-        at::Tensor buf = at::empty({rows * (2 + 2LL * top)}, options);
-        at::Tensor parts[4] = {buf.narrow(0, 0, rows), buf.narrow(0, rows, rows), buf.narrow(0, 2 * rows, rows * top).view(at::kInt).view({rows, (int64_t)top}),
-                               buf.narrow(0, (2 + top) * rows, rows * top).view({rows, (int64_t)top})};
+        // (one allocation: the four are places of one storage)
+        at::Tensor buf = at::empty({rows * (2 + 2LL * top)}, x->options().dtype(at::kFloat));
         float* p = static_cast<float*>(buf.data_ptr());
+        auto place = [&](at::ScalarType of, int64_t offset, int64_t columns) {
+            at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), c10::scalarTypeToTypeMeta(of));
+            part.unsafeGetTensorImpl()->set_storage_offset(offset);
+            if (columns < 0) part.unsafeGetTensorImpl()->set_sizes_contiguous({rows});
+            else part.unsafeGetTensorImpl()->set_sizes_contiguous({rows, columns});
+            return part;
+        };
+        at::Tensor parts[4] = {place(at::kFloat, 0, -1), place(at::kFloat, rows, -1), place(at::kInt, 2 * rows, top), place(at::kFloat, (2 + top) * rows, top)};
         int rc;
         called = true;
         {

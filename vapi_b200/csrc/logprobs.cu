@@ -8,9 +8,9 @@
 // blocks of a cluster join theirs in a fixed order.
 //
 // The k most likely tokens need no second pass over the row.  A thread's maximum is m, which it has anyway, and where it stands
-// is looked up only when it moves.  The k-th largest of the maxima of the 128 groups of four threads is a bound with at least k
-// elements at or above it, and only threads whose maximum is at or above it can hold one: about k of 512, whose elements are read
-// again (a few hundredths of the row, out of L2).  What they find is ranked by comparison, by (logit descending, id ascending) in
+// is looked up only when it moves.  The k-th largest of the maxima of the 64 groups of four threads is a bound with at least k
+// elements at or above it, and only threads whose maximum is at or above it can hold one: about k of 256, whose elements are read
+// again (a tenth of the row at most, out of L2).  What they find is ranked by comparison, by (logit descending, id ascending) in
 // one 64-bit key, so that the result does not depend on the order in which it was found.  If more is found than the list holds
 // (rows made for it), the k largest are taken one after the other.
 //
@@ -21,8 +21,8 @@
 
 using namespace vapi;
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_GROUPS = LP_THREADS / 4;
-constexpr int LP_MAX_TOP = 64;                     // alternatives at most (below the number of groups)
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_GROUPS = LP_THREADS / 4;
+constexpr int LP_MAX_TOP = 64;                     // alternatives at most (as many as there are groups)
 constexpr int LP_LIST = 1024;
 constexpr int LP_MAX_CLUSTER = 16;
 // a distance in powers of two at which nothing is left of a term (2^-126 is the smallest that ex2 gives), kept finite so that zero times it is zero
@@ -62,6 +62,18 @@ __device__ __forceinline__ Share lp_join(const Share& a, const Share& b) {
     return r;
 }
 
+// the shares of a warp's lanes, joined: onto the largest m first, so that the sums are only added
+__device__ __forceinline__ Share lp_warp(const Share& a) {
+    Share r;
+    r.m = warp_max(a.m);
+    const float d = a.m == -INFINITY ? 0.f : fmaxf((a.m - r.m) * LOG2E, LP_FAR), f = lp_ex2(d);
+    r.s = warp_sum(a.s * f);
+    r.t = warp_sum(fmaf(a.s, d, a.t) * f);
+    return r;
+}
+
+template <bool V> struct Truth { static constexpr bool value = V; };
+
 template <typename T> struct LpVec;
 template <> struct LpVec<float> {
     static constexpr int N = 4;
@@ -81,7 +93,7 @@ template <> struct LpVec<__nv_bfloat16> {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 2)
+__global__ void __launch_bounds__(LP_THREADS, 4)
 logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const int* __restrict__ tokens, int top, float* __restrict__ logprob,
                 float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_lp, int slices, int* __restrict__ status) {
     constexpr int N = LpVec<T>::N, BATCH = 32 / N;
@@ -111,11 +123,12 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
     // ---- one pass: m, s, t of this thread's elements, and where m stands
     Share a = {-INFINITY, 0.f, 0.f};
     int at = has_head ? tid : (from + tid < upto ? head + (from + tid) * N : head + pieces * N + tid);
-    auto add = [&](float v) {
-        const float d = (v - (a.m == -INFINITY ? 0.f : a.m)) * LOG2E, e = lp_ex2(d);
+    auto add = [&](float v, float mu) {            // mu: m, or 0 where nothing but -inf has been seen
+        const float d = (v - mu) * LOG2E, e = lp_ex2(d);
         a.s += e;
         a.t = fmaf(e, fmaxf(d, LP_FAR), a.t);      // (an e of zero stays zero beside a logit of -inf)
     };
+    auto ground = [&]() { return a.m == -INFINITY ? 0.f : a.m; };
     auto raise = [&](float mx) {                   // a new largest logit: what was summed moves onto it
         const float d = a.m == -INFINITY ? 0.f : fmaxf((a.m - mx) * LOG2E, LP_FAR), f = lp_ex2(d);
         a.t = fmaf(a.s, d, a.t) * f;
@@ -125,13 +138,14 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
     if (has_head) {
         const float v = to_f32(x[tid]);
         if (v > a.m) a.m = v;
-        add(v);
+        add(v, ground());
     }
-    for (int i = from + tid; i < upto; i += BATCH * LP_THREADS) {
+    int i = from + tid;
+    auto batch = [&](auto whole) {                 // 32 elements; not whole: pieces behind the slice are -inf
         float v[BATCH][N];
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            if (i + b * LP_THREADS < upto) {
+            if (decltype(whole)::value || i + b * LP_THREADS < upto) {
                 LpVec<T>::load(body + (size_t)(i + b * LP_THREADS) * N, v[b]);
             } else {
 #pragma unroll
@@ -145,33 +159,32 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
             for (int e = 0; e < N; ++e) mx = fmaxf(mx, v[b][e]);
         if (mx > a.m) {
             raise(mx);
-            bool found = false;
+            int first = 0;
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b)
+            for (int b = BATCH - 1; b >= 0; --b)
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (!found && v[b][e] == mx) { found = true; at = head + (i + b * LP_THREADS) * N + e; }
+                for (int e = N - 1; e >= 0; --e) first = v[b][e] == mx ? b * LP_THREADS * N + e : first;
+            at = head + i * N + first;
         }
+        const float mu = ground();
 #pragma unroll
         for (int b = 0; b < BATCH; ++b)
 #pragma unroll
-            for (int e = 0; e < N; ++e) add(v[b][e]);
-    }
+            for (int e = 0; e < N; ++e) add(v[b][e], mu);
+        i += BATCH * LP_THREADS;
+    };
+    while (i + (BATCH - 1) * LP_THREADS < upto) batch(Truth<true>());
+    if (i < upto) batch(Truth<false>());
     if (has_tail) {
         const int id = head + pieces * N + tid;
         const float v = to_f32(x[id]);
         if (v > a.m) { raise(v); at = id; }
-        add(v);
+        add(v, ground());
     }
     const bool any = has_head || from + tid < upto || has_tail;
 
     // ---- the block's share
-    Share w = a;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Share other = {__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o), __shfl_xor_sync(0xffffffffu, w.t, o)};
-        w = (lane & o) ? lp_join(other, w) : lp_join(w, other);
-    }
+    const Share w = lp_warp(a);
     if (lane == 0) warp_share[warp] = w;
 
     // ---- the block's k largest
@@ -186,10 +199,9 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
         if (tid == 0) bound = 0ull;                // (fewer than k groups with an element: every element is looked at)
     }
     __syncthreads();
-    if (tid == 0) {
-        Share b = warp_share[0];
-        for (int j = 1; j < LP_WARPS; ++j) b = lp_join(b, warp_share[j]);
-        own_share = b;
+    if (warp == LP_WARPS - 1) {
+        const Share b = lp_warp(lane < LP_WARPS ? warp_share[lane] : Share{-INFINITY, 0.f, 0.f});
+        if (lane == 0) own_share = b;
     }
     if (top > 0) {
         if (tid < LP_GROUPS) {
@@ -270,7 +282,7 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
         cluster_sync();                            // nobody reads this block's memory any more
         if (slice != 0) return;
         const int all = slices * top;
-        if (tid < top) groups[tid] = 0ull;         // (the number of groups is above that of the alternatives)
+        if (tid < top) groups[tid] = 0ull;         // (there are as many groups as alternatives at most)
         __syncthreads();
         for (int j = tid; j < all; j += LP_THREADS) {
             const Key k = list[j];
@@ -304,7 +316,7 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
     }
 }
 
-// blocks that share a row: a power of two, while they are all on the device at once and have at least 2,048 elements each
+// blocks that share a row: a power of two, while there are at most two a multiprocessor and each has at least 2,048 elements
 static int lp_slices(int rows, int vocab) {
     int s = 1;
     while (s < LP_MAX_CLUSTER && 2LL * s * rows <= 2LL * sm_count() && vocab / (2 * s) >= 2048) s *= 2;

@@ -48,10 +48,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sta
         raise KernelError(f"{top} alternatives are outside 0..{min(LOGPROBS_MAX_TOP, vocab)}")
     _cuda(logits, tokens)
     _here(logits, tokens)
-    # (one buffer: a call costs one allocation, and a reader on the host one copy)
-    buf = torch.empty((rows * (2 + 2 * top),), dtype=torch.float32, device=logits.device)
-    out = TokenLogprobs(buf[:rows], buf[rows:2 * rows], buf[2 * rows:(2 + top) * rows].view(torch.int32).view(rows, top),
-                        buf[(2 + top) * rows:].view(rows, top))
+    empty = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=logits.device)
+    out = TokenLogprobs(empty(rows), empty(rows), empty((rows, top), torch.int32), empty((rows, top)))
     lib = _lib("logprobs")
     _check(lib, lib.vapi_token_logprobs(_p(logits), dt, rows, vocab, logits.stride(0), _p(tokens), top, out.logprob.data_ptr(),
                                         out.entropy.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), slices, _p(status),
