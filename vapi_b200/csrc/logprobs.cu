@@ -9,13 +9,15 @@
 //
 // The k most likely tokens need no second pass over the row.  A thread's maximum is m, which it has anyway, and where it stands
 // is looked up only when it moves.  The k-th largest of the maxima of the 64 groups of four threads is a bound with at least k
-// elements at or above it, and only threads whose maximum is at or above it can hold one: about k of 256, whose elements are read
-// again (a tenth of the row at most, out of L2).  What they find is ranked by comparison, by (logit descending, id ascending) in
+// elements at or above it, and only batches of 32 whose maximum (kept in shared memory) is at or above it can hold one: about
+// k of a row's 2,048, which are read again.  (Without the batches' maxima a thread's whole 256 elements are, 32-byte sectors for
+// 16-byte pieces: 2,047 rows of 65,536 with 20 alternatives 117 us, 82 without alternatives.)  What they find is ranked by comparison, by (logit descending, id ascending) in
 // one 64-bit key, so that the result does not depend on the order in which it was found.  If more is found than the list holds
 // (rows made for it), the k largest are taken one after the other.
 //
-// Few rows: up to 16 blocks share a row as a cluster and join through its shared memory; from two blocks a multiprocessor on a
-// block has its row for itself.
+// Few rows: up to 8 blocks share a row as a cluster and join through its shared memory (8 rows of 65,536: 10.4 us on one block
+// each, 7.5 on eight, 9.1 on sixteen); from one block a multiprocessor on a block has its row for itself (300 rows: 22 us, on two
+// 22, on four 29).
 #include "common.cuh"
 #include "cluster.cuh"
 
@@ -24,7 +26,8 @@ using namespace vapi;
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_GROUPS = LP_THREADS / 4;
 constexpr int LP_MAX_TOP = 64;                     // alternatives at most (as many as there are groups)
 constexpr int LP_LIST = 1024;
-constexpr int LP_MAX_CLUSTER = 16;
+constexpr int LP_SLOTS = 16;                       // batches whose maxima are kept apart (the 17th shares with the first, and so on)
+constexpr int LP_MAX_CLUSTER = 8;
 // a distance in powers of two at which nothing is left of a term (2^-126 is the smallest that ex2 gives), kept finite so that zero times it is zero
 constexpr float LP_FAR = -200.f;
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
@@ -104,7 +107,8 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
     __shared__ Key list[LP_LIST];
     __shared__ Key best[LP_MAX_TOP];               // this block's k largest, in order, read by the first block of its cluster
     __shared__ Key warp_best[LP_WARPS];
-    __shared__ int again[LP_THREADS];              // threads whose elements are looked at again
+    __shared__ float batch_max[LP_SLOTS][LP_THREADS];
+    __shared__ unsigned short again[LP_SLOTS * LP_THREADS];       // batches that are looked at again: thread | slot << 8
     __shared__ int n_again, n_list;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -140,7 +144,9 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
         if (v > a.m) a.m = v;
         add(v, ground());
     }
-    int i = from + tid;
+    int i = from + tid, slot = 0;
+    const int slots = top > 0 ? min(LP_SLOTS, (upto - from + BATCH * LP_THREADS - 1) / (BATCH * LP_THREADS)) : 0;
+    for (int k = 0; k < slots; ++k) batch_max[k][tid] = -INFINITY;
     auto batch = [&](auto whole) {                 // 32 elements; not whole: pieces behind the slice are -inf
         float v[BATCH][N];
 #pragma unroll
@@ -157,6 +163,10 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
         for (int b = 0; b < BATCH; ++b)
 #pragma unroll
             for (int e = 0; e < N; ++e) mx = fmaxf(mx, v[b][e]);
+        if (top > 0) {
+            batch_max[slot][tid] = fmaxf(batch_max[slot][tid], mx);
+            slot = slot + 1 < LP_SLOTS ? slot + 1 : 0;
+        }
         if (mx > a.m) {
             raise(mx);
             int first = 0;
@@ -213,27 +223,38 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
         }
         __syncthreads();
         const Key least = bound;
-        if (mine != 0ull && mine >= least) again[atomicAdd(&n_again, 1)] = tid;
+        // batches that can hold an element at or above the bound: a larger maximum, or an equal one whose first place is not behind it
+        const float least_x = lp_logit(least);
+        const int least_id = least == 0ull ? 0x7fffffff : lp_id(least);
+        for (int k = 0; k < slots; ++k) {
+            const int piece = from + tid + k * BATCH * LP_THREADS;
+            const float mx = batch_max[k][tid];
+            if (piece < upto && (least == 0ull || mx > least_x || (mx == least_x && head + piece * N <= least_id)))
+                again[atomicAdd(&n_again, 1)] = (unsigned short)(tid | k << 8);
+        }
+        auto offer = [&](Key k) {
+            if (k != 0ull && k >= least) {
+                const int place = atomicAdd(&n_list, 1);
+                if (place < LP_LIST) list[place] = k;
+            }
+        };
+        if (has_head) offer(lp_key(to_f32(x[tid]), tid));
+        if (has_tail) offer(lp_key(to_f32(x[head + pieces * N + tid]), head + pieces * N + tid));
         __syncthreads();
         const int n = n_again;
-        // every element of thread `t` by a warp: visit(key) for those at or above the bound
-        auto visit_all = [&](int t, auto&& visit) {
-            if (lane == 0 && slice == 0 && t < head) visit(lp_key(to_f32(x[t]), t));
-            for (int p = from + t + lane * LP_THREADS; p < upto; p += 32 * LP_THREADS) {
-                float v[N];
-                LpVec<T>::load(body + (size_t)p * N, v);
+        // the elements of those batches, a batch by 32 / N lanes (one piece each)
+        auto visit_all = [&](auto&& visit) {
+            for (int j = warp * N + lane / BATCH; j < n; j += LP_WARPS * N) {
+                const int t = again[j] & 0xff;
+                for (int p = from + t + ((again[j] >> 8) * BATCH + lane % BATCH) * LP_THREADS; p < upto; p += LP_SLOTS * BATCH * LP_THREADS) {
+                    float v[N];
+                    LpVec<T>::load(body + (size_t)p * N, v);
 #pragma unroll
-                for (int e = 0; e < N; ++e) visit(lp_key(v[e], head + p * N + e));
-            }
-            if (lane == 0 && slice == slices - 1 && t < tail) visit(lp_key(to_f32(x[head + pieces * N + t]), head + pieces * N + t));
-        };
-        for (int j = warp; j < n; j += LP_WARPS)
-            visit_all(again[j], [&](Key k) {
-                if (k != 0ull && k >= least) {
-                    const int place = atomicAdd(&n_list, 1);
-                    if (place < LP_LIST) list[place] = k;
+                    for (int e = 0; e < N; ++e) visit(lp_key(v[e], head + p * N + e));
                 }
-            });
+            }
+        };
+        visit_all(offer);
         if (tid < top) best[tid] = 0ull;
         __syncthreads();
         const int found = n_list;
@@ -248,7 +269,10 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
             Key last = ~0ull;
             for (int r = 0; r < top && last != 0ull; ++r) {                 // (the same for all threads)
                 Key b = 0ull;
-                for (int j = warp; j < n; j += LP_WARPS) visit_all(again[j], [&](Key k) { if (k < last && k > b) b = k; });
+                auto look = [&](Key k) { if (k < last && k > b) b = k; };
+                visit_all(look);
+                if (has_head) look(lp_key(to_f32(x[tid]), tid));
+                if (has_tail) look(lp_key(to_f32(x[head + pieces * N + tid]), head + pieces * N + tid));
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
                     const Key other = __shfl_xor_sync(0xffffffffu, b, o);
@@ -316,24 +340,16 @@ logprobs_kernel(const T* __restrict__ logits, int vocab, long long stride, const
     }
 }
 
-// blocks that share a row: a power of two, while there are at most two a multiprocessor and each has at least 2,048 elements
+// blocks that share a row: a power of two, while there is at most one a multiprocessor and each has at least 2,048 elements
 static int lp_slices(int rows, int vocab) {
     int s = 1;
-    while (s < LP_MAX_CLUSTER && 2LL * s * rows <= 2LL * sm_count() && vocab / (2 * s) >= 2048) s *= 2;
+    while (s < LP_MAX_CLUSTER && 2LL * s * rows <= sm_count() && vocab / (2 * s) >= 2048) s *= 2;
     return s;
 }
 
 template <typename T>
 static int launch_logprobs(const void* logits, int rows, int vocab, long long stride, const int* tokens, int top, float* logprob, float* entropy,
                            int* top_ids, float* top_lp, int slices, int* status, cudaStream_t stream) {
-    static int ready[64] = {0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "token_logprobs: cannot tell the current device");
-    if (!ready[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return fail(-101, "token_logprobs: %s", cudaGetErrorString(e));
-        ready[dev] = 1;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long long)rows * slices));
     cfg.blockDim = dim3(LP_THREADS);

@@ -28,7 +28,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sta
 
     A token outside the vocabulary gets NaN and a status.  Logits of -inf are tokens of probability zero, like any other in the
     ranking.  A row with a NaN or +inf, or of nothing but -inf, has NaN for its numbers (which tokens it then ranks is not said; -1 stands
-    where there are none).  ``slices``: into how many blocks a row is cut (a power of two up to 16; 0: as many as pay); in another
+    where there are none).  ``slices``: into how many blocks a row is cut (a power of two up to 8; 0: as many as pay); in another
     cut the sums are added in another order."""
     if logits.is_cuda:
         lib = _lib("logprobs")
