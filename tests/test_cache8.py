@@ -313,6 +313,18 @@ def test_portions_on_tcgen05(lens, news, nh, nkv, d, page, window):
 
 
 @gpu
+@pytest.mark.parametrize("d,window", [(64, 0), (64, 100), (128, 0)])
+def test_long_portions_beside_single_tokens(d, window):
+    """Portions long enough for the tcgen05 kernel in one step with shorter ones and single tokens, which go to the mma.sync kernel."""
+    c = _attention_case([1700, 60, 900, 33, 1], [1650, 1, 31, 32, 1], 16, 4, d, 64, torch.bfloat16, d)
+    ops = _ops()
+    before = ops.launch_count
+    got = _run_attention(c, d ** -0.5, window)
+    assert ops.launch_count == before + 2
+    _portion_check(c, got, d ** -0.5, window)
+
+
+@gpu
 @pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
 @pytest.mark.parametrize("rows", [1, 3])
 def test_attention_split_over_a_cluster(splits, rows):

@@ -1,13 +1,15 @@
 // Attention of prompt portions over an 8-bit cache on the fifth-generation tensor cores (tcgen05): bfloat16 queries, head size 64
 // or 128, sequences that bring at least `min_q` tokens to the step (shorter ones are decode8_kernel's).
 //
-// A block owns 128 rows (query token, q head of the group) of one (sequence, kv head) and walks the key tiles, 64 keys each, that any
-// of them can see:
-//   warp 0 (one lane)  issues S = Q K^T into one of two tensor-memory buffers and O += P V into a third; owns the allocation;
+// A block owns twice 128 rows (query token, q head of the group) of one (sequence, kv head) and walks the key tiles, 64 keys each, that
+// any of them can see:
+//   warp 0 (one lane)  issues S = Q K^T of either half into one of its two tensor-memory buffers and O += P V into a third; owns the
+//                      allocation;
 //   warps 1..3         bring the codes of a tile into registers while the tile before is worked on, and write it to a ring of
-//                      shared-memory stages as 16-bit numbers;
-//   warps 4..7         softmax, one row a thread, as the 16-bit kernel does it (attention_tc.cuh): the running maximum only moves
-//                      when a tile exceeds it by more than 2^8, so O is rescaled a few times a row.
+//                      shared-memory stages as 16-bit numbers, once for both halves: with 128 rows a block, and two blocks a
+//                      multiprocessor, this was a third of all instructions (2,048 tokens behind 5,952, 32 / 8 heads of 64: 338 us);
+//   warps 4..7, 8..11  softmax of a half, one row a thread, as the 16-bit kernel does it (attention_tc.cuh): the running maximum only
+//                      moves when a tile exceeds it by more than 2^8, so O is rescaled a few times a row.
 //
 //   K: a code is an f16 number; Q's rows are f16 too, each scaled by a power of two so that its largest element is near 2^14 (as in
 //      cache8_decode.cuh).  The scale of a block of 16 keys multiplies 16 columns of S, where a score is multiplied by something
@@ -23,12 +25,12 @@
 
 namespace vapi {
 
-constexpr int P8_ROWS = 128, P8_KEYS = 64, P8_THREADS = 256, P8_LOADERS = 96;
+constexpr int P8_HALF = 128, P8_HALVES = 2, P8_ROWS = P8_HALF * P8_HALVES, P8_KEYS = 64, P8_LOADERS = 96, P8_THREADS = 128 + P8_ROWS;
 constexpr int P8_MIN_Q = 32;                       // in a step of several sequences, those with fewer tokens go to decode8_kernel
-template <int HD> constexpr int P8_STAGES = HD == 64 ? 3 : 2;
+template <int HD> constexpr int P8_STAGES = HD == 64 ? 4 : 2;
 template <int HD> constexpr int P8_TILE = P8_KEYS * HD * 2;                                  // bytes of K (or V) of a tile
 template <int HD> constexpr size_t P8_SMEM = 1024 + P8_ROWS * HD * 2 + 2 * P8_ROWS * P8_KEYS * 2 + (size_t)P8_STAGES<HD> * 2 * P8_TILE<HD> + 512;
-constexpr int P8_TMEM_COLS = 256;                  // S0 | S1 | O, 64 + 64 + HD columns
+constexpr int P8_TMEM_COLS = 512;                  // a half's S0 | S1, the other's, then O of either, HD columns
 
 // 16 codes as 16 halves
 __device__ __forceinline__ void p8_halves(const uint4& c, uint4& lo, uint4& hi) {
@@ -54,16 +56,16 @@ __device__ __forceinline__ void p8_numbers(const uint4& c, float f, uint4& lo, u
 }
 
 template <int HD>
-__global__ void __launch_bounds__(P8_THREADS, HD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(P8_THREADS, 1)
 prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int num_seqs, const int min_q) {
     constexpr int STAGES = P8_STAGES<HD>, TILE = P8_TILE<HD>, ATOMS = HD / 64, ATOM = P8_KEYS * 128;     // 64 elements of 64 keys
     extern __shared__ unsigned char p8_smem[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p8_smem) + 1023) & ~(uintptr_t)1023);
-    unsigned char* sQ = base;                                   // [atom][128 rows][128 B], 128-byte swizzle
-    unsigned char* sP = base + P8_ROWS * HD * 2;                // two buffers [128 rows][128 B]
+    unsigned char* sQ = base;                                   // [half][atom][128 rows][128 B], 128-byte swizzle
+    unsigned char* sP = base + P8_ROWS * HD * 2;                // [half][two buffers][128 rows][128 B]
     unsigned char* sKV = sP + 2 * P8_ROWS * P8_KEYS * 2;        // [stage][K | V][atom][64 keys][128 B]
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(sKV + (size_t)STAGES * 2 * TILE);
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 16);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 32);
     int* flags = reinterpret_cast<int*>(tmem_slot + 1);
     float* sE = reinterpret_cast<float*>(tmem_slot + 4);        // [stage][4]: the scales of the tile's blocks of keys
 
@@ -86,18 +88,19 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     const int nt = p_max < key_lo ? 0 : p_max / P8_KEYS - kt_lo + 1;
 
     const unsigned kv_full = smem_u32(bars), kv_empty = smem_u32(bars + STAGES);
-    const unsigned s_full = smem_u32(bars + 2 * STAGES), s_free = smem_u32(bars + 2 * STAGES + 2);
-    const unsigned p_ready = smem_u32(bars + 2 * STAGES + 4), pv_done = smem_u32(bars + 2 * STAGES + 6);
-    const unsigned q_ready = smem_u32(bars + 2 * STAGES + 8);
+    // of half h and buffer b: 16 h + 8 b bytes further on
+    const unsigned s_full = smem_u32(bars + 2 * STAGES), s_free = smem_u32(bars + 2 * STAGES + 4);
+    const unsigned p_ready = smem_u32(bars + 2 * STAGES + 8), pv_done = smem_u32(bars + 2 * STAGES + 12);
+    const unsigned q_ready = smem_u32(bars + 2 * STAGES + 16);
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(kv_full + 8 * i, P8_LOADERS); mbar_init(kv_empty + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 * P8_HALVES; ++i) {
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(s_free + 8 * i, 128);
-            mbar_init(p_ready + 8 * i, 128);
+            mbar_init(s_free + 8 * i, P8_HALF);
+            mbar_init(p_ready + 8 * i, P8_HALF);
             mbar_init(pv_done + 8 * i, 1);
         }
-        mbar_init(q_ready, 128);
+        mbar_init(q_ready, P8_ROWS);
         flags[0] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -108,46 +111,62 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
-    const unsigned tmem_base = *tmem_slot, tS0 = tmem_base, tO = tmem_base + 128;
+    const unsigned tmem_base = *tmem_slot;       // half h: S at 128 h (and 64 further on), O at 256 + HD h
 
     if (warp == 0) {
         if (lane == 0) {
             // instruction descriptors: float accumulate, N = 64, M = 128; f16 x f16, both K-major, and bf16 x bf16 with V's
             // contiguous dimension N
-            const unsigned shape = (1u << 4) | ((unsigned)(P8_KEYS >> 3) << 17) | ((unsigned)(P8_ROWS >> 4) << 24);
+            const unsigned shape = (1u << 4) | ((unsigned)(P8_KEYS >> 3) << 17) | ((unsigned)(P8_HALF >> 4) << 24);
             const unsigned idesc_s = shape, idesc_o = shape | (1u << 7) | (1u << 10) | (1u << 16);
             bool ok = true;
-            auto pv = [&](int j) {          // O += P(j) . V(j)
-                if (!ok) return;
-                if (!mbar_wait(p_ready + 8 * (j & 1), (j >> 1) & 1)) { ok = false; return; }
-                tc5_fence_after();
-                const int stage = j % STAGES;
-                const unsigned pa = smem_u32(sP + (j & 1) * P8_ROWS * P8_KEYS * 2);
-                const unsigned vb = smem_u32(sKV + (size_t)stage * 2 * TILE) + TILE;
+            // One thread issues everything, at a few cycles an instruction: descriptors are made once (tcgen05.cuh: umma_desc,
+            // umma_desc_mn), and a step's is a sum.  (Worked out for every step they cost 130 cycles a product, which takes 48: what bounded
+            // the kernel.)
+            const unsigned high = (1024u >> 4) | 1u << 14 | 2u << 29;
+            const unsigned q_low = ((smem_u32(sQ) >> 4) & 0x3FFF) | 1u << 16, p_low = ((smem_u32(sP) >> 4) & 0x3FFF) | 1u << 16;
+            const unsigned k_low = ((smem_u32(sKV) >> 4) & 0x3FFF) | 1u << 16, v_low = (((smem_u32(sKV) + TILE) >> 4) & 0x3FFF) | (1024u >> 4) << 16;
+            auto desc = [&](unsigned low) { return (unsigned long long)high << 32 | low; };
+            auto pv = [&](int j, unsigned vb) {                  // O += P(j) . V(j), either half
 #pragma unroll
-                for (int a = 0; a < ATOMS; ++a)
+                for (int h = 0; h < P8_HALVES; ++h) {
+                    if (!ok || !mbar_wait(p_ready + 16 * h + 8 * (j & 1), (j >> 1) & 1)) { ok = false; break; }
+                    tc5_fence_after();
+                    const unsigned pa = p_low + (2 * h + (j & 1)) * (P8_HALF * P8_KEYS * 2 >> 4), tO = tmem_base + 256 + h * HD;
 #pragma unroll
-                    for (int k = 0; k < P8_KEYS / 16; ++k)
-                        umma_f16(tO + a * 64, umma_desc(pa + k * 32), umma_desc_mn(vb + a * ATOM + k * 16 * 128), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-                umma_commit(pv_done + 8 * (j & 1));
-                umma_commit(kv_empty + 8 * stage);
+                    for (int a = 0; a < ATOMS; ++a)
+#pragma unroll
+                        for (int k = 0; k < P8_KEYS / 16; ++k)
+                            umma_f16(tO + a * 64, desc(pa + k * (32 >> 4)), desc(vb + (a * ATOM + k * 16 * 128 >> 4)), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(pv_done + 16 * h + 8 * (j & 1));
+                }
             };
+            int stage = 0, parity = 0, before = 0;
             for (int i = 0; i < nt && ok; ++i) {
-                const int stage = i % STAGES, sb = i & 1;
-                if (!mbar_wait(kv_full + 8 * stage, (i / STAGES) & 1)) { ok = false; break; }
-                if (i >= 2 && !mbar_wait(s_free + 8 * sb, ((i >> 1) - 1) & 1)) { ok = false; break; }
+                const int sb = i & 1;
+                if (!mbar_wait(kv_full + 8 * stage, parity)) { ok = false; break; }
                 if (i == 0 && !mbar_wait(q_ready, 0)) { ok = false; break; }
-                tc5_fence_after();
-                const unsigned qa = smem_u32(sQ), kb = smem_u32(sKV + (size_t)stage * 2 * TILE);
+                const unsigned kb = k_low + stage * (2 * TILE >> 4);
 #pragma unroll
-                for (int a = 0; a < ATOMS; ++a)
+                for (int h = 0; h < P8_HALVES; ++h) {
+                    if (!ok || (i >= 2 && !mbar_wait(s_free + 16 * h + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
+                    tc5_fence_after();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_f16(tS0 + sb * 64, umma_desc(qa + a * P8_ROWS * 128 + k * 32), umma_desc(kb + a * ATOM + k * 32), idesc_s, (a > 0 || k > 0) ? 1u : 0u);
-                umma_commit(s_full + 8 * sb);
-                if (i >= 1) pv(i - 1);
+                    for (int a = 0; a < ATOMS; ++a)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_f16(tmem_base + h * 128 + sb * 64, desc(q_low + (h * P8_HALF * HD * 2 + a * P8_HALF * 128 + k * 32 >> 4)), desc(kb + (a * ATOM + k * 32 >> 4)),
+                                     idesc_s, (a > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(s_full + 16 * h + 8 * sb);
+                }
+                if (i >= 1 && ok) {
+                    pv(i - 1, v_low + before * (2 * TILE >> 4));
+                    if (ok) umma_commit(kv_empty + 8 * before);
+                }
+                before = stage;
+                if (++stage == STAGES) { stage = 0; parity ^= 1; }
             }
-            if (nt > 0) pv(nt - 1);
+            if (nt > 0 && ok) pv(nt - 1, v_low + before * (2 * TILE >> 4));
             if (!ok) flags[0] = 1;
         }
     } else if (warp < 4) {
@@ -156,57 +175,65 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         constexpr int PER = 2 * P8_KEYS * HD / 16, EACH = (PER + P8_LOADERS - 1) / P8_LOADERS;       // 16-byte pieces of a tile, a thread
         const int* bt = p.block_table + (size_t)s * p.table_stride;
         const int per_head = p.page_size / C8_BLOCK;
+        const int fresh = base_pos < 0 ? 0 : base_pos / C8_BLOCK * C8_BLOCK;      // from here on the kernel before this one wrote
         bool waited = false;
-        // lane b < 4: where block b of a tile lies, and its scales
-        auto find = [&](int i) {
-            int at = 0;
-            if (lane < 4 && i < nt) {
-                const int key = (kt_lo + i) * P8_KEYS + lane * C8_BLOCK;
-                if (key <= p_max) {                             // (blocks behind the last key that is seen: the first block's place, and masked)
-                    int page = bt[key / p.page_size];
-                    if (page < 0 || page >= p.num_pages) {
-                        if (p.status) atomicExch(p.status, 4);
-                        page = 0;
-                    }
-                    at = (page * 2 * p.nkv + g) * per_head + key % p.page_size / C8_BLOCK;
-                }
-            }
-            return at;
+        // Where the 32 blocks of eight tiles lie, one a lane, and their scales.  Looked up in two steps, both well before they are
+        // wanted: a tile's codes are asked for two tiles ahead, and waiting for the table first would double the way.
+        auto key_of = [&](int from) { return (kt_lo + from) * P8_KEYS + lane * C8_BLOCK; };
+        auto pages = [&](int from) {                             // of tiles from .. from + 7
+            const int key = key_of(from);
+            return from + (lane >> 2) < nt && key <= p_max ? bt[key / p.page_size] : -1;
         };
-        uint4 codes[EACH];
-        int exps = 0;
-        auto load = [&](int i, int where) {                      // tile i, whose blocks lie at `where`
-            // a tile that reaches into this step's keys was written by the kernel before this one (and the block they begin in)
-            if (!waited && (kt_lo + i) * P8_KEYS + P8_KEYS > (base_pos < 0 ? 0 : base_pos / C8_BLOCK * C8_BLOCK)) { pdl_wait(); waited = true; }
-            if (lane < 4) exps = c8_scales(p, where, per_head);
+        auto places = [&](int from, int page) {
+            const int key = key_of(from);
+            if (!(from + (lane >> 2) < nt && key <= p_max)) return 0;             // (no row sees it: any block, and masked)
+            if (page < 0 || page >= p.num_pages) {
+                if (p.status) atomicExch(p.status, 4);
+                page = 0;
+            }
+            return (page * 2 * p.nkv + g) * per_head + key % p.page_size / C8_BLOCK;
+        };
+        auto scales_of = [&](int from, int where) {
+            if (!waited && (kt_lo + from + 8) * P8_KEYS > fresh) { pdl_wait(); waited = true; }
+            return c8_scales(p, where, per_head);
+        };
+        const size_t to_values = (size_t)p.nkv * per_head * C8_BLOCK * HD;
+        int where = 0, scales = 0, next_page = -1, next_where = 0, next_scales = 0;
+        struct Tile { uint4 codes[EACH]; int scales; } even, odd;
+        auto load = [&](int i, Tile& to) {                       // tile i (one after the other)
+            const int at = i & 7;
+            if (i > 0 && at == 0) { where = next_where; scales = next_scales; }
+            if (at == 3) next_page = pages(i + 5);
+            if (at == 5) {
+                next_where = places(i + 3, next_page);
+                next_scales = scales_of(i + 3, next_where);
+            }
+            to.scales = __shfl_sync(0xffffffffu, scales, at * 4 + (lane & 3));
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
                 const int piece = t + j * P8_LOADERS;
                 const int kind = piece / (PER / 2), r = piece % (PER / 2) / (HD / 16), c = piece % (HD / 16);
-                const int block = __shfl_sync(0xffffffffu, where, r / C8_BLOCK);
+                const int block = __shfl_sync(0xffffffffu, where, at * 4 + (r / C8_BLOCK & 3));
                 if (piece < PER)
-                    codes[j] = __ldcg(reinterpret_cast<const uint4*>(p.codes + ((size_t)block + (kind ? (size_t)p.nkv * per_head : 0)) * C8_BLOCK * HD +
-                                                                    (r & (C8_BLOCK - 1)) * HD) + c);
+                    to.codes[j] = __ldcg(reinterpret_cast<const uint4*>(p.codes + (size_t)block * (C8_BLOCK * HD) + (kind ? to_values : 0) + (r & (C8_BLOCK - 1)) * HD) + c);
             }
         };
-        int next = find(0), later = find(1);
-        if (nt > 0) load(0, next);
-        for (int i = 0; i < nt; ++i) {
+        auto write = [&](int i, const Tile& from) {
             const int stage = i % STAGES, k0 = (kt_lo + i) * P8_KEYS;
-            if (!__all_sync(0xffffffffu, i < STAGES || mbar_wait(kv_empty + 8 * stage, ((i / STAGES) - 1) & 1))) { flags[0] = 1; break; }
+            if (!__all_sync(0xffffffffu, i < STAGES || mbar_wait(kv_empty + 8 * stage, ((i / STAGES) - 1) & 1))) { flags[0] = 1; return false; }
             unsigned char* dst = sKV + (size_t)stage * 2 * TILE;
-            if (t < 4) sE[stage * 4 + t] = c8_power((int)(signed char)(exps & 0xff));
+            if (t < 4) sE[stage * 4 + t] = c8_power((int)(signed char)(from.scales & 0xff));
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
                 const int piece = t + j * P8_LOADERS;
                 const int kind = piece / (PER / 2), r = piece % (PER / 2) / (HD / 16), c = piece % (HD / 16);
-                const int e = (int)(signed char)(__shfl_sync(0xffffffffu, exps, r / C8_BLOCK) >> 8 & 0xff);
+                const int e = (int)(signed char)(__shfl_sync(0xffffffffu, from.scales, r / C8_BLOCK & 3) >> 8 & 0xff);
                 if (piece >= PER) continue;
                 uint4 lo, hi;
                 if (kind == 0) {
-                    p8_halves(codes[j], lo, hi);
+                    p8_halves(from.codes[j], lo, hi);
                 } else if (k0 + r <= p_max) {                   // (what no row sees may be anything)
-                    p8_numbers(codes[j], c8_power(e), lo, hi);
+                    p8_numbers(from.codes[j], c8_power(e), lo, hi);
                 } else {
                     lo = hi = make_uint4(0u, 0u, 0u, 0u);
                 }
@@ -217,19 +244,33 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             }
             fence_proxy_async();
             mbar_arrive(kv_full + 8 * stage);
-            if (i + 1 < nt) {
-                next = later;
-                later = find(i + 2);
-                load(i + 1, next);
-            }
+            return true;
+        };
+        if (nt > 0) {
+            where = places(0, pages(0));
+            scales = scales_of(0, where);
+            load(0, even);
+        }
+        if (nt > 1) load(1, odd);
+        for (int i = 0; i < nt; i += 2) {
+            if (!write(i, even)) break;
+            if (i + 2 < nt) load(i + 2, even);
+            if (i + 1 >= nt || !write(i + 1, odd)) break;
+            if (i + 3 < nt) load(i + 3, odd);
         }
         if (!waited) pdl_wait();
     } else {
         // ---- softmax and epilogue: one row per thread ----
-        const int quarter = warp & 3;                               // the tensor-memory lanes this warp may touch
+        const int half = (warp - 4) >> 2, quarter = warp & 3;       // (a quarter: the tensor-memory lanes this warp may touch)
         const int row = quarter * 32 + lane;
         const unsigned lane_addr = (unsigned)(quarter * 32) << 16;
-        const int rr = tile_start + row;
+        const unsigned tS0 = tmem_base + half * 128, tO = tmem_base + 256 + half * HD;
+        const unsigned my_full = s_full + 16 * half, my_free = s_free + 16 * half, my_ready = p_ready + 16 * half, my_done = pv_done + 16 * half;
+        unsigned char* const myP = sP + half * 2 * P8_HALF * P8_KEYS * 2;
+        const int start = tile_start + half * P8_HALF;
+        const int rr = start + row;
+        // the least and the largest position of the half's rows (a half without rows: nothing is stored of it)
+        const int my_min = base_pos + start / n_rep, my_max = base_pos + min(last_row, start + P8_HALF - 1) / n_rep;
         const bool row_ok = rr < rows_total;
         const int tok = row_ok ? rr / n_rep : 0;
         const int head = g * n_rep + (row_ok ? rr - tok * n_rep : 0);
@@ -256,7 +297,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                 unsigned h[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[i] = d8_half2(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
-                *reinterpret_cast<uint4*>(sQ + (c >> 3) * P8_ROWS * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(sQ + half * P8_HALF * HD * 2 + (c >> 3) * P8_HALF * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
             }
             fence_proxy_async();
             mbar_arrive(q_ready);
@@ -267,7 +308,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             const int sb = i & 1, stage = i % STAGES;
             const int k0 = (kt_lo + i) * P8_KEYS;
             // (a wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide instructions)
-            if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, (i >> 1) & 1))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, mbar_wait(my_full + 8 * sb, (i >> 1) & 1))) { ok = false; break; }
             if (!__all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (i / STAGES) & 1))) { ok = false; break; }     // complete already: makes the scales visible here
             tc5_fence_after();
             float sv[P8_KEYS];
@@ -282,12 +323,12 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                     for (int e = 0; e < 16; ++e) sv[j * 16 + e] = __uint_as_float(raw[j][e]);
             }
             tc5_fence_before();
-            mbar_arrive(s_free + 8 * sb);                           // the scores are in registers
+            mbar_arrive(my_free + 8 * sb);                           // the scores are in registers
             const float4 ek = *reinterpret_cast<const float4*>(sE + stage * 4);
             // (kept above zero: a masked score is -inf before it is multiplied)
             const float f[4] = {fmaxf(ek.x * row_f, 1.2e-38f), fmaxf(ek.y * row_f, 1.2e-38f), fmaxf(ek.z * row_f, 1.2e-38f), fmaxf(ek.w * row_f, 1.2e-38f)};
 
-            const bool need_mask = (k0 + P8_KEYS - 1 > p_min) || (p.window > 0 && k0 <= p_max - p.window);
+            const bool need_mask = (k0 + P8_KEYS - 1 > my_min) || (p.window > 0 && k0 <= my_max - p.window);
             if (need_mask) {
 #pragma unroll
                 for (int e = 0; e < P8_KEYS; ++e) {
@@ -309,7 +350,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;         // m_run = -inf: 0
             if (i >= 1 && __any_sync(0xffffffffu, grow)) {
                 // the accumulator must be at rest: P.V of the tile before this one has completed
-                if (!__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, mbar_wait(my_done + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1))) { ok = false; break; }
                 tc5_fence_after();
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j) {
@@ -325,7 +366,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             m_run = m_new;
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             // this tile's P buffer was last read by P.V of the tile two before
-            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(my_done + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
             const float2 mu2 = make_float2(-m_use, -m_use);
             float rs4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -339,14 +380,14 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                     rs4[e] += x.x + x.y;
                     w[e] = pack_bf16(x.x, x.y);
                 }
-                *reinterpret_cast<uint4*>(sP + sb * P8_ROWS * P8_KEYS * 2 + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(myP + sb * P8_HALF * P8_KEYS * 2 + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             l_run += (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
             fence_proxy_async();
             tc5_fence_before();
-            mbar_arrive(p_ready + 8 * sb);
+            mbar_arrive(my_ready + 8 * sb);
         }
-        if (ok && nt > 0 && !__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * ((nt - 1) & 1), ((nt - 1) >> 1) & 1))) ok = false;
+        if (ok && nt > 0 && !__all_sync(0xffffffffu, mbar_wait(my_done + 8 * ((nt - 1) & 1), ((nt - 1) >> 1) & 1))) ok = false;
         tc5_fence_after();
         if (ok) {                                                   // (uniform over the warp)
             const float inv = l_run == 0.f ? 0.f : 1.f / l_run;     // a row that sees nothing: zeros

@@ -115,8 +115,8 @@ def attention8_splits(num_seqs: int, max_q: int, max_k: int, nh: int, nkv: int, 
 
 
 _IMPL8 = {"auto": 0, "general": 1, "tensor_core": 2, "tcgen05": 3}
-#: steps whose longest portion has at least this many tokens go to the tcgen05 kernel (the library's own rule, restated)
-PORTION8_MIN_Q = 32
+#: portions shorter than this never go to the tcgen05 kernel beside other sequences (csrc/cache8_prompt.cuh)
+_PORTION8_MIN_Q = 32
 
 
 def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_table: torch.Tensor, cu_q: torch.Tensor,
@@ -126,18 +126,20 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     """:func:`paged_attention` over a cache in 8 bits; returns [n, nh*d].  Arguments as there; the numbers of the cache are taken
     exactly, scores, softmax and sums are float32.  A query without a visible key gets zeros.
 
-    ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions of 32 tokens or more, and the
+    ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions long enough to fill the device, and the
     mma.sync kernel, whose ``splits`` (up to 16) blocks share the keys as a cluster, for the others; the general kernel for every other
     type, head size (a multiple of 16 up to 256) and alignment.  "tcgen05", "tensor_core" and "general" force one (the first two raise where
     they do not apply)."""
     code = _IMPL8.get(impl)
-    two = max_q >= PORTION8_MIN_Q and num_seqs > 1 and code == 0 and q.dtype == torch.bfloat16 and d in (64, 128)
+    kernels = 1 if n > 0 else 0
+    if max_q >= _PORTION8_MIN_Q and num_seqs > 1 and code == 0 and q.dtype == torch.bfloat16 and d in (64, 128) and nkv > 0 and q.is_cuda:
+        kernels *= int(_lib("cache8").vapi_attention8_kernels(num_seqs, max_q, nh, nkv))
     if q.is_cuda and code is not None:
         lib = _lib("cache8")
         got = _native("attention8", lib, "vapi_paged_attention8", q, q_row_stride, cache[0], cache[1], block_table, cu_q, seqlens_k, n, num_seqs,
                       max_q, max_k, nh, nkv, d, scale, window, splits or 0, code, _p(status))
         if got is not NotImplemented:
-            _check(lib, got if type(got) is int else 0, (2 if two else 1) if n > 0 else 0)
+            _check(lib, got if type(got) is int else 0, kernels)
             return got
     for t, w in ((block_table, "block table"), (cu_q, "cu_q"), (seqlens_k, "seqlens_k")):
         _i32(t, w)
@@ -160,5 +162,5 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     lib = _lib("cache8")
     _check(lib, lib.vapi_paged_attention8(_p(q), q_row_stride, _p(cache.codes), _p(cache.exps), _dt(q), _p(block_table), block_table.stride(0),
                                           _p(cu_q), _p(seqlens_k), _p(out), n, num_seqs, max_q, max_k, nh, nkv, d, page_size, pages,
-                                          scale, window, splits or 0, code, _p(status), _stream()), launches=(2 if two else 1) if n > 0 else 0)
+                                          scale, window, splits or 0, code, _p(status), _stream()), launches=kernels)
     return out
