@@ -55,6 +55,15 @@ __device__ __forceinline__ void p8_numbers(const uint4& c, float f, uint4& lo, u
     hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
+// one lane of a whole warp, the same every time
+__device__ __forceinline__ bool p8_elect() {
+    unsigned yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
+}
+// a wait by a whole warp, with one outcome
+__device__ __forceinline__ bool mbar_wait_warp(unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
 template <int HD>
 __global__ void __launch_bounds__(P8_THREADS, 1)
 prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int num_seqs, const int min_q) {
@@ -69,7 +78,8 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     int* flags = reinterpret_cast<int*>(tmem_slot + 1);
     float* sE = reinterpret_cast<float*>(tmem_slot + 4);        // [stage][4]: the scales of the tile's blocks of keys
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (by a shuffle: what depends on the warp alone is then known to be the same for all its lanes)
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int g = (int)blockIdx.x % p.nkv, n_rep = p.nh / p.nkv;
     pdl_trigger();
     // index data was copied from the host before the step's first kernel: safe before the wait
@@ -111,18 +121,21 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
-    const unsigned tmem_base = *tmem_slot;       // half h: S at 128 h (and 64 further on), O at 256 + HD h
+    const unsigned tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);          // half h: S at 128 h (and 64 further on), O at 256 + HD h
 
     if (warp == 0) {
-        if (lane == 0) {
+        {
+            // (the whole warp goes through the loop and waits; one lane issues)
+            const bool leader = p8_elect();
             // instruction descriptors: float accumulate, N = 64, M = 128; f16 x f16, both K-major, and bf16 x bf16 with V's
             // contiguous dimension N
             const unsigned shape = (1u << 4) | ((unsigned)(P8_KEYS >> 3) << 17) | ((unsigned)(P8_HALF >> 4) << 24);
             const unsigned idesc_s = shape, idesc_o = shape | (1u << 7) | (1u << 10) | (1u << 16);
             bool ok = true;
-            // One thread issues everything, at a few cycles an instruction: descriptors are made once (tcgen05.cuh: umma_desc,
-            // umma_desc_mn), and a step's is a sum.  (Worked out for every step they cost 130 cycles a product, which takes 48: what bounded
-            // the kernel.)
+            // Descriptors are made once (tcgen05.cuh: umma_desc, umma_desc_mn), and a step's is a sum, of numbers that are the same for the
+            // whole warp: a product's operands are in uniform registers.  (With one lane alone in the loop each of them was moved there
+            // for every product: four products and a commit took 310 cycles to issue and 192 to run, and the waits between them were not
+            // hidden: what bounded the kernel.)
             const unsigned high = (1024u >> 4) | 1u << 14 | 2u << 29;
             const unsigned q_low = ((smem_u32(sQ) >> 4) & 0x3FFF) | 1u << 16, p_low = ((smem_u32(sP) >> 4) & 0x3FFF) | 1u << 16;
             const unsigned k_low = ((smem_u32(sKV) >> 4) & 0x3FFF) | 1u << 16, v_low = (((smem_u32(sKV) + TILE) >> 4) & 0x3FFF) | (1024u >> 4) << 16;
@@ -130,27 +143,31 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             auto pv = [&](int j, unsigned vb) {                  // O += P(j) . V(j), either half
 #pragma unroll
                 for (int h = 0; h < P8_HALVES; ++h) {
-                    if (!ok || !mbar_wait(p_ready + 16 * h + 8 * (j & 1), (j >> 1) & 1)) { ok = false; break; }
+                    if (!ok || !mbar_wait_warp(p_ready + 16 * h + 8 * (j & 1), (j >> 1) & 1)) { ok = false; break; }
                     tc5_fence_after();
                     const unsigned pa = p_low + (2 * h + (j & 1)) * (P8_HALF * P8_KEYS * 2 >> 4), tO = tmem_base + 256 + h * HD;
+                    if (leader) {
 #pragma unroll
                     for (int a = 0; a < ATOMS; ++a)
 #pragma unroll
                         for (int k = 0; k < P8_KEYS / 16; ++k)
                             umma_f16(tO + a * 64, desc(pa + k * (32 >> 4)), desc(vb + (a * ATOM + k * 16 * 128 >> 4)), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
                     umma_commit(pv_done + 16 * h + 8 * (j & 1));
+                    }
+                    __syncwarp();
                 }
             };
             int stage = 0, parity = 0, before = 0;
             for (int i = 0; i < nt && ok; ++i) {
                 const int sb = i & 1;
-                if (!mbar_wait(kv_full + 8 * stage, parity)) { ok = false; break; }
-                if (i == 0 && !mbar_wait(q_ready, 0)) { ok = false; break; }
+                if (!mbar_wait_warp(kv_full + 8 * stage, parity)) { ok = false; break; }
+                if (i == 0 && !mbar_wait_warp(q_ready, 0)) { ok = false; break; }
                 const unsigned kb = k_low + stage * (2 * TILE >> 4);
 #pragma unroll
                 for (int h = 0; h < P8_HALVES; ++h) {
-                    if (!ok || (i >= 2 && !mbar_wait(s_free + 16 * h + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
+                    if (!ok || (i >= 2 && !mbar_wait_warp(s_free + 16 * h + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
                     tc5_fence_after();
+                    if (leader) {
 #pragma unroll
                     for (int a = 0; a < ATOMS; ++a)
 #pragma unroll
@@ -158,10 +175,12 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                             umma_f16(tmem_base + h * 128 + sb * 64, desc(q_low + (h * P8_HALF * HD * 2 + a * P8_HALF * 128 + k * 32 >> 4)), desc(kb + (a * ATOM + k * 32 >> 4)),
                                      idesc_s, (a > 0 || k > 0) ? 1u : 0u);
                     umma_commit(s_full + 16 * h + 8 * sb);
+                    }
+                    __syncwarp();
                 }
                 if (i >= 1 && ok) {
                     pv(i - 1, v_low + before * (2 * TILE >> 4));
-                    if (ok) umma_commit(kv_empty + 8 * before);
+                    if (ok && leader) umma_commit(kv_empty + 8 * before);
                 }
                 before = stage;
                 if (++stage == STAGES) { stage = 0; parity ^= 1; }
