@@ -58,18 +58,18 @@ __device__ __forceinline__ unsigned c8_codes4(float x, float y, float z, float w
 __device__ __forceinline__ void c8_halves4(unsigned c, unsigned& lo, unsigned& hi) {
     asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(c));
 }
-__device__ __forceinline__ float c8_half_lo(unsigned h) {
-    float f;
-    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %1;\ncvt.f32.f16 %0, a;\n}" : "=f"(f) : "r"(h));
+__device__ __forceinline__ float2 c8_pair(unsigned h) {          // two halves as floats
+    float2 f;
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.f32.f16 %0, a;\ncvt.f32.f16 %1, b;\n}" : "=f"(f.x), "=f"(f.y) : "r"(h));
     return f;
 }
-__device__ __forceinline__ float c8_half_hi(unsigned h) { return c8_half_lo(h >> 16); }
 
 // Four codes as floats.
 __device__ __forceinline__ float4 c8_floats(unsigned c) {
     unsigned lo, hi;
     c8_halves4(c, lo, hi);
-    return make_float4(c8_half_lo(lo), c8_half_hi(lo), c8_half_lo(hi), c8_half_hi(hi));
+    const float2 x = c8_pair(lo), y = c8_pair(hi);
+    return make_float4(x.x, x.y, y.x, y.y);
 }
 
 // Four codes times f, rounded again.

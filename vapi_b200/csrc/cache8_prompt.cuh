@@ -3,13 +3,16 @@
 //
 // A block owns twice 128 rows (query token, q head of the group) of one (sequence, kv head) and walks the key tiles, 64 keys each, that
 // any of them can see:
-//   warp 0 (one lane)  issues S = Q K^T of either half into one of its two tensor-memory buffers and O += P V into a third; owns the
+//   warp 12            issues S = Q K^T of either half into one of its two tensor-memory buffers and O += P V into a third; owns the
 //                      allocation;
-//   warps 1..3         bring the codes of a tile into registers while the tile before is worked on, and write it to a ring of
-//                      shared-memory stages as 16-bit numbers, once for both halves: with 128 rows a block, and two blocks a
-//                      multiprocessor, this was a third of all instructions (2,048 tokens behind 5,952, 32 / 8 heads of 64: 338 us);
-//   warps 4..7, 8..11  softmax of a half, one row a thread, as the 16-bit kernel does it (attention_tc.cuh): the running maximum only
-//                      moves when a tile exceeds it by more than 2^8, so O is rescaled a few times a row.
+//   warps 0..3         bring the codes of a tile into registers while the tile before is worked on, and write it to a ring of
+//                      shared-memory stages as 16-bit numbers, once for both halves (with 128 rows a block, and two blocks a
+//                      multiprocessor, this was a third of all instructions), a warp on each of the four schedulers, which have two
+//                      of the softmax warps each: with three, those beside them were what the others waited for;
+//   warps 4..7, 8..11  softmax of a half, one row a thread, as the 16-bit kernel does it (attention_tc.cuh), but that the running
+//                      maximum only moves when a tile exceeds it by more than 2^24: P is bfloat16, whose rounding is the same at
+//                      any magnitude, and float sums hold 2^24 times as much.  A rescaling of O waits for P V and costs 1,500
+//                      cycles of a tile's 2,000; at 2^8 one tile in seven had one.
 //
 //   K: a code is an f16 number; Q's rows are f16 too, each scaled by a power of two so that its largest element is near 2^14 (as in
 //      cache8_decode.cuh).  The scale of a block of 16 keys multiplies 16 columns of S, where a score is multiplied by something
@@ -25,11 +28,12 @@
 
 namespace vapi {
 
-constexpr int P8_HALF = 128, P8_HALVES = 2, P8_ROWS = P8_HALF * P8_HALVES, P8_KEYS = 64, P8_LOADERS = 96, P8_THREADS = 128 + P8_ROWS;
+constexpr int P8_HALF = 128, P8_HALVES = 2, P8_ROWS = P8_HALF * P8_HALVES, P8_KEYS = 64, P8_LOADERS = 128, P8_THREADS = P8_LOADERS + P8_ROWS + 32;
 constexpr int P8_MIN_Q = 32;                       // in a step of several sequences, those with fewer tokens go to decode8_kernel
-template <int HD> constexpr int P8_STAGES = HD == 64 ? 4 : 2;
+template <int HD> constexpr int P8_STAGES = HD == 64 ? 4 : 3;                                // (S two tiles ahead of P V: three at least)
 template <int HD> constexpr int P8_TILE = P8_KEYS * HD * 2;                                  // bytes of K (or V) of a tile
 template <int HD> constexpr size_t P8_SMEM = 1024 + P8_ROWS * HD * 2 + 2 * P8_ROWS * P8_KEYS * 2 + (size_t)P8_STAGES<HD> * 2 * P8_TILE<HD> + 512;
+constexpr float P8_RAISE = 24.f;                   // log2 units by which a tile must exceed the running maximum to raise it
 constexpr int P8_TMEM_COLS = 512;                  // a half's S0 | S1, the other's, then O of either, HD columns
 
 // 16 codes as 16 halves
@@ -47,9 +51,11 @@ __device__ __forceinline__ void p8_numbers(const uint4& c, float f, uint4& lo, u
     unsigned h[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float4 v = c8_floats(w[i]);
-        h[2 * i] = pack_bf16(v.x * f, v.y * f);
-        h[2 * i + 1] = pack_bf16(v.z * f, v.w * f);
+        unsigned a, b;
+        c8_halves4(w[i], a, b);
+        const float2 x = __fmul2_rn(c8_pair(a), make_float2(f, f)), y = __fmul2_rn(c8_pair(b), make_float2(f, f));
+        h[2 * i] = pack_bf16(x.x, x.y);
+        h[2 * i + 1] = pack_bf16(y.x, y.y);
     }
     lo = make_uint4(h[0], h[1], h[2], h[3]);
     hi = make_uint4(h[4], h[5], h[6], h[7]);
@@ -99,14 +105,13 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
 
     const unsigned kv_full = smem_u32(bars), kv_empty = smem_u32(bars + STAGES);
     // of half h and buffer b: 16 h + 8 b bytes further on
-    const unsigned s_full = smem_u32(bars + 2 * STAGES), s_free = smem_u32(bars + 2 * STAGES + 4);
-    const unsigned p_ready = smem_u32(bars + 2 * STAGES + 8), pv_done = smem_u32(bars + 2 * STAGES + 12);
-    const unsigned q_ready = smem_u32(bars + 2 * STAGES + 16);
+    const unsigned s_full = smem_u32(bars + 2 * STAGES);
+    const unsigned p_ready = smem_u32(bars + 2 * STAGES + 4), pv_done = smem_u32(bars + 2 * STAGES + 8);
+    const unsigned q_ready = smem_u32(bars + 2 * STAGES + 12);
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(kv_full + 8 * i, P8_LOADERS); mbar_init(kv_empty + 8 * i, 1); }
         for (int i = 0; i < 2 * P8_HALVES; ++i) {
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(s_free + 8 * i, P8_HALF);
             mbar_init(p_ready + 8 * i, P8_HALF);
             mbar_init(pv_done + 8 * i, 1);
         }
@@ -114,7 +119,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         flags[0] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) {
+    if (warp == P8_THREADS / 32 - 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((unsigned)P8_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -123,7 +128,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     tc5_fence_after();
     const unsigned tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);          // half h: S at 128 h (and 64 further on), O at 256 + HD h
 
-    if (warp == 0) {
+    if (warp == P8_THREADS / 32 - 1) {
         {
             // (the whole warp goes through the loop and waits; one lane issues)
             const bool leader = p8_elect();
@@ -140,57 +145,65 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             const unsigned q_low = ((smem_u32(sQ) >> 4) & 0x3FFF) | 1u << 16, p_low = ((smem_u32(sP) >> 4) & 0x3FFF) | 1u << 16;
             const unsigned k_low = ((smem_u32(sKV) >> 4) & 0x3FFF) | 1u << 16, v_low = (((smem_u32(sKV) + TILE) >> 4) & 0x3FFF) | (1024u >> 4) << 16;
             auto desc = [&](unsigned low) { return (unsigned long long)high << 32 | low; };
-            auto pv = [&](int j, unsigned vb) {                  // O += P(j) . V(j), either half
-#pragma unroll
-                for (int h = 0; h < P8_HALVES; ++h) {
-                    if (!ok || !mbar_wait_warp(p_ready + 16 * h + 8 * (j & 1), (j >> 1) & 1)) { ok = false; break; }
-                    tc5_fence_after();
-                    const unsigned pa = p_low + (2 * h + (j & 1)) * (P8_HALF * P8_KEYS * 2 >> 4), tO = tmem_base + 256 + h * HD;
-                    if (leader) {
-#pragma unroll
-                    for (int a = 0; a < ATOMS; ++a)
-#pragma unroll
-                        for (int k = 0; k < P8_KEYS / 16; ++k)
-                            umma_f16(tO + a * 64, desc(pa + k * (32 >> 4)), desc(vb + (a * ATOM + k * 16 * 128 >> 4)), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(pv_done + 16 * h + 8 * (j & 1));
-                    }
-                    __syncwarp();
-                }
-            };
-            int stage = 0, parity = 0, before = 0;
-            for (int i = 0; i < nt && ok; ++i) {
-                const int sb = i & 1;
-                if (!mbar_wait_warp(kv_full + 8 * stage, parity)) { ok = false; break; }
-                if (i == 0 && !mbar_wait_warp(q_ready, 0)) { ok = false; break; }
-                const unsigned kb = k_low + stage * (2 * TILE >> 4);
-#pragma unroll
-                for (int h = 0; h < P8_HALVES; ++h) {
-                    if (!ok || (i >= 2 && !mbar_wait_warp(s_free + 16 * h + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
-                    tc5_fence_after();
-                    if (leader) {
+            auto score = [&](int h, int i, unsigned kb) {        // S(i) of half h
+                if (leader) {
 #pragma unroll
                     for (int a = 0; a < ATOMS; ++a)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            umma_f16(tmem_base + h * 128 + sb * 64, desc(q_low + (h * P8_HALF * HD * 2 + a * P8_HALF * 128 + k * 32 >> 4)), desc(kb + (a * ATOM + k * 32 >> 4)),
-                                     idesc_s, (a > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(s_full + 16 * h + 8 * sb);
+                            umma_f16(tmem_base + h * 128 + (i & 1) * 64, desc(q_low + (h * P8_HALF * HD * 2 + a * P8_HALF * 128 + k * 32 >> 4)),
+                                     desc(kb + (a * ATOM + k * 32 >> 4)), idesc_s, (a > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(s_full + 16 * h + 8 * (i & 1));
+                }
+                __syncwarp();
+            };
+            // S runs two tiles ahead of P V, so that a half's softmax finds its next scores there: when P(i) of a half is ready, its
+            // S(i) has been read too, and O += P(i) V and S(i + 2) follow one another without another wait.
+            int ahead = 0, parity = 0;                           // the stage of the next S
+            auto next_tile = [&](unsigned& kb) {
+                if (!mbar_wait_warp(kv_full + 8 * ahead, parity)) return false;
+                tc5_fence_after();
+                kb = k_low + ahead * (2 * TILE >> 4);
+                if (++ahead == STAGES) { ahead = 0; parity ^= 1; }
+                return true;
+            };
+            unsigned kb = 0;
+            if (nt > 0 && !mbar_wait_warp(q_ready, 0)) ok = false;
+            for (int i = 0; i < min(nt, 2) && ok; ++i) {
+                if (!next_tile(kb)) { ok = false; break; }
+                score(0, i, kb);
+                score(1, i, kb);
+            }
+            int stage = 0;
+            for (int i = 0; i < nt && ok; ++i) {
+                const unsigned vb = v_low + stage * (2 * TILE >> 4);
+#pragma unroll
+                for (int h = 0; h < P8_HALVES; ++h) {
+                    if (!ok || !mbar_wait_warp(p_ready + 16 * h + 8 * (i & 1), (i >> 1) & 1)) { ok = false; break; }
+                    tc5_fence_after();
+                    const unsigned pa = p_low + (2 * h + (i & 1)) * (P8_HALF * P8_KEYS * 2 >> 4), tO = tmem_base + 256 + h * HD;
+                    if (leader) {
+#pragma unroll
+                        for (int a = 0; a < ATOMS; ++a)
+#pragma unroll
+                            for (int k = 0; k < P8_KEYS / 16; ++k)
+                                umma_f16(tO + a * 64, desc(pa + k * (32 >> 4)), desc(vb + (a * ATOM + k * 16 * 128 >> 4)), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(pv_done + 16 * h + 8 * (i & 1));
                     }
                     __syncwarp();
+                    if (i + 2 < nt) {
+                        if (h == 0 && !next_tile(kb)) { ok = false; break; }
+                        score(h, i + 2, kb);
+                    }
                 }
-                if (i >= 1 && ok) {
-                    pv(i - 1, v_low + before * (2 * TILE >> 4));
-                    if (ok && leader) umma_commit(kv_empty + 8 * before);
-                }
-                before = stage;
-                if (++stage == STAGES) { stage = 0; parity ^= 1; }
+                if (ok && leader) umma_commit(kv_empty + 8 * stage);
+                if (++stage == STAGES) stage = 0;
             }
-            if (nt > 0 && ok) pv(nt - 1, v_low + before * (2 * TILE >> 4));
             if (!ok) flags[0] = 1;
         }
     } else if (warp < 4) {
         // ---- codes to numbers ----
-        const int t = threadIdx.x - 32;
+        const int t = threadIdx.x;
         constexpr int PER = 2 * P8_KEYS * HD / 16, EACH = (PER + P8_LOADERS - 1) / P8_LOADERS;       // 16-byte pieces of a tile, a thread
         const int* bt = p.block_table + (size_t)s * p.table_stride;
         const int per_head = p.page_size / C8_BLOCK;
@@ -284,7 +297,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         const int row = quarter * 32 + lane;
         const unsigned lane_addr = (unsigned)(quarter * 32) << 16;
         const unsigned tS0 = tmem_base + half * 128, tO = tmem_base + 256 + half * HD;
-        const unsigned my_full = s_full + 16 * half, my_free = s_free + 16 * half, my_ready = p_ready + 16 * half, my_done = pv_done + 16 * half;
+        const unsigned my_full = s_full + 16 * half, my_ready = p_ready + 16 * half, my_done = pv_done + 16 * half;
         unsigned char* const myP = sP + half * 2 * P8_HALF * P8_KEYS * 2;
         const int start = tile_start + half * P8_HALF;
         const int rr = start + row;
@@ -328,22 +341,22 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             const int k0 = (kt_lo + i) * P8_KEYS;
             // (a wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide instructions)
             if (!__all_sync(0xffffffffu, mbar_wait(my_full + 8 * sb, (i >> 1) & 1))) { ok = false; break; }
-            if (!__all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (i / STAGES) & 1))) { ok = false; break; }     // complete already: makes the scales visible here
             tc5_fence_after();
             float sv[P8_KEYS];
+            float4 ek;
             {
                 unsigned raw[P8_KEYS / 16][16];                     // all four loads in flight, one wait
 #pragma unroll
                 for (int j = 0; j < P8_KEYS / 16; ++j) tmem_ld16_nowait(tS0 + sb * 64 + lane_addr + j * 16, raw[j]);
+                // (complete already: makes the scales visible here)
+                if (!__all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (i / STAGES) & 1))) { ok = false; tmem_ld_wait(); break; }
+                ek = *reinterpret_cast<const float4*>(sE + stage * 4);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < P8_KEYS / 16; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sv[j * 16 + e] = __uint_as_float(raw[j][e]);
             }
-            tc5_fence_before();
-            mbar_arrive(my_free + 8 * sb);                           // the scores are in registers
-            const float4 ek = *reinterpret_cast<const float4*>(sE + stage * 4);
             // (kept above zero: a masked score is -inf before it is multiplied)
             const float f[4] = {fmaxf(ek.x * row_f, 1.2e-38f), fmaxf(ek.y * row_f, 1.2e-38f), fmaxf(ek.z * row_f, 1.2e-38f), fmaxf(ek.w * row_f, 1.2e-38f)};
 
@@ -364,7 +377,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                 for (int e = 1; e < 16; ++e) m4 = fmaxf(m4, sv[16 * b + e]);
                 mx = fmaxf(mx, m4 * f[b]);                          // (the scales are positive)
             }
-            const bool grow = mx > m_run + FT_RAISE;                // also the first tile with a visible key
+            const bool grow = mx > m_run + P8_RAISE;                // also the first tile with a visible key
             const float m_new = grow ? mx : m_run;
             const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;         // m_run = -inf: 0
             if (i >= 1 && __any_sync(0xffffffffu, grow)) {
@@ -384,8 +397,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             l_run *= alpha;
             m_run = m_new;
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
-            // this tile's P buffer was last read by P.V of the tile two before
-            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(my_done + 8 * sb, ((i >> 1) - 1) & 1))) { ok = false; break; }
+            // (this tile's P buffer was last read by P.V of the tile two before, which the half's S of this one was issued behind: it has ended)
             const float2 mu2 = make_float2(-m_use, -m_use);
             float rs4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -434,7 +446,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     tc5_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && flags[0] && p.status) atomicExch(p.status, 16);
-    if (warp == 0) {
+    if (warp == P8_THREADS / 32 - 1) {
         tc5_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((unsigned)P8_TMEM_COLS) : "memory");
     }
