@@ -28,10 +28,7 @@
 
 namespace vapi {
 
-#ifndef D8_WARPS_N
-#define D8_WARPS_N 8
-#endif
-constexpr int D8_WARPS = D8_WARPS_N;
+constexpr int D8_WARPS = 8;
 constexpr int D8_MAX_CLUSTER = 16;
 constexpr int D8_STAGES = 3;                                                           // of two chunks of K and of V
 constexpr float D8_RAISE = 8.f;                                                        // log2 units by which a score must pass a maximum to raise it
@@ -479,8 +476,8 @@ static int launch_decode8_of(const C8Params& p, const void* q, void* out, int nu
     return check_launch("paged_attention8", cudaLaunchKernelEx(&cfg, decode8_kernel<HD, WIDE>, p, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, splits, most_q));
 }
 
-template <int HD>
 // sequences that bring more than `most_q` tokens are left alone
+template <int HD>
 static int launch_decode8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int splits, int most_q, cudaStream_t stream) {
     if (splits < 1) splits = 1;
     if (splits > D8_MAX_CLUSTER) return fail(-1, "paged_attention8: %d splits are more than %d", splits, D8_MAX_CLUSTER);
