@@ -325,6 +325,23 @@ def test_long_portions_beside_single_tokens(d, window):
 
 
 @gpu
+@pytest.mark.parametrize("splits", [1, 2, 3, 4, 8, 16])
+@pytest.mark.parametrize("nh,nkv,d,window", [(8, 2, 64, 0), (6, 2, 128, 0), (3, 1, 64, 150), (8, 1, 128, 70)])
+def test_portions_split_over_a_cluster(splits, nh, nkv, d, window):
+    """Blocks of a cluster with several tiles of keys, with one and with none (30 keys are one tile), rows behind a sequence's last, and
+    tokens before a sequence's first key, which see nothing."""
+    c = _attention_case([1500, 30, 130], [45, 30, 130], nh, nkv, d, 64, torch.bfloat16, 3 * splits + d)
+    first = _run_attention(c, d ** -0.5, window, splits=splits, impl="tcgen05")
+    _portion_check(c, first, d ** -0.5, window)
+    assert torch.equal(first, _run_attention(c, d ** -0.5, window, splits=splits, impl="tcgen05"))
+    c["kl"] = torch.tensor([1500, 12, 0], dtype=torch.int32)
+    blind = _run_attention(c, d ** -0.5, window, splits=splits, impl="tcgen05")
+    assert torch.equal(blind[:45], first[:45])
+    assert not blind[45:45 + 18].any() and not blind[75:].any()
+    assert torch.isfinite(blind).all() and blind[63:75].any()
+
+
+@gpu
 @pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
 @pytest.mark.parametrize("rows", [1, 3])
 def test_attention_split_over_a_cluster(splits, rows):

@@ -514,19 +514,31 @@ static int c8_splits(int num_seqs, int max_q, int max_k, int nh, int nkv, int d)
     return splits;
 }
 
+// Whether a step's portions are for the tcgen05 kernel: whether by these estimates it takes less time.  The mma.sync kernel's are rounds of
+// blocks of 16 rows, of 5 us and 7.5 (head size 128: 6.5) a thousand keys.  Its tiles are smaller and its keys can be shared out further, so it is
+// ahead where rows or keys are few: 32 / 8 heads of 64, us on mma.sync and on tcgen05: 32 tokens of 4,000 15 / 19, 64 22 / 22, 128 35 / 28, 256
+// 68 / 30, 2,048 of 8,000 782 / 238; 64 of 32,000 127 / 83; 128 of 1,000 13 / 16; 512 of 512 29 / 14.
+template <int HD>
+static bool c8_portions_of(const C8Params& p, int n, int num_seqs, int max_q, int max_k) {
+    float tcgen05;
+    p8_step<HD>(p, n, max_k, tcgen05);
+    const long long seen = p.window > 0 && p.window + 16 < max_k ? p.window + 16 : max_k;
+    const float blocks = (float)(((long long)n * (p.nh / p.nkv) + 15) / 16 * p.nkv), slots = (float)decode8_slots<HD>();
+    const int splits = c8_splits(num_seqs, max_q, max_k, p.nh, p.nkv, HD);
+    const float rounds = blocks * splits / slots;
+    return tcgen05 < (rounds > 1.f ? rounds : 1.f) * (5.f + (HD == 64 ? 0.0075f : 0.0065f) * (float)seen / (float)splits);
+}
+static bool c8_portions(const C8Params& p, int n, int num_seqs, int max_q, int max_k) {
+    if (max_q < P8_MIN_Q) return false;
+    return p.d == 64 ? c8_portions_of<64>(p, n, num_seqs, max_q, max_k) : c8_portions_of<128>(p, n, num_seqs, max_q, max_k);
+}
+
 // q: [n, *] with `q_row_stride` elements between tokens, head h at h * d; out: [n, nh * d].
 // impl: 0 = the fastest kernel that applies: for bfloat16 and head size 64 or 128 the tcgen05 kernel for steps with a long enough portion
 // (c8_portions; in a step of several sequences for those of at least P8_MIN_Q tokens, beside the mma.sync kernel for the others), else the mma.sync
 // kernel; the general kernel for everything else.  1 = the general kernel; 2 = the mma.sync kernel, or an error;
-// 3 = the tcgen05 kernel for every sequence, or an error.  splits 0: as many as pay (max_k: the most keys a sequence has).
-
-// Whether a step's longest portion is for the tcgen05 kernel: whether its tiles of 128 rows are at least 3 blocks to 5 multiprocessors.
-// Fewer leave the device idle, and the mma.sync kernel, whose tiles are 16 rows and whose keys can be shared out, is ahead: 32 / 8 heads of 64
-// behind 4,000 keys, us on mma.sync and on tcgen05: 32 tokens 15 / 80, 64 22 / 80, 256 68 / 92; 2,048 behind 5,952 782 / 338.
-static bool c8_portions(int max_q, int nh, int nkv) {
-    const long long tiles = ((long long)max_q * (nh / nkv) + P8_ROWS - 1) / P8_ROWS;
-    return 5 * tiles * nkv >= 3LL * sm_count();
-}
+// 3 = the tcgen05 kernel for every sequence, or an error.  splits 0: as many as pay (max_k: the most keys
+// a sequence has); else those of the mma.sync kernel, up to 16, and at most 8, a power of two, of the tcgen05 kernel.
 VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, const void* codes, const void* exps, int dtype, const int* block_table,
                                       int table_stride, const int* cu_q, const int* seqlens_k, void* out, int n, int num_seqs, int max_q,
                                       int max_k, int nh, int nkv, int d, int page_size, int num_pages, float scale, int window, int splits,
@@ -549,9 +561,9 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
         if ((long long)num_pages * 2 * nkv * (page_size / C8_BLOCK) > 0x7fffffffLL)
             return fail(-1, "paged_attention8: %d pages of %d tokens and %d kv heads are more blocks than an index holds", num_pages, page_size, nkv);
         int rc = 0, most_q = 0x7fffffff;
-        if (impl == 3 || (impl == 0 && scale > 0.f && c8_portions(max_q, nh, nkv))) {
+        if (impl == 3 || (impl == 0 && scale > 0.f && c8_portions(p, n, num_seqs, max_q, max_k))) {
             const int min_q = impl == 3 || num_seqs == 1 ? 1 : P8_MIN_Q;
-            rc = d == 64 ? launch_prompt8<64>(p, q, out, n, num_seqs, max_q, min_q, stream) : launch_prompt8<128>(p, q, out, n, num_seqs, max_q, min_q, stream);
+            rc = d == 64 ? launch_prompt8<64>(p, q, out, n, num_seqs, max_q, max_k, min_q, splits, stream) : launch_prompt8<128>(p, q, out, n, num_seqs, max_q, max_k, min_q, splits, stream);
             if (rc != 0 || min_q == 1) return rc;
             most_q = min_q - 1;
         }
@@ -572,5 +584,10 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
 
 VAPI_EXPORT int vapi_attention8_splits(int num_seqs, int max_q, int max_k, int nh, int nkv, int d) { return c8_splits(num_seqs, max_q, max_k, nh, nkv, d); }
 // how many kernels a step of several sequences takes: 2 where its portions go to the tcgen05 kernel and the rest to the mma.sync one
-VAPI_EXPORT int vapi_attention8_kernels(int num_seqs, int max_q, int nh, int nkv) { return num_seqs > 1 && c8_portions(max_q, nh, nkv) ? 2 : 1; }
+VAPI_EXPORT int vapi_attention8_kernels(int n, int num_seqs, int max_q, int max_k, int nh, int nkv, int d, int window) {
+    if (num_seqs <= 1 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || (d != 64 && d != 128)) return 1;
+    C8Params p = {};
+    p.nh = nh; p.nkv = nkv; p.d = d; p.window = window;
+    return c8_portions(p, n, num_seqs, max_q, max_k) ? 2 : 1;
+}
 VAPI_EXPORT const char* vapi_last_error() { return error_buffer(); }

@@ -404,7 +404,9 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     }
     if (splits > 1) {
         cluster_sync();                                                     // every block's result is in place
-        for (int i = threadIdx.x * splits + rank; i < ROWS * HD / 4; i += D8_WARPS * 32 * splits) {
+        // (each block pieces that follow one another: neighbours' reads of another block's memory are then one)
+        const int mine = (ROWS * HD / 4 + splits - 1) / splits;
+        for (int i = rank * mine + threadIdx.x; i < min((rank + 1) * mine, ROWS * HD / 4); i += D8_WARPS * 32) {
             const int r = i / (HD / 4), c = i % (HD / 4) * 4;
             float mx = -INFINITY, rx = -INFINITY, sum = 0.f;
             for (int j = 0; j < splits; ++j) {

@@ -2,7 +2,14 @@
 // or 128, sequences that bring at least `min_q` tokens to the step (shorter ones are decode8_kernel's).
 //
 // A block owns twice 128 rows (query token, q head of the group) of one (sequence, kv head) and walks the key tiles, 64 keys each, that
-// any of them can see:
+// any of them can see; where those blocks would leave multiprocessors without one, up to 8 of a cluster walk a part of the tiles each and
+// join what they have (its log-sum form, always in the same order) through one another's shared memory.
+//
+// What bounds it: the softmax.  256 rows of 64 keys are 16,384 exponentials, 1,024 cycles of a multiprocessor's, and the tile takes 1,950: the
+// two softmax warps of a scheduler are mostly in the same phase, and loads of scores, the maximum and the barriers are not hidden behind the other's
+// exponentials.  The products take 960 cycles.  2,048 tokens behind 5,952, 32 / 8 heads of 64: 238 us, 492 TFLOP/s (the 16-bit kernel 243);
+// head size 128 426.
+//
 //   warp 12            issues S = Q K^T of either half into one of its two tensor-memory buffers and O += P V into a third; owns the
 //                      allocation;
 //   warps 0..3         bring the codes of a tile into registers while the tile before is worked on, and write it to a ring of
@@ -25,6 +32,8 @@
 #pragma once
 #include "cache8.cuh"
 #include "attention_tc.cuh"        // ft_tile
+#include "cluster.cuh"
+#include <type_traits>
 
 namespace vapi {
 
@@ -76,9 +85,12 @@ __device__ __forceinline__ bool p8_ended(unsigned bar, unsigned parity) {
 // a wait by a whole warp, with one outcome
 __device__ __forceinline__ bool mbar_wait_warp(unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
-template <int HD>
+// JOIN: whether `splits` blocks of a cluster share a tile's keys.  (A kernel of its own: the registers of the join in the same one cost the
+// other 5%.)
+template <int HD, bool JOIN>
 __global__ void __launch_bounds__(P8_THREADS, 1)
-prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int num_seqs, const int min_q) {
+prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int num_seqs, const int min_q,
+               const int blocks) {
     constexpr int STAGES = P8_STAGES<HD>, TILE = P8_TILE<HD>, ATOMS = HD / 64, ATOM = P8_KEYS * 128;     // 64 elements of 64 keys
     extern __shared__ unsigned char p8_smem[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p8_smem) + 1023) & ~(uintptr_t)1023);
@@ -89,14 +101,19 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 32);
     int* flags = reinterpret_cast<int*>(tmem_slot + 1);
     float* sE = reinterpret_cast<float*>(tmem_slot + 4);        // [stage][4]: the scales of the tile's blocks of keys
+    // for the join of a cluster, where Q, P, K and V were: O [row][piece of 16 bytes], then the rows' maxima and sums
+    auto join_at = [&](int r, int piece) { return reinterpret_cast<float*>(base + (size_t)r * HD * 4 + ((piece ^ (r & 7)) << 4)); };
+    float* join_m = reinterpret_cast<float*>(base + P8_ROWS * HD * 4);
+    float* join_l = join_m + P8_ROWS;
+    static_assert(P8_ROWS * HD * 4 + P8_ROWS * 8 <= P8_ROWS * HD * 2 + 2 * P8_ROWS * P8_KEYS * 2 + STAGES * 2 * TILE, "the join fits");
 
     // (by a shuffle: what depends on the warp alone is then known to be the same for all its lanes)
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int g = (int)blockIdx.x % p.nkv, n_rep = p.nh / p.nkv;
+    const int splits = JOIN ? blocks : 1, rank = JOIN ? (int)blockIdx.x % splits : 0, unit = (int)blockIdx.x / splits, g = unit % p.nkv, n_rep = p.nh / p.nkv;
     pdl_trigger();
     // index data was copied from the host before the step's first kernel: safe before the wait
     int s = 0, tile = 0;
-    if (!ft_tile(p.cu_q, num_seqs, min_q, n_rep, P8_ROWS, (int)blockIdx.x / p.nkv, s, tile)) {
+    if (!ft_tile(p.cu_q, num_seqs, min_q, n_rep, P8_ROWS, unit / p.nkv, s, tile)) {        // (the same for the whole cluster)
         pdl_wait();
         return;
     }
@@ -106,8 +123,9 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     const int base_pos = klen - qlen;
     const int p_min = base_pos + tile_start / n_rep, p_max = base_pos + last_row / n_rep;
     const int key_lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
-    const int kt_lo = key_lo / P8_KEYS;
-    const int nt = p_max < key_lo ? 0 : p_max / P8_KEYS - kt_lo + 1;
+    const int nt_all = p_max < key_lo ? 0 : p_max / P8_KEYS - key_lo / P8_KEYS + 1;
+    const int nt_before = (int)((long long)nt_all * rank / splits), nt = (int)((long long)nt_all * (rank + 1) / splits) - nt_before;
+    const int kt_lo = key_lo / P8_KEYS + nt_before;                 // this block's tiles: kt_lo .. kt_lo + nt - 1
 
     const unsigned kv_full = smem_u32(bars), kv_empty = smem_u32(bars + STAGES);
     // of half h and buffer b: 16 h + 8 b bytes further on
@@ -317,11 +335,13 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         float row_f;
         {
             const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(q0 + tok) * p.q_row_stride + (size_t)head * HD);
+            uint4 v[HD / 8];
             float big = 0.f;
 #pragma unroll
+            for (int c = 0; c < HD / 8; ++c) v[c] = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-                const uint4 v = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
             }
@@ -330,8 +350,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             row_f = c8_power(x - 14) * p.scale_log2e;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-                const uint4 v = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
                 unsigned h[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[i] = d8_half2(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
@@ -437,7 +456,26 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         }
         if (ok && nt > 0 && !__all_sync(0xffffffffu, mbar_wait(my_done + 8 * ((nt - 1) & 1), ((nt - 1) >> 1) & 1))) ok = false;
         tc5_fence_after();
-        if (ok) {                                                   // (uniform over the warp)
+        if constexpr (JOIN) {
+            // Every product of the block is awaited by its half, so with both halves here nothing reads Q, P, K or V any more: O goes there,
+            // as floats, a row's pieces of 16 bytes turned by the row so that eight rows' stores meet in no bank.
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+                float o16[16];
+                if (nt > 0 && ok) {
+                    tmem_ld16(tO + lane_addr + j * 16, o16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o16[e] = 0.f;
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<float4*>(join_at(half * P8_HALF + row, j * 4 + c)) = make_float4(o16[4 * c], o16[4 * c + 1], o16[4 * c + 2], o16[4 * c + 3]);
+            }
+            join_m[half * P8_HALF + row] = m_run;
+            join_l[half * P8_HALF + row] = l_run;
+        } else if (ok) {                                            // (uniform over the warp)
             const float inv = l_run == 0.f ? 0.f : 1.f / l_run;     // a row that sees nothing: zeros
             __nv_bfloat16* o = out + ((size_t)(q0 + tok) * p.nh + head) * HD;
 #pragma unroll
@@ -460,6 +498,51 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         }
         if (!ok) flags[0] = 1;
     }
+    if constexpr (JOIN) {
+        if (warp < 4 || warp == P8_THREADS / 32 - 1) __syncthreads();       // (with the softmax warps')
+        cluster_sync();                                             // every block's result is in place
+        const auto join = [&](auto blocks) {
+            constexpr int C = decltype(blocks)::value;
+            // (a block joins rows that follow one another: neighbours' reads of another block's memory are then one; with every C-th piece
+            // a block, 64 KB took 6 us)
+            constexpr int MINE = P8_ROWS / C * (HD / 8);
+            for (int i = rank * MINE + threadIdx.x; i < (rank + 1) * MINE; i += P8_THREADS) {
+                const int r = i / (HD / 8), c = i % (HD / 8), at = tile_start + r;
+                if (at >= rows_total) break;
+                // (everything is asked for before any of it is used: one after the other, 8 blocks' took 10 us)
+                float m[C], l[C], big = -INFINITY, sum = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                float4 o[C][2];
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    m[j] = cluster_f32(cluster_peer(join_m + r, (unsigned)j));
+                    l[j] = cluster_f32(cluster_peer(join_l + r, (unsigned)j));
+                    o[j][0] = cluster_f32x4(cluster_peer(join_at(r, 2 * c), (unsigned)j));
+                    o[j][1] = cluster_f32x4(cluster_peer(join_at(r, 2 * c + 1), (unsigned)j));
+                }
+#pragma unroll
+                for (int j = 0; j < C; ++j) big = fmaxf(big, m[j]);
+                const float used = big == -INFINITY ? 0.f : big;
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    const float f = ex2_approx(m[j] - used);
+                    const float4 a = o[j][0], b = o[j][1];
+                    sum = fmaf(l[j], f, sum);
+                    x[0] = fmaf(a.x, f, x[0]); x[1] = fmaf(a.y, f, x[1]); x[2] = fmaf(a.z, f, x[2]); x[3] = fmaf(a.w, f, x[3]);
+                    x[4] = fmaf(b.x, f, x[4]); x[5] = fmaf(b.y, f, x[5]); x[6] = fmaf(b.z, f, x[6]); x[7] = fmaf(b.w, f, x[7]);
+                }
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                unsigned w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = inv == 0.f ? 0u : pack_bf16(x[2 * e] * inv, x[2 * e + 1] * inv);
+                const int token = at / n_rep;
+                *reinterpret_cast<uint4*>(out + ((size_t)(q0 + token) * p.nh + g * n_rep + (at - token * n_rep)) * HD + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        };
+        if (splits == 2) join(std::integral_constant<int, 2>());
+        else if (splits == 4) join(std::integral_constant<int, 4>());
+        else join(std::integral_constant<int, 8>());
+        cluster_sync();                                             // nobody reads this block's memory any more
+    }
     tc5_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && flags[0] && p.status) atomicExch(p.status, 16);
@@ -469,24 +552,98 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     }
 }
 
+// The limits that a device has to allow, asked once per device, and how many blocks of clusters of 1, 2, 4 and 8 it holds at a time.
 template <int HD>
-static int launch_prompt8(const C8Params& p, const void* q, void* out, int n, int num_seqs, int max_q, int min_q, cudaStream_t stream) {
-    static int ready[64] = {0};
+static int prompt8_ready(const int** slots) {
+    static int held[64][4];
+    static bool ready[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "paged_attention8: cannot tell the current device");
     if (!ready[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(prompt8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P8_SMEM<HD>);
+        cudaError_t e = cudaFuncSetAttribute(prompt8_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P8_SMEM<HD>);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(prompt8_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P8_SMEM<HD>);
         if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", P8_SMEM<HD>, cudaGetErrorString(e));
-        ready[dev] = 1;
+        for (int i = 0; i < 4; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(8u << i);
+            cfg.blockDim = dim3(P8_THREADS);
+            cfg.dynamicSmemBytes = P8_SMEM<HD>;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 1u << i;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int clusters = 0;
+            if (cudaOccupancyMaxActiveClusters(&clusters, prompt8_kernel<HD, true>, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                clusters = 0;
+            }
+            held[dev][i] = clusters << i;
+        }
+        ready[dev] = true;
     }
+    *slots = held[dev];
+    return 0;
+}
+
+// How many blocks share the keys of a tile of rows, and how long the step then takes, in microseconds: rounds of blocks, each of a time a key
+// tile and one beside (start, Q, the last stores; in a cluster its blocks' wait for one another and the join).  32 / 8 heads of 64, us with 1, 2, 4
+// and 8 blocks: 64 tokens behind 3,936 75 / 44 / 28 / 22; 256 behind 3,744 76 / 44 / 30 / 67; 512 behind 3,488 76 / 44 / 59 / 113; 2,048 behind
+// 5,952 238 / 279 / 341 / 520.  Head size 128: 128 behind 3,872 124 / 71 / 44 / 69; 1,024 behind 2,976 125 / 130 / 176 / 314.
+template <int HD>
+static int p8_splits(long long units, int tiles, const int* slots, float& least) {
+    const float tile = HD == 64 ? 1.05f : 1.85f, size = HD == 64 ? 1.f : 1.5f;
+    int best = 1;
+    for (int i = 0; i < 4; ++i) {
+        const int c = 1 << i, held = slots[i] > 0 ? slots[i] : 1;
+        if (i > 0 && (slots[i] < c || tiles < 2 * c)) break;
+        const float time = (float)((units * c + held - 1) / held) * ((float)((tiles + c - 1) / c) * tile + (i == 0 ? 7.f : (8.f + c / 2) * size));
+        if (i == 0 || time < least) { best = c; least = time; }
+    }
+    return best;
+}
+// the same of a step: n tokens of sequences with at most max_k keys
+template <int HD>
+static int p8_step(const C8Params& p, int n, int max_k, float& time) {
+    time = INFINITY;
+    const int* slots = nullptr;
+    if (prompt8_ready<HD>(&slots) != 0) return 1;
+    const int n_rep = p.nh / p.nkv;
+    const long long units = ((long long)n * n_rep + P8_ROWS - 1) / P8_ROWS * p.nkv;
+    const long long seen = (long long)p.window + P8_ROWS / n_rep, keys = p.window > 0 && seen < max_k ? seen : max_k;
+    return p8_splits<HD>(units, (int)((keys + P8_KEYS - 1) / P8_KEYS), slots, time);
+}
+
+template <int HD>
+static int launch_prompt8(const C8Params& p, const void* q, void* out, int n, int num_seqs, int max_q, int max_k, int min_q, int splits, cudaStream_t stream) {
+    const int* slots = nullptr;
+    const int rc = prompt8_ready<HD>(&slots);
+    if (rc != 0) return rc;
     // tiles of all sequences together: at most those of n tokens in one piece and a ragged one a sequence of at least min_q tokens
     const int n_rep = p.nh / p.nkv;
     const long long longest = ((long long)max_q * n_rep + P8_ROWS - 1) / P8_ROWS, most = n / min_q < num_seqs ? n / min_q : num_seqs;
     const long long whole = (long long)n * n_rep / P8_ROWS + most, tiles = longest * most < whole ? longest * most : whole;
     if (tiles == 0) return 0;
-    if (tiles * p.nkv > 0x7fffffffLL) return fail(-1, "paged_attention8: the step exceeds the grid (%lld row tiles, %d kv heads)", tiles, p.nkv);
-    return check_launch("paged_attention8 (tcgen05)", launch(prompt8_kernel<HD>, dim3((unsigned)(tiles * p.nkv)), P8_THREADS, P8_SMEM<HD>, stream, p,
-                                                             (const __nv_bfloat16*)q, (__nv_bfloat16*)out, num_seqs, min_q));
+    float time;
+    if (splits <= 0) splits = p8_step<HD>(p, n, max_k, time);
+    splits = splits >= 8 ? 8 : splits >= 4 ? 4 : splits >= 2 ? 2 : 1;      // (what the kernel joins)
+    if (tiles * p.nkv * splits > 0x7fffffffLL) return fail(-1, "paged_attention8: the step exceeds the grid (%lld row tiles, %d kv heads)", tiles, p.nkv);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * p.nkv * splits));
+    cfg.blockDim = dim3(P8_THREADS);
+    cfg.dynamicSmemBytes = P8_SMEM<HD>;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return check_launch("paged_attention8 (tcgen05)", cudaLaunchKernelEx(&cfg, splits > 1 ? prompt8_kernel<HD, true> : prompt8_kernel<HD, false>, p,
+                                                                         (const __nv_bfloat16*)q, (__nv_bfloat16*)out, num_seqs, min_q, splits));
 }
 
 }  // namespace vapi

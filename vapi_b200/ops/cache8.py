@@ -126,14 +126,15 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     """:func:`paged_attention` over a cache in 8 bits; returns [n, nh*d].  Arguments as there; the numbers of the cache are taken
     exactly, scores, softmax and sums are float32.  A query without a visible key gets zeros.
 
-    ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions long enough to fill the device, and the
-    mma.sync kernel, whose ``splits`` (up to 16) blocks share the keys as a cluster, for the others; the general kernel for every other
-    type, head size (a multiple of 16 up to 256) and alignment.  "tcgen05", "tensor_core" and "general" force one (the first two raise where
+    ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions (where rows and keys are enough for
+    it), and the mma.sync kernel for the others, in both of which ``splits`` blocks (up to 16, and up to 8) share the keys as a cluster; the
+    general kernel for every other type, head size (a multiple of 16 up to 256) and alignment.  "tcgen05", "tensor_core" and "general" force one (the first two raise where
     they do not apply)."""
     code = _IMPL8.get(impl)
     kernels = 1 if n > 0 else 0
-    if max_q >= _PORTION8_MIN_Q and num_seqs > 1 and code == 0 and q.dtype == torch.bfloat16 and d in (64, 128) and nkv > 0 and q.is_cuda:
-        kernels *= int(_lib("cache8").vapi_attention8_kernels(num_seqs, max_q, nh, nkv))
+    if (max_q >= _PORTION8_MIN_Q and num_seqs > 1 and code == 0 and q.dtype == torch.bfloat16 and d in (64, 128) and nkv > 0 and q.is_cuda and scale > 0
+            and q_row_stride % 8 == 0 and q.data_ptr() % 16 == 0):
+        kernels *= int(_lib("cache8").vapi_attention8_kernels(n, num_seqs, max_q, max_k, nh, nkv, d, window))
     if q.is_cuda and code is not None:
         lib = _lib("cache8")
         got = _native("attention8", lib, "vapi_paged_attention8", q, q_row_stride, cache[0], cache[1], block_table, cu_q, seqlens_k, n, num_seqs,
