@@ -401,6 +401,58 @@ def test_a_query_without_keys_gets_zeros_and_a_bad_page_a_status():
 
 
 @gpu
+@pytest.mark.parametrize("d,impl", [(64, "tensor_core"), (128, "tensor_core"), (64, "tcgen05"), (128, "tcgen05"), (64, "general"), (48, "auto")])
+@pytest.mark.parametrize("lens,news", [([200, 333], [1, 1]), ([500, 99], [150, 40])])
+def test_what_a_window_has_left_behind_is_not_looked_up(d, impl, lens, news):
+    """Pages before every row's window are no pages any more, and what no row sees in the first that is one, or behind the last, is NaN."""
+    window, dtype = 21, torch.bfloat16
+    c = _attention_case(lens, news, 4, 2, d, 16, dtype, d + len(impl))
+    raw = c["codes"].view(torch.uint8)
+    for s, (k, n) in enumerate(zip(lens, news)):
+        least = k - n - window + 1                       # the first key that a row sees
+        c["table"][s, :least // 16] = -1
+        raw[c["table"][s, least // 16].long(), :, :, :least % 16] = 0x7f
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for splits in (1, 4):
+        got = _run_attention(c, d ** -0.5, window, splits=splits, impl=impl, status=status)
+        assert int(status) == 0
+        _portion_check(_seen_only(c), got, d ** -0.5, window)
+
+
+def _seen_only(c):
+    """The case with numbers where there is no page and where nothing is seen (the plain form takes 0 * NaN)."""
+    c = dict(c)
+    raw = c["codes"].view(torch.uint8).clone()
+    raw[(raw & 0x7f) == 0x7f] = 0
+    c["codes"], c["table"] = raw.view(torch.float8_e4m3fn), c["table"].clamp(min=0)
+    return c
+
+
+@gpu
+def test_pages_beyond_32_bits_of_offset():
+    """A cache of 4.6 GB, of which the first and the last pages are written, read and attended to."""
+    ops = _ops()
+    nh, nkv, d, page, pages = 8, 2, 128, 64, 141_000
+    cache = ops.cache8_empty(pages, nkv, page, d)
+    assert cache.codes.numel() > 2 ** 32
+    n = 3 * page
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(n, (nh + 2 * nkv) * d, generator=g).bfloat16().cuda()
+    ids = torch.tensor([pages - 1, 0, pages - 2], dtype=torch.int32)
+    slots = (ids[:, None].long() * page + torch.arange(page)).view(-1).int().cuda()
+    q = ops.qk_norm_rope_write8(qkv, nh, nkv, d, None, None, 0.0, None, None, 0, cache, slots)
+    back = ops.cache8_read(cache, ids.cuda(), torch.bfloat16)
+    small = ops.cache8_empty(3, nkv, page, d)
+    assert torch.equal(q, ops.qk_norm_rope_write8(qkv, nh, nkv, d, None, None, 0.0, None, None, 0, small, torch.arange(n, dtype=torch.int32, device="cuda")))
+    assert torch.equal(back, ops.cache8_read(small, torch.arange(3, dtype=torch.int32, device="cuda"), torch.bfloat16))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    for impl in ("tensor_core", "tcgen05", "general"):
+        a, b = (ops.paged_attention8(q, nh * d, where, table[None], i32(0, n), i32(n), n, 1, n, n, nh, nkv, d, d ** -0.5, impl=impl)
+                for where, table in ((cache, ids.cuda()), (small, i32(0, 1, 2))))
+        assert torch.equal(a, b), impl
+
+
+@gpu
 def test_queries_of_unlike_size_and_blocks_of_unlike_scale():
     """Rows of queries from 2^-60 to 2^60 (their scores scaled back), values from 2^-80 to 2^80 in neighbouring blocks: no row loses its own."""
     c = _attention_case([100], [1], 8, 2, 64, 16, torch.bfloat16, 9)

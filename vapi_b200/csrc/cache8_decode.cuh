@@ -19,8 +19,8 @@
 //                to 2^15, float the sums), which no lane has to ask its neighbours for: a vote a chunk, and a reduction a few times
 //                a row.  P is turned about by movmatrix; the values of two tokens are paired by byte permutes.
 //
-// Keys behind a sequence's end are masked by selection, and their values taken as zeros.  (A NaN among the keys and values that a
-// sequence did write, though a row may not see it, can reach that row through 0 * NaN; the step that wrote it was lost.)
+// Keys that a row does not see are masked by selection, and the values of those that no row of the block sees taken as zeros.  (A NaN among the
+// values that some of the block's rows see and others do not can reach the others through 0 * NaN; the step that wrote it was lost.)
 #pragma once
 #include "cache8.cuh"
 #include "cluster.cuh"
@@ -311,7 +311,8 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                     const uint4 x = d8_lds16(at);
                     v[i][0] = x.x; v[i][1] = x.y; v[i][VW - 2] = x.z; v[i][VW - 1] = x.w;
                 }
-                if (edge && k0 + j * C8_BLOCK + 4 * i + tq >= klen) {
+                const int key = k0 + j * C8_BLOCK + 4 * i + tq;
+                if (edge && (key > p_max || key < key_lo)) {                // (what no row sees may be anything)
 #pragma unroll
                     for (int c = 0; c < VW; ++c) v[i][c] = 0u;
                 }

@@ -27,7 +27,8 @@
 //   V: O is one sum over all tiles, so V must be on one scale; code * 2^e is a bfloat16 number exactly, and P is bfloat16 as in
 //      the 16-bit kernel.
 //
-// Keys behind the last that a row of the block sees are masked by selection, and their values written as zeros.  Every wait is bounded; a role that
+// Keys that a row does not see are masked by selection, and the values of those that no row of the block sees are written as zeros.  (A NaN among the
+// values that some of the block's rows see and others do not can reach the others through 0 * NaN; the step that wrote it was lost.)  Every wait is bounded; a role that
 // gives up records status 16 and the block drains (tensor memory is released on every path).
 #pragma once
 #include "cache8.cuh"
@@ -235,14 +236,16 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         bool waited = false;
         // Where the 32 blocks of eight tiles lie, one a lane, and their scales.  Looked up in two steps, both well before they are
         // wanted: a tile's codes are asked for two tiles ahead, and waiting for the table first would double the way.
+        // Blocks before the window of the block's first row are not looked up either: their pages may have been given back.
+        const int first = key_lo / C8_BLOCK * C8_BLOCK;
         auto key_of = [&](int from) { return (kt_lo + from) * P8_KEYS + lane * C8_BLOCK; };
         auto pages = [&](int from) {                             // of tiles from .. from + 7
             const int key = key_of(from);
-            return from + (lane >> 2) < nt && key <= p_max ? bt[key / p.page_size] : -1;
+            return from + (lane >> 2) < nt && key >= first && key <= p_max ? bt[key / p.page_size] : -1;
         };
         auto places = [&](int from, int page) {
             const int key = key_of(from);
-            if (!(from + (lane >> 2) < nt && key <= p_max)) return 0;             // (no row sees it: any block, and masked)
+            if (!(from + (lane >> 2) < nt && key >= first && key <= p_max)) return 0;             // (no row sees it: any block, and masked)
             if (page < 0 || page >= p.num_pages) {
                 if (p.status) atomicExch(p.status, 4);
                 page = 0;
@@ -288,7 +291,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
                 uint4 lo, hi;
                 if (kind == 0) {
                     p8_halves(from.codes[j], lo, hi);
-                } else if (k0 + r <= p_max) {                   // (what no row sees may be anything)
+                } else if (k0 + r >= key_lo && k0 + r <= p_max) {       // (what no row sees may be anything)
                     p8_numbers(from.codes[j], c8_power(e), lo, hi);
                 } else {
                     lo = hi = make_uint4(0u, 0u, 0u, 0u);

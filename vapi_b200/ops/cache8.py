@@ -50,7 +50,8 @@ def qk_norm_rope_write8(qkv: torch.Tensor, nh: int, nkv: int, d: int, q_weight: 
     [n, (nh+2nkv)*d], which is left as it was; returns q [n, nh*d], and writes the keys (normed, rotated, rounded to the
     activations' type) and the values to ``cache`` at ``slot_mapping``.
 
-    Tokens of one block of 16 must follow one another in the step, as a request's do.  A block whose first token (place 0) is
+    Tokens of one block of 16 must follow one another in the step, as a request's do, and no two name one slot (what such a block then
+    holds is not said: its tokens may be on another's scale).  A block whose first token (place 0) is
     among them begins afresh; the older tokens of another one are rounded again when a new token needs a larger scale.  What
     is not finite is kept as NaN."""
     if qkv.is_cuda:
@@ -124,7 +125,9 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
                      scale: float, window: int = 0, splits: Optional[int] = None, status: Optional[torch.Tensor] = None,
                      impl: str = "auto") -> torch.Tensor:
     """:func:`paged_attention` over a cache in 8 bits; returns [n, nh*d].  Arguments as there; the numbers of the cache are taken
-    exactly, scores, softmax and sums are float32.  A query without a visible key gets zeros.
+    exactly, scores, softmax and sums are float32.  A query without a visible key gets zeros.  Pages before the window and behind a
+    request's end are not looked at.  A value that is not a number reaches the queries that see its token, and on the tensor cores also those
+    of the same portion that stand before it in one tile, as with :func:`paged_attention`.
 
     ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions (where rows and keys are enough for
     it), and the mma.sync kernel for the others, in both of which ``splits`` blocks (up to 16, and up to 8) share the keys as a cluster; the
