@@ -71,6 +71,19 @@ def test_what_does_not_fit_is_refused():
     assert not ops.few_rows_applies(1, w)
 
 
+def test_a_weight_of_another_layout_is_refused():
+    ops = _ops()
+    for group in (32, 64):
+        w = ops.int4_pack(*_random(24, 192, group, 2))
+        same = ops.Int4Weight(w.codes, w.scales, 24, 192, group)
+        assert same.shape == (24, 192)
+        for args, words in (((w.codes, w.scales, 40, 192, group), "codes"), ((w.codes, w.scales, 24, 256, group), "codes"), ((w.codes, w.scales, 24, 192, 48), "groups of 48"),
+                            ((w.codes, w.scales[:, :1], 24, 192, group), "scales"), ((w.codes.float(), w.scales, 24, 192, group), "int32"), ((w.codes, w.scales, 0, 192, group), "0 x 192"),
+                            ((w.codes[:, ::2], w.scales, 24, 128, group), "codes")):
+            with pytest.raises(ops.KernelError, match=words):
+                ops.Int4Weight(*args)
+
+
 def _to_device(w):
     return _ops().Int4Weight(w.codes.cuda(), w.scales.cuda(), w.n, w.k, w.group)
 

@@ -17,13 +17,20 @@ INT4_MAX_ROWS = int(os.environ.get("VAPI_INT4_MAX_ROWS", "64"))
 
 
 class Int4Weight:
-    """A matrix [n, k] of numbers ``(code - zero) * scale`` as the kernels read it (:func:`int4_pack`, :func:`int4_quantize`): codes and
-    zeros in 0..15, a bfloat16 scale and a zero for each group of ``group`` columns of a row."""
+    """A matrix [n, k] of numbers ``(code - zero) * scale`` as the kernels read it (:func:`int4_pack` and :func:`int4_quantize` make one): codes
+    and zeros in 0..15, a bfloat16 scale and a zero for each group of ``group`` columns of a row."""
 
     __slots__ = ("codes", "scales", "n", "k", "group")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, group: int):
         self.codes, self.scales, self.n, self.k, self.group = codes, scales, int(n), int(k), int(group)
+        n, k, group = self.n, self.k, self.group
+        if n <= 0 or k <= 0 or group not in INT4_GROUPS or k % group:
+            raise KernelError(f"a 4-bit weight of {n} x {k} in groups of {group}")
+        tiles, chunks = -(-n // 16), -(-k // 64)
+        for t, shape, what in ((codes, (tiles, chunks, 32, 4), "codes"), (scales, (tiles, 2 * chunks if group == 32 else k // group, 8, 2), "scales")):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise KernelError(f"the {what} of a 4-bit weight must be {shape} of int32 in one piece, got {tuple(t.shape)} of {t.dtype}")
 
     @property
     def shape(self) -> Tuple[int, int]:
