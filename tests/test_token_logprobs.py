@@ -82,6 +82,16 @@ def test_rows_at_any_stride_and_many_rows(dtype):
 
 
 @gpu
+def test_rows_further_apart_than_32_bits():
+    ops = _ops()
+    x, t = _logits(2, 5000, 8, torch.bfloat16)
+    stride = 2 ** 31 + 8
+    wide = torch.empty(stride + 5000, dtype=torch.bfloat16, device="cuda").as_strided((2, 5000), (stride, 1))
+    wide.copy_(x)
+    _check(x, t, ops.token_logprobs(wide, t.cuda(), 7), 7)
+
+
+@gpu
 @pytest.mark.parametrize("slices", [1, 2, 8])
 def test_ties_and_rows_made_to_fill_the_list(slices):
     """Equal logits go by id; descending and ascending rows; the largest all in the elements of a few threads (more above the bound
