@@ -124,15 +124,50 @@ def test_few_rows(n, k, group, rows):
     g = torch.Generator().manual_seed(rows)
     x = (torch.randn(rows, k, generator=g) * torch.exp(torch.randn(1, k, generator=g))).bfloat16()
     bias = torch.randn(n, generator=g)
+    # (above 32 rows a weight's number is rounded to bfloat16: half a step, at most 2^-8 of the number, so of the sum of magnitudes)
+    rounded = rows > 32
     got = ops.int4_linear(x.cuda(), d)
     assert got.dtype == torch.bfloat16
-    _check(x, w, got)
+    _check(x, w, got, rounded=rounded)
     assert torch.equal(ops.linear(x.cuda(), d), got)
-    _check(x, w, ops.int4_linear(x.cuda(), d, bias.cuda()), bias)
-    _check(x, w, ops.int4_linear(x.cuda(), d, bias.cuda(), torch.float32), bias)
+    _check(x, w, ops.int4_linear(x.cuda(), d, bias.cuda()), bias, rounded=rounded)
+    _check(x, w, ops.int4_linear(x.cuda(), d, bias.cuda(), torch.float32), bias, rounded=rounded)
     if n % 2 == 0:
         for act in ("silu", "gelu_tanh"):
-            _check(x, w, ops.linear_swiglu(x.cuda(), d, act), act=act, rounded=n % 32 != 0)
+            _check(x, w, ops.linear_swiglu(x.cuda(), d, act), act=act, rounded=rounded or n % 32 != 0)
+
+
+@gpu
+@pytest.mark.parametrize("n,k,group", [(2048, 8192, 128), (16416, 1024, 64), (8200, 2080, 32)])
+@pytest.mark.parametrize("rows", [100, 129, 300, 512])
+def test_rows_enough_for_a_tile(n, k, group, rows):
+    """Weights large enough for the tcgen05 kernel at any of these rows; all the same a second time, and in a graph."""
+    ops = _ops()
+    w = ops.int4_pack(*_random(n, k, group, n + rows))
+    d = _to_device(w)
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn(rows, k, generator=g) * torch.exp(torch.randn(1, k, generator=g))).bfloat16()
+    bias, dev = torch.randn(n, generator=g), x.cuda()
+    db = bias.cuda()
+    before = ops.launch_count
+    got = ops.int4_linear(dev, d, db)
+    assert ops.launch_count == before + 1
+    _check(x, w, got, bias, rounded=True)
+    wide = ops.int4_linear(dev, d, db, torch.float32)
+    assert torch.equal(wide.bfloat16(), got) and torch.equal(ops.int4_linear(dev, d, db), got)
+    if n % 32 == 0:
+        _check(x, w, ops.int4_linear_swiglu(dev, d), rounded=True, act="silu")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ops.int4_linear(dev, d, db)
+    dev.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, bias.bfloat16().cuda().expand(rows, n))
+    dev.copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, got)
 
 
 @gpu

@@ -71,20 +71,12 @@ __device__ __forceinline__ void p8_numbers(const uint4& c, float f, uint4& lo, u
     hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
-// one lane of a whole warp, the same every time
-__device__ __forceinline__ bool p8_elect() {
-    unsigned yes;
-    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
-    return yes != 0;
-}
 // whether a phase has ended, without waiting for it
 __device__ __forceinline__ bool p8_ended(unsigned bar, unsigned parity) {
     unsigned yes;
     asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes) : "r"(bar), "r"(parity) : "memory");
     return yes != 0;
 }
-// a wait by a whole warp, with one outcome
-__device__ __forceinline__ bool mbar_wait_warp(unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
 // JOIN: whether `splits` blocks of a cluster share a tile's keys.  (A kernel of its own: the registers of the join in the same one cost the
 // other 5%.)
@@ -156,7 +148,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     if (warp == P8_THREADS / 32 - 1) {
         {
             // (the whole warp goes through the loop and waits; one lane issues)
-            const bool leader = p8_elect();
+            const bool leader = elect_lane();
             // instruction descriptors: float accumulate, N = 64, M = 128; f16 x f16, both K-major, and bf16 x bf16 with V's
             // contiguous dimension N
             const unsigned shape = (1u << 4) | ((unsigned)(P8_KEYS >> 3) << 17) | ((unsigned)(P8_HALF >> 4) << 24);

@@ -16,6 +16,7 @@
 using namespace vapi;
 
 constexpr int I4_WARPS = 8;
+constexpr int I4_MOST_ROWS = 32;                   // of int4_rows_kernel; more go to int4_tile_kernel
 constexpr int I4_TILE_WORDS = 128;                 // 16 x 64 codes
 
 struct I4Params {
@@ -41,6 +42,8 @@ __device__ __forceinline__ __nv_bfloat162 i4_zero(unsigned w) {
     return *reinterpret_cast<const __nv_bfloat162*>(&u);
 }
 __device__ __forceinline__ float i4_scale(unsigned w) { return __uint_as_float(w << 16); }
+
+#include "int4_tile.cuh"
 
 // ---- few rows -------------------------------------------------------------------------------------
 // A block owns WN tile rows (16 features each; for a gated product half of them the gate's and half up's) and 8 NT rows of x; its eight
@@ -281,10 +284,15 @@ VAPI_EXPORT int vapi_int4_linear(const void* codes, const void* scales, int n, i
     if (k % group != 0) return fail(-1, "int4_linear: %d columns are not a multiple of the group's %d", k, group);
     if (gated && (n % 32 != 0 || bias || y32)) return fail(-1, "int4_linear: a gated product needs a multiple of 32 features (got %d), no bias and bfloat16 results", n);
     if ((((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)x) & 15) != 0) return fail(-1, "int4_linear: an operand is not 16-byte aligned");
-    if (rows > 65535 * 32) return fail(-1, "int4_linear: %d rows exceed the grid", rows);
+    if (rows > 65535 * 128) return fail(-1, "int4_linear: %d rows exceed the grid", rows);
     I4Params p;
     p.codes = (const unsigned*)codes; p.scales = (const unsigned*)scales; p.n = n; p.k = k; p.group = group; p.chunks = (k + 63) / 64;
     p.x = (const __nv_bfloat16*)x; p.rows = rows; p.bias = bias; p.y = (__nv_bfloat16*)y; p.y32 = y32; p.act = act;
+    if (rows > I4_MOST_ROWS) {
+        if (group == 32) return int4_tile<2>(p, gated != 0, stream);
+        if (group == 64) return int4_tile<4>(p, gated != 0, stream);
+        return int4_tile<8>(p, gated != 0, stream);
+    }
     if (group == 32) return int4_rows<2>(p, gated != 0, stream);
     if (group == 64) return int4_rows<4>(p, gated != 0, stream);
     return int4_rows<8>(p, gated != 0, stream);

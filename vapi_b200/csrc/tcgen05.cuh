@@ -30,6 +30,14 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
     }
     return false;
 }
+// the same by a whole warp, with one outcome
+__device__ __forceinline__ bool mbar_wait_warp(unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// one lane of a whole warp, the same every time
+__device__ __forceinline__ bool elect_lane() {
+    unsigned yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
+}
 // the same for a role of a block, which also ends when another role has given up
 __device__ __forceinline__ bool mbar_wait_role(unsigned bar, unsigned parity, volatile int* abort_flag, unsigned polls = TC5_WAIT_LIMIT) {
     for (unsigned i = 0; i < polls; ++i) {

@@ -12,8 +12,12 @@ from . import linear_swiglu as _linear_swiglu
 from . import swiglu as _swiglu
 
 INT4_GROUPS = (32, 64, 128)
-#: products of more rows than this take the weight as bfloat16 numbers through this package's and the library's products
-INT4_MAX_ROWS = int(os.environ.get("VAPI_INT4_MAX_ROWS", "64"))
+#: products of more bfloat16 rows than this take the weight as bfloat16 numbers through this package's and the library's products, and from
+#: _SMALL_ROWS rows on those of weights of fewer than _LARGE numbers do: writing a weight out costs 0.43 us for each million of its numbers, the
+#: kernel's lesser rate a fifth of the product.  us of the kernel and of the other form: 6,144 x 2,048, 128 rows 11 / 13, 256 rows 15 / 14; 16,384 x 2,048
+#: gated, 256 rows 20 / 33, 512 rows 38 / 43, 1,024 rows 74 / 66; 8,192 x 28,672, 512 rows 214 / 274
+INT4_MAX_ROWS = int(os.environ.get("VAPI_INT4_MAX_ROWS", "512"))
+_SMALL_ROWS, _LARGE = 128, 1 << 24
 
 
 class Int4Weight:
@@ -134,6 +138,11 @@ def int4_dequantize(w: Int4Weight, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
+def _own(rows: int, w: Int4Weight) -> bool:
+    """Whether a product of so many bfloat16 rows is csrc/int4.cu's."""
+    return rows <= INT4_MAX_ROWS and (rows <= _SMALL_ROWS or w.n * w.k >= _LARGE)
+
+
 def _rows(x: torch.Tensor, w: Int4Weight, bias, out: torch.Tensor, gated: int, act: int) -> torch.Tensor:
     lib = _lib("int4")
     f32 = out.dtype == torch.float32
@@ -145,10 +154,10 @@ def _rows(x: torch.Tensor, w: Int4Weight, bias, out: torch.Tensor, gated: int, a
 def int4_linear(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """:func:`linear` with a 4-bit weight: ``x @ W.T (+ bias)`` for ``x`` [n, k], in ``out_dtype`` (the type of ``x``, or float32).
 
-    Up to INT4_MAX_ROWS bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in
-    float32, and the result is rounded once.  Larger steps, and float32 ones, take the weight as numbers of the type of ``x``
-    (:func:`int4_dequantize`) through :func:`linear`."""
-    if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] <= INT4_MAX_ROWS and out_dtype in (None, torch.bfloat16, torch.float32):
+    Up to 32 bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in float32, and the
+    result is rounded once.  More rows take the weight's numbers rounded to bfloat16, in the product itself up to INT4_MAX_ROWS rows, else,
+    as float32 ``x`` does with them in float32, through :func:`int4_dequantize` and :func:`linear`."""
+    if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and _own(x.shape[0], w) and out_dtype in (None, torch.bfloat16, torch.float32):
         lib = _lib("int4")
         got = _native("int4", lib, "vapi_int4_linear", w.codes, w.scales, w.n, w.k, w.group, x, bias, 0, 0, int(out_dtype == torch.float32))
         if got is not NotImplemented:
@@ -158,14 +167,14 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = N
     _bias(bias, w.n)
     if out_dtype not in (None, x.dtype, torch.float32):
         raise KernelError(f"a 4-bit product of {x.dtype} gives {x.dtype} or float32, not {out_dtype}")
-    if _DT[x.dtype] == BF16 and x.shape[0] <= INT4_MAX_ROWS:
+    if _DT[x.dtype] == BF16 and _own(x.shape[0], w):
         return _rows(x, w, bias, torch.empty((x.shape[0], w.n), dtype=out_dtype or x.dtype, device=x.device), 0, 0)
     return _linear(x, int4_dequantize(w, x.dtype), bias, out_dtype)
 
 
 def int4_linear_swiglu(x: torch.Tensor, w: Int4Weight, act: str = "silu") -> torch.Tensor:
     """:func:`linear_swiglu` with a 4-bit weight [Wg; Wu]: ``act(x @ Wg.T) * (x @ Wu.T)``, the gate in the product's epilogue."""
-    if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] <= INT4_MAX_ROWS and w.n % 32 == 0:
+    if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and _own(x.shape[0], w) and w.n % 32 == 0:
         lib = _lib("int4")
         got = _native("int4", lib, "vapi_int4_linear", w.codes, w.scales, w.n, w.k, w.group, x, None, 1, _glu(act), 0)
         if got is not NotImplemented:
@@ -175,7 +184,7 @@ def int4_linear_swiglu(x: torch.Tensor, w: Int4Weight, act: str = "silu") -> tor
     if w.n % 2:
         raise KernelError("a gated product needs an even number of features")
     kind = _glu(act)
-    if _DT[x.dtype] == BF16 and x.shape[0] <= INT4_MAX_ROWS:
+    if _DT[x.dtype] == BF16 and _own(x.shape[0], w):
         if w.n % 32 == 0:
             return _rows(x, w, None, torch.empty((x.shape[0], w.n // 2), dtype=x.dtype, device=x.device), 1, kind)
         return _swiglu(int4_linear(x, w), act)
