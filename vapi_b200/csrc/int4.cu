@@ -16,7 +16,10 @@
 using namespace vapi;
 
 constexpr int I4_WARPS = 8;
-constexpr int I4_MOST_ROWS = 32;                   // of int4_rows_kernel; more go to int4_tile_kernel
+// Rows of int4_rows_kernel; more go to int4_tile_kernel, which takes the time of 64 for any number up to that.  us of the one with as many rows as it can
+// hold (32) and of the other: 2,048 x 2,048, 24 rows 5.4 / 6.0, 32 rows 8.5 / 6.2; 16,384 x 2,048 gated 12.3 / 12.8 and 14.2 / 12.8; 2,048 x 8,192 9.3 / 11.5
+// and 12.0 / 11.8; 13,824 x 1,536 gated 9.4 / 10.6 and 11.6 / 10.2.
+constexpr int I4_MOST_ROWS = 24;
 constexpr int I4_TILE_WORDS = 128;                 // 16 x 64 codes
 
 struct I4Params {
@@ -54,7 +57,7 @@ __device__ __forceinline__ float i4_scale(unsigned w) { return __uint_as_float(w
 // would be most of the traffic.  Partial results are added in the order of slices, then of blocks.
 constexpr int I4_PART = 8 * 16;                    // rows of partial results: eight warps x 16 features
 
-template <int NT> constexpr int I4_SEG = NT >= 3 ? 16 : 32;              // tiles of columns of x that shared memory holds at most
+template <int NT> constexpr int I4_SEG = NT >= 3 ? 24 : 32;              // tiles of columns of x that shared memory holds at most
 template <int NT> constexpr int I4_AHEAD = NT >= 3 ? 4 : 6;
 
 template <int NT, int GS, bool GLU>                // GS: k-steps of 16 columns a group (2, 4, 8)
@@ -224,12 +227,14 @@ int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg
     if (splits > 1) cluster_sync();                // nobody reads this block's memory any more
 }
 
-// How the work falls to blocks: as many tile rows a block (1, 2, 4 or 8) as leave about two blocks a multiprocessor, and at least NT, so that x is
-// not read more often than the weights; then, while there are fewer blocks, a cluster of up to 8 shares the columns as long as each
-// warp still has four tiles.
+// How the work falls to blocks: as many tile rows a block (1, 2, 4 or 8) as leave about two blocks a multiprocessor, and where K is long at least NT,
+// so that x is not read more often than the weights (of a short K, blocks are worth more: 16 rows, one tile row a block or two, 2,048 x 2,048 3.8 / 4.5
+// us, 2,048 x 8,192 8.5 / 7.4; 19 rows, two or four, 2,048 x 2,048 5.4 / 6.8, 2,048 x 8,192 9.2 / 9.3, 8,192 x 28,672 84 / 68); then, while there are fewer
+// blocks, a cluster of up to 8 shares the columns as long as each warp still has four tiles.
 static void int4_shape(int tiles, int chunks, int nt, bool glu, int& wn, int& splits) {
+    const int least = nt == 1 ? 1 : nt == 2 ? (chunks > 48 ? 2 : 1) : (chunks > 128 ? 4 : 2);
     wn = glu ? 2 : 1;
-    while (wn < 8 && (wn < nt || (tiles + wn - 1) / wn > 2 * sm_count())) wn *= 2;
+    while (wn < 8 && (wn < least || (tiles + wn - 1) / wn > 2 * sm_count())) wn *= 2;
     const long long blocks = (tiles + wn - 1) / wn;
     splits = 1;
     while (splits < 8 && 2 * splits * blocks <= 2LL * sm_count() && chunks / (2 * splits * (I4_WARPS / wn)) >= 4) splits *= 2;
@@ -270,8 +275,7 @@ template <int GS>
 static int int4_rows(const I4Params& p, bool glu, cudaStream_t stream) {
     if (p.rows <= 8) return glu ? launch_int4_rows<1, GS, true>(p, stream) : launch_int4_rows<1, GS, false>(p, stream);
     if (p.rows <= 16) return glu ? launch_int4_rows<2, GS, true>(p, stream) : launch_int4_rows<2, GS, false>(p, stream);
-    if (p.rows <= 24) return glu ? launch_int4_rows<3, GS, true>(p, stream) : launch_int4_rows<3, GS, false>(p, stream);
-    return glu ? launch_int4_rows<4, GS, true>(p, stream) : launch_int4_rows<4, GS, false>(p, stream);
+    return glu ? launch_int4_rows<3, GS, true>(p, stream) : launch_int4_rows<3, GS, false>(p, stream);
 }
 
 // x [rows][k] bfloat16 with 16-byte aligned rows.  gated: W is [gate; up], y [rows][n / 2] = act(gate) * up, n / 2 a multiple of 16.

@@ -154,7 +154,7 @@ def _rows(x: torch.Tensor, w: Int4Weight, bias, out: torch.Tensor, gated: int, a
 def int4_linear(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """:func:`linear` with a 4-bit weight: ``x @ W.T (+ bias)`` for ``x`` [n, k], in ``out_dtype`` (the type of ``x``, or float32).
 
-    Up to 32 bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in float32, and the
+    Up to 24 bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in float32, and the
     result is rounded once.  More rows take the weight's numbers rounded to bfloat16, in the product itself up to INT4_MAX_ROWS rows, else,
     as float32 ``x`` does with them in float32, through :func:`int4_dequantize` and :func:`linear`."""
     if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and _own(x.shape[0], w) and out_dtype in (None, torch.bfloat16, torch.float32):
