@@ -356,6 +356,22 @@ def test_attention_split_over_a_cluster(splits, rows):
 
 
 @gpu
+@pytest.mark.parametrize("d,nh,nkv", [(64, 16, 8), (128, 8, 4)])
+@pytest.mark.parametrize("rows,window", [(1, 0), (1, 40), (5, 0)])
+def test_many_requests_of_few_keys(d, nh, nkv, rows, window):
+    """More blocks than the device holds at once, which then have four warps; requests of one key and of none among them."""
+    S = 100
+    lens = [1 + (37 * i) % 300 for i in range(S)]
+    lens[3] = 1000
+    news = [min(rows, k) if i % 5 else 1 for i, k in enumerate(lens)]
+    c = _attention_case(lens, news, nh, nkv, d, 16, torch.bfloat16, rows + d)
+    c["kl"][7] = 0
+    got = _run_attention(c, d ** -0.5, window)
+    _check_attention(c, got, d ** -0.5, window)
+    assert torch.equal(got, _run_attention(c, d ** -0.5, window))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("nh,nkv,d,page", [(4, 2, 64, 64), (3, 1, 16, 16), (2, 2, 128, 32), (6, 3, 48, 48), (2, 1, 256, 16)])
 @pytest.mark.parametrize("window", [0, 20])

@@ -568,8 +568,8 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
             most_q = min_q - 1;
         }
         if (splits <= 0) splits = c8_splits(num_seqs, most_q < max_q ? 1 : max_q, max_k, nh, nkv, d);      // (beside a portion: as for single tokens)
-        return d == 64 ? launch_decode8<64>(p, q, out, num_seqs, max_q, splits, most_q, stream)
-                       : launch_decode8<128>(p, q, out, num_seqs, max_q, splits, most_q, stream);
+        return d == 64 ? launch_decode8<64>(p, q, out, num_seqs, max_q, max_k, splits, most_q, stream)
+                       : launch_decode8<128>(p, q, out, num_seqs, max_q, max_k, splits, most_q, stream);
     }
 #define VAPI_ATT8(T, DM) return launch_attention8<T, DM>(p, q, out, num_seqs, max_q, stream)
     if (dtype == VAPI_F32) {

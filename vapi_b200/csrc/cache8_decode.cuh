@@ -2,7 +2,7 @@
 // or 128, any page size and any number of rows.
 //
 // A decode step reads every key and value of every live request once, so the kernel is built around that stream.  A cluster of
-// up to 16 blocks owns one (sequence, kv head, tile of 8 or 16 rows) and its eight warps each a run of chunks: the 16
+// up to 16 blocks owns one (sequence, kv head, tile of 8 or 16 rows) and its eight (or four) warps each a run of chunks: the 16
 // tokens that share a scale, one piece of memory of 16 * head size bytes for K and one for V.  A warp brings its own chunks,
 // two at a time, in by bulk copies through a ring of its own, and no warp waits for another before the end, where their partial
 // results are joined: through shared memory in a block, through the cluster's among its blocks, always in the same order.
@@ -28,13 +28,13 @@
 
 namespace vapi {
 
-constexpr int D8_WARPS = 8;
+constexpr int D8_WARPS = 8, D8_FEW_WARPS = 4;                                           // of a block; of one where blocks are many and keys few
 constexpr int D8_MAX_CLUSTER = 16;
 constexpr int D8_STAGES = 3;                                                           // of two chunks of K and of V
 constexpr float D8_RAISE = 8.f;                                                        // log2 units by which a score must pass a maximum to raise it
 template <int HD> constexpr int D8_CHUNK = C8_BLOCK * HD;                              // bytes of a chunk of K, or of V
 template <int HD> constexpr int D8_WARP_BYTES = D8_STAGES * 4 * D8_CHUNK<HD>;
-template <int HD> constexpr size_t D8_SMEM = (size_t)D8_WARPS * D8_WARP_BYTES<HD>;
+template <int HD, int WARPS> constexpr size_t D8_SMEM = (size_t)WARPS * D8_WARP_BYTES<HD>;
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -73,14 +73,14 @@ __device__ __forceinline__ uint2 d8_lds8(unsigned addr) {
 template <int V> struct Number { static constexpr int value = V; };
 
 // WIDE: tiles of 16 rows, else of 8.
-template <int HD, bool WIDE>
-__global__ void __launch_bounds__(D8_WARPS * 32, (HD == 64 ? 16 : 8) / D8_WARPS)
+template <int HD, bool WIDE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (HD == 64 ? 16 : 8) / WARPS)
 decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const int splits, const int most_q) {
     constexpr int ROWS = WIDE ? 16 : 8, H = WIDE ? 2 : 1, CHUNK = D8_CHUNK<HD>;
     constexpr int KS = HD / 16, Q64 = HD / 64, VW = HD / 32;                // k-steps of S; runs of 64 elements; words of a token's values that a lane holds
     extern __shared__ __align__(128) unsigned char d8_smem[];
-    __shared__ __align__(8) unsigned long long bars[D8_WARPS * D8_STAGES];
-    __shared__ float sM[D8_WARPS][ROWS], sR[D8_WARPS][ROWS], sL[D8_WARPS][ROWS];
+    __shared__ __align__(8) unsigned long long bars[WARPS * D8_STAGES];
+    __shared__ float sM[WARPS][ROWS], sR[WARPS][ROWS], sL[WARPS][ROWS];
     __shared__ float xM[ROWS], xR[ROWS], xL[ROWS];
     __shared__ __align__(16) float xO[ROWS][HD];
     __shared__ int failed;
@@ -100,7 +100,7 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     const int key_lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
     const int c_lo = key_lo / C8_BLOCK;
     const long long chunks = p_max < key_lo ? 0 : p_max / C8_BLOCK - c_lo + 1;
-    const int units = splits * D8_WARPS, unit = rank * D8_WARPS + warp;
+    const int units = splits * WARPS, unit = rank * WARPS + warp;
     const int begin = c_lo + (int)(chunks * unit / units), end = c_lo + (int)(chunks * (unit + 1) / units), nt = end - begin, pairs = (nt + 1) / 2;
 
     const unsigned bar = smem_u32(bars + warp * D8_STAGES), ring = smem_u32(d8_smem + (size_t)warp * D8_WARP_BYTES<HD>);
@@ -382,15 +382,15 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         *reinterpret_cast<uint2*>(out + ((size_t)(q0 + tok) * p.nh + head) * HD + c) =
             make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
     };
-    for (int i = threadIdx.x; i < ROWS * HD / 4; i += D8_WARPS * 32) {
+    for (int i = threadIdx.x; i < ROWS * HD / 4; i += WARPS * 32) {
         const int r = i / (HD / 4), c = i % (HD / 4) * 4;
         float mx = -INFINITY, rx = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < D8_WARPS; ++w) { mx = fmaxf(mx, sM[w][r]); rx = fmaxf(rx, sR[w][r]); }
+        for (int w = 0; w < WARPS; ++w) { mx = fmaxf(mx, sM[w][r]); rx = fmaxf(rx, sR[w][r]); }
         const float mu = mx == -INFINITY ? 0.f : mx, ru = rx == -INFINITY ? 0.f : rx;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < D8_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float a = d8_ex2(sR[w][r] - ru);
             const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(d8_smem + (size_t)w * D8_WARP_BYTES<HD>) + r * HD + c);
             sum = fmaf(sL[w][r], d8_ex2(sM[w][r] - mu), sum);
@@ -407,7 +407,7 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         cluster_sync();                                                     // every block's result is in place
         // (each block pieces that follow one another: neighbours' reads of another block's memory are then one)
         const int mine = (ROWS * HD / 4 + splits - 1) / splits;
-        for (int i = rank * mine + threadIdx.x; i < min((rank + 1) * mine, ROWS * HD / 4); i += D8_WARPS * 32) {
+        for (int i = rank * mine + threadIdx.x; i < min((rank + 1) * mine, ROWS * HD / 4); i += WARPS * 32) {
             const int r = i / (HD / 4), c = i % (HD / 4) * 4;
             float mx = -INFINITY, rx = -INFINITY, sum = 0.f;
             for (int j = 0; j < splits; ++j) {
@@ -430,15 +430,15 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
 }
 
 // The limits that a device has to allow, asked once per device: shared memory, clusters of more than 8 blocks.
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, int WARPS>
 static int decode8_ready() {
     static int done[64] = {0};                     // 0 unknown, 1 yes
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "paged_attention8: cannot tell the current device");
     if (!done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(decode8_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D8_SMEM<HD>);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode8_kernel<HD, WIDE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", D8_SMEM<HD>, cudaGetErrorString(e));
+        cudaError_t e = cudaFuncSetAttribute(decode8_kernel<HD, WIDE, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D8_SMEM<HD, WARPS>);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode8_kernel<HD, WIDE, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", D8_SMEM<HD, WARPS>, cudaGetErrorString(e));
         done[dev] = 1;
     }
     return 0;
@@ -447,8 +447,8 @@ static int decode8_ready() {
 template <int HD>
 static int decode8_slots() {
     static int per_sm = 0;                         // (the same on every device that the kernel is built for)
-    if (per_sm == 0 && (decode8_ready<HD, false>() != 0 ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode8_kernel<HD, false>, D8_WARPS * 32, D8_SMEM<HD>) != cudaSuccess || per_sm <= 0)) {
+    if (per_sm == 0 && (decode8_ready<HD, false, D8_WARPS>() != 0 ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode8_kernel<HD, false, D8_WARPS>, D8_WARPS * 32, D8_SMEM<HD, D8_WARPS>) != cudaSuccess || per_sm <= 0)) {
         cudaGetLastError();
         per_sm = 0;
         return 2 * sm_count();
@@ -456,17 +456,17 @@ static int decode8_slots() {
     return sm_count() * per_sm;
 }
 
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, int WARPS>
 static int launch_decode8_of(const C8Params& p, const void* q, void* out, int num_seqs, long long rows, int splits, int most_q, cudaStream_t stream) {
-    const int rc = decode8_ready<HD, WIDE>();
+    const int rc = decode8_ready<HD, WIDE, WARPS>();
     if (rc != 0) return rc;
     const long long tiles = (rows + (WIDE ? 15 : 7)) / (WIDE ? 16 : 8);
     if (tiles * splits > 0x7fffffffLL || p.nkv > 65535 || num_seqs > 65535)
         return fail(-1, "paged_attention8: the step exceeds the grid (%lld row tiles, %d kv heads, %d sequences)", tiles, p.nkv, num_seqs);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits), p.nkv, num_seqs);
-    cfg.blockDim = dim3(D8_WARPS * 32);
-    cfg.dynamicSmemBytes = D8_SMEM<HD>;
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = D8_SMEM<HD, WARPS>;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -476,17 +476,25 @@ static int launch_decode8_of(const C8Params& p, const void* q, void* out, int nu
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return check_launch("paged_attention8", cudaLaunchKernelEx(&cfg, decode8_kernel<HD, WIDE>, p, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, splits, most_q));
+    return check_launch("paged_attention8", cudaLaunchKernelEx(&cfg, decode8_kernel<HD, WIDE, WARPS>, p, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, splits, most_q));
 }
 
 // sequences that bring more than `most_q` tokens are left alone
 template <int HD>
-static int launch_decode8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int splits, int most_q, cudaStream_t stream) {
+static int launch_decode8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int max_k, int splits, int most_q, cudaStream_t stream) {
     if (splits < 1) splits = 1;
     if (splits > D8_MAX_CLUSTER) return fail(-1, "paged_attention8: %d splits are more than %d", splits, D8_MAX_CLUSTER);
     const long long rows = (long long)(max_q < most_q ? max_q : most_q) * (p.nh / p.nkv);
-    if (rows <= 8) return launch_decode8_of<HD, false>(p, q, out, num_seqs, rows, splits, most_q, stream);
-    return launch_decode8_of<HD, true>(p, q, out, num_seqs, rows, splits, most_q, stream);
+    // Blocks of four warps where not all of eight would be on the device at once and a sequence's keys (or the window's) are few: a block's time is then
+    // mostly its start, its first copies' way and its join, and twice as many are under way.  us with eight and with four, 32 / 8 heads of 64: 64 requests of
+    // 64 keys 7.9 / 4.4, 300 10.2 / 6.7, 60 to 500 10.3 / 7.9, 125 to 1,000 13.7 / 12.5; 40 of 1,000 14.4 / 14.0; but 64 of 128 to 2,048 19.8 / 22.0, whose longest
+    // are then alone for longer, and 64 of 60 to 500 with half the heads, all at once, 5.4 / 6.8.
+    const long long blocks = (rows + (rows <= 8 ? 7 : 15)) / (rows <= 8 ? 8 : 16) * p.nkv * num_seqs;
+    const bool few = splits == 1 && blocks > decode8_slots<HD>() && (max_k <= 1024 || (p.window > 0 && p.window <= 1024));
+    if (rows <= 8) return few ? launch_decode8_of<HD, false, D8_FEW_WARPS>(p, q, out, num_seqs, rows, splits, most_q, stream)
+                              : launch_decode8_of<HD, false, D8_WARPS>(p, q, out, num_seqs, rows, splits, most_q, stream);
+    return few ? launch_decode8_of<HD, true, D8_FEW_WARPS>(p, q, out, num_seqs, rows, splits, most_q, stream)
+               : launch_decode8_of<HD, true, D8_WARPS>(p, q, out, num_seqs, rows, splits, most_q, stream);
 }
 
 }  // namespace vapi
