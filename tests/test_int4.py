@@ -116,6 +116,26 @@ SIZES = [(16, 32, 32), (1, 64, 64), (48, 128, 128), (33, 96, 32), (200, 512, 64)
 
 @gpu
 @pytest.mark.parametrize("n,k,group", SIZES)
+def test_packing_on_the_device_is_the_hosts(n, k, group):
+    ops = _ops()
+    codes, scales, zeros = _random(n, k, group, 3)
+    for z in (zeros, None):
+        a, b = ops.int4_pack(codes, scales, z), ops.int4_pack(codes.cuda(), scales.cuda(), None if z is None else z.cuda())
+        assert torch.equal(a.codes, b.codes.cpu()) and torch.equal(a.scales, b.scales.cpu())
+    wide = torch.zeros(n, k + 3, dtype=torch.uint8)
+    wide[:, 3:] = codes
+    b = ops.int4_pack(wide.cuda()[:, 3:], scales.cuda(), zeros.cuda())
+    assert torch.equal(ops.int4_pack(codes, scales, zeros).codes, b.codes.cpu())
+    for which in (0, 1):
+        bad = [codes.clone(), zeros.clone()]
+        bad[which][-1, -1] = 16
+        with pytest.raises(ops.KernelError, match="0..15"):
+            ops.int4_pack(bad[0].cuda(), scales.cuda(), bad[1].cuda())
+
+
+
+@gpu
+@pytest.mark.parametrize("n,k,group", SIZES)
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 24, 25, 32, 33, 64])
 def test_few_rows(n, k, group, rows):
     ops = _ops()

@@ -366,4 +366,61 @@ VAPI_EXPORT int vapi_int4_numbers(const void* codes, const void* scales, int n, 
     return check_launch("int4_dequantize", e);
 }
 
+// ---- a weight laid out -----------------------------------------------------------------------------
+// What int4_pack makes of row-major codes, scales and zeros (null: 8 everywhere): a lane a tile's 16 bytes, then a thread a word of scales.  A code or a
+// zero above 15 is left in `bad`.
+__global__ void int4_pack_kernel(const unsigned char* __restrict__ codes, const unsigned short* __restrict__ scales, const unsigned char* __restrict__ zeros,
+                                 int n, int k, int group, int chunks, unsigned* __restrict__ words, unsigned* __restrict__ pairs, long long pieces,
+                                 long long all, int* __restrict__ bad) {
+    pdl_trigger();
+    pdl_wait();
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= all) return;
+    bool over = false;
+    if (i < pieces) {
+        const int lane = (int)(i & 31), g = lane >> 2, c = lane & 3, tile = (int)(i / 32 / chunks), ch = (int)(i / 32 % chunks);
+        unsigned w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int row = tile * 16 + 8 * h + g, col = ch * 64 + 32 * a + 8 * c;
+                if (row >= n || col >= k) continue;
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)row * k + col));
+                over |= ((x.x | x.y) & 0xf0f0f0f0u) != 0u;
+                // columns 4b + 2p + e: byte 2p + e of word b, to bits from 8p + 4h + 16e on
+                const unsigned in[2] = {x.x & 0x0f0f0f0fu, x.y & 0x0f0f0f0fu};
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    w[2 * a + b] |= ((in[b] & 15u) | (in[b] >> 8 & 15u) << 16 | (in[b] >> 16 & 15u) << 8 | (in[b] >> 24) << 24) << (4 * h);
+            }
+        reinterpret_cast<uint4*>(words)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        const long long j = i - pieces;            // [tile][group][g][h]
+        const int groups = k / group, wide = group == 32 ? 2 * chunks : groups;
+        const int h = (int)(j & 1), g = (int)(j >> 1 & 7), at = (int)((j >> 4) % wide), tile = (int)((j >> 4) / wide), row = tile * 16 + 8 * h + g;
+        unsigned pair = 0u;
+        if (row < n && at < groups) {
+            const unsigned z = zeros ? zeros[(size_t)row * groups + at] : 8u;
+            over = z > 15u;
+            pair = scales[(size_t)row * groups + at] | (0x4300u + (z & 15u)) << 16;      // (128 + zero as bfloat16)
+        }
+        pairs[j] = pair;
+    }
+    if (over) atomicExch(bad, 1);
+}
+
+// words [tiles][chunks][32][4] and pairs [tiles][groups, or 2 chunks of them][8][2] as int4_pack says; bad: set to 1 or left
+VAPI_EXPORT int vapi_int4_pack(const void* codes, const void* scales, const void* zeros, int n, int k, int group, void* words, void* pairs, int* bad,
+                               cudaStream_t stream) {
+    if (n <= 0 || k <= 0) return fail(-1, "int4_pack: a weight of %d x %d", n, k);
+    if ((group != 32 && group != 64 && group != 128) || k % group != 0) return fail(-1, "int4_pack: groups of %d of %d columns", group, k);
+    if (((uintptr_t)codes & 7) != 0 || ((uintptr_t)words & 15) != 0) return fail(-1, "int4_pack: the codes are not 8-byte aligned, or the words not 16-byte");
+    const int chunks = (k + 63) / 64, tiles = (n + 15) / 16;
+    const long long pieces = (long long)tiles * chunks * 32, all = pieces + (long long)tiles * (group == 32 ? 2 * chunks : k / group) * 16, blocks = (all + 255) / 256;
+    if (blocks > 0x7fffffffLL) return fail(-1, "int4_pack: %d x %d exceeds the grid", n, k);
+    return check_launch("int4_pack", launch(int4_pack_kernel, (unsigned)blocks, 256, 0, stream, (const unsigned char*)codes, (const unsigned short*)scales,
+                                            (const unsigned char*)zeros, n, k, group, chunks, (unsigned*)words, (unsigned*)pairs, pieces, all, bad));
+}
+
 VAPI_EXPORT const char* vapi_last_error() { return error_buffer(); }

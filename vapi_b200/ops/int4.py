@@ -60,12 +60,14 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.T
     group = k // groups
     if group not in INT4_GROUPS:
         raise KernelError(f"groups of {group} columns are not one of {', '.join(map(str, INT4_GROUPS))}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise KernelError(f"the zeros must be {tuple(scales.shape)} of uint8, got {tuple(zeros.shape)} of {zeros.dtype}")
+    if codes.device != scales.device or (zeros is not None and codes.device != zeros.device):
+        raise KernelError("codes, scales and zeros must be on one device")
+    if codes.is_cuda:
+        return _pack(codes, scales, zeros, group)
     if zeros is None:
         zeros = torch.full_like(scales, 8, dtype=torch.uint8)
-    if zeros.dtype != torch.uint8 or zeros.shape != scales.shape:
-        raise KernelError(f"the zeros must be {tuple(scales.shape)} of uint8, got {tuple(zeros.shape)} of {zeros.dtype}")
-    if codes.device != scales.device or codes.device != zeros.device:
-        raise KernelError("codes, scales and zeros must be on one device")
     if int(codes.max()) > 15 or int(zeros.max()) > 15:
         raise KernelError("codes and zeros must be in 0..15")
     tiles, chunks = -(-n // 16), -(-k // 64)
@@ -87,6 +89,25 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.T
     pairs = bits(scales) | bits(zeros.to(torch.float32) + 128.0) << 16
     wide = 2 * chunks if group == 32 else groups                   # (whole tiles of 64 columns)
     pairs = torch.nn.functional.pad(pairs, (0, wide - groups, 0, tiles * 16 - n)).view(tiles, 2, 8, wide).permute(0, 3, 2, 1).contiguous()
+    return Int4Weight(words, pairs, n, k, group)
+
+
+def _pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int) -> Int4Weight:
+    """The same on the device, by one kernel."""
+    n, k = codes.shape
+    _here(codes)
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 8:
+        codes = codes.clone()
+    zeros = None if zeros is None else zeros.contiguous()
+    tiles, chunks = -(-n // 16), -(-k // 64)
+    words = torch.empty((tiles, chunks, 32, 4), dtype=torch.int32, device=codes.device)
+    pairs = torch.empty((tiles, 2 * chunks if group == 32 else k // group, 8, 2), dtype=torch.int32, device=codes.device)
+    bad = torch.zeros(1, dtype=torch.int32, device=codes.device)
+    lib = _lib("int4")
+    _check(lib, lib.vapi_int4_pack(_p(codes), _p(scales), _p(zeros), n, k, group, _p(words), _p(pairs), _p(bad), _stream()))
+    if int(bad):
+        raise KernelError("codes and zeros must be in 0..15")
     return Int4Weight(words, pairs, n, k, group)
 
 
