@@ -130,12 +130,12 @@ def unpack(w):
     """(codes, scales, zeros) of an Int4Weight, read from its words bit by bit (host)."""
     words, pairs = w.codes.cpu(), w.scales.cpu()
     tiles, chunks = words.shape[:2]
-    codes = torch.zeros(tiles, 2, 8, chunks, 2, 4, 2, 2, 2, dtype=torch.uint8)
-    lanes = words.view(tiles, chunks, 8, 4, 2, 2)
+    codes = torch.zeros(tiles, 2, 8, chunks, 4, 2, 4, 2, dtype=torch.uint8)
+    lanes = words.view(tiles, chunks, 8, 4, 4)
     for h in range(2):
         for p in range(2):
             for e in range(2):
-                codes[:, h, :, :, :, :, :, p, e] = ((lanes >> (8 * p + 4 * h + 16 * e)) & 15).permute(0, 2, 1, 4, 3, 5).to(torch.uint8)
+                codes[:, h, :, :, :, p, :, e] = ((lanes >> (8 * p + 4 * h + 16 * e)) & 15).permute(0, 2, 1, 4, 3).to(torch.uint8)
     table = pairs.permute(0, 3, 2, 1).reshape(tiles * 16, -1)[:w.n, :w.k // w.group]
     number = lambda t: (t & 0xffff).to(torch.int16).view(torch.bfloat16)
     return codes.reshape(tiles * 16, chunks * 64)[:w.n, :w.k], number(table), number(table >> 16) - 128

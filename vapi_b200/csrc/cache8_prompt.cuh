@@ -103,7 +103,6 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     // (by a shuffle: what depends on the warp alone is then known to be the same for all its lanes)
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int splits = JOIN ? blocks : 1, rank = JOIN ? (int)blockIdx.x % splits : 0, unit = (int)blockIdx.x / splits, g = unit % p.nkv, n_rep = p.nh / p.nkv;
-    pdl_trigger();
     // index data was copied from the host before the step's first kernel: safe before the wait
     int s = 0, tile = 0;
     if (!ft_tile(p.cu_q, num_seqs, min_q, n_rep, P8_ROWS, unit / p.nkv, s, tile)) {        // (the same for the whole cluster)
@@ -143,6 +142,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
+    pdl_trigger();                                  // (not before the allocation: a block of the next kernel that came between would be waited for, and wait)
     const unsigned tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);          // half h: S at 128 h (and 64 further on), O at 256 + HD h
 
     if (warp == P8_THREADS / 32 - 1) {

@@ -2,12 +2,11 @@
 // each group of 32, 64 or 128 columns of a row.
 //
 // How a weight is laid out (int4_pack in ops/int4.py): tiles of 16 rows x 64 columns, 512 bytes each, a row of tiles in one piece.
-// Within a tile lane l of a warp has 16 bytes: rows l/4 and l/4 + 8, columns 8 (l & 3) .. + 7 and 32 + 8 (l & 3) .. + 7, a word four of
-// those, that is the A operands of one mma.sync m16n8k16.  A pair of codes stands 16 bits apart, so that one logical operation
-// makes two bfloat16 of it: 0x4300 | code is 128 + code.  Taking 128 + zero off is exact, and so is the product of what is left
-// (-15 .. 15) with a bfloat16; a group's sum is a float and is multiplied by the scale in float.  Nothing is rounded but the
-// float sums and the result.  The order of 32 columns (the smallest group) is free as long as x follows it: a lane's 8 columns of
-// x are 16 bytes in one piece, its B operands of two k-steps.
+// Within a tile lane l of a warp has 16 bytes, a word for each 16 columns: of rows l/4 and l/4 + 8 columns 2 (l & 3), + 1, + 8 and + 9, that is
+// the A operands of one mma.sync m16n8k16 (and a store's to tensor memory, int4_tile.cuh).  A pair of codes stands 16 bits apart, so
+// that one logical operation makes two bfloat16 of it: 0x4300 | code is 128 + code.  Taking 128 + zero off is exact, and so is the product
+// of what is left (-15 .. 15) with a bfloat16; a group's sum is a float and is multiplied by the scale in float.  Nothing is rounded but the
+// float sums and the result.
 //
 // Scales: for each tile row and group (of 32: two for every 64 columns, the last perhaps of nothing) 8 pairs of words, word = scale | (128 + zero) << 16 as two bfloat16, rows l/4 and l/4 + 8.
 #include "cluster.cuh"
@@ -46,6 +45,13 @@ __device__ __forceinline__ __nv_bfloat162 i4_zero(unsigned w) {
 }
 __device__ __forceinline__ float i4_scale(unsigned w) { return __uint_as_float(w << 16); }
 
+// four 8 x 8 pieces of 16-bit numbers, a row's address a lane: the B operands of two k-steps
+__device__ __forceinline__ uint4 i4_pieces(unsigned addr) {
+    uint4 v;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+
 #include "int4_tile.cuh"
 
 // ---- few rows -------------------------------------------------------------------------------------
@@ -64,10 +70,10 @@ template <int NT, int GS, bool GLU>                // GS: k-steps of 16 columns 
 __global__ void __launch_bounds__(I4_WARPS * 32, 2)
 int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg) {
     constexpr int AHEAD = I4_AHEAD<NT>, CPG = GS > 4 ? GS / 4 : 1, GPC = GS < 4 ? 4 / GS : 1;      // tiles a group; groups a tile
-    extern __shared__ __align__(16) unsigned char i4_smem[];
+    extern __shared__ __align__(128) unsigned char i4_smem[];
     float (*part)[8 * NT + 1] = reinterpret_cast<float (*)[8 * NT + 1]>(i4_smem);
-    __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(i4_smem + ((I4_PART * (8 * NT + 1) * 4 + 15) & ~15));
-    constexpr int PITCH = I4_SEG<NT> * 64 + 32;    // (64 bytes more than whole tiles: two rows of a quarter of a warp are in unlike banks)
+    __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(i4_smem + ((I4_PART * (8 * NT + 1) * 4 + 127) & ~127));
+    constexpr int PITCH = I4_SEG<NT> * 64;         // (a row's pieces of 16 bytes are turned by the row, so that eight rows' are in unlike banks)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rank = (int)blockIdx.x % splits, block = (int)blockIdx.x / splits, r0 = blockIdx.y * 8 * NT;
     const int tiles = (p.n + 15) / 16, groups = GS < 4 ? p.chunks * GPC : p.k / p.group;
@@ -120,14 +126,15 @@ int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg
                 const __nv_bfloat16* src = p.x + (ok ? (size_t)(r0 + row) * p.k : 0) + s0 * 64;
                 for (int i = lane * 8; i < tiles_here * 64; i += 256) {
                     const bool in = ok && s0 * 64 + i < p.k;
-                    cp_async_16(sx + row * PITCH + i, in ? src + i : p.x, in ? 16 : 0);
+                    cp_async_16(sx + row * PITCH + (i ^ (row & 7) << 3), in ? src + i : p.x, in ? 16 : 0);
                 }
             }
             cp_async_commit();
             cp_async_wait<0>();
         }
         __syncthreads();
-        const __nv_bfloat16* xr = sx + g * PITCH + c * 8 + (begin - s0) * 64;
+        // a lane's address in four 8 x 8 pieces of x: eight rows, 32 columns
+        unsigned xr = (unsigned)__cvta_generic_to_shared(sx + (lane & 7) * PITCH + (begin - s0) * 64) + (((lane >> 3) ^ (lane & 7)) << 4);
         for (int base = begin; base < end; base += AHEAD) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
@@ -136,10 +143,10 @@ int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg
                 uint4 xa[NT], xb[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    xa[n] = *reinterpret_cast<const uint4*>(xr + n * 8 * PITCH);
-                    xb[n] = *reinterpret_cast<const uint4*>(xr + n * 8 * PITCH + 32);
+                    xa[n] = i4_pieces(xr + n * 8 * PITCH * 2);
+                    xb[n] = i4_pieces((xr ^ 64) + n * 8 * PITCH * 2);
                 }
-                xr += 64;
+                xr += 128;
                 const unsigned words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
                 for (int q = 0; q < GPC; ++q) {
@@ -246,7 +253,7 @@ static int launch_int4_rows(const I4Params& p, cudaStream_t stream) {
     int wn, splits;
     int4_shape(tiles, p.chunks, NT, GLU, wn, splits);
     const int each = (p.chunks + splits - 1) / splits + 1, seg = (each < I4_SEG<NT> ? each + (each & 1) : I4_SEG<NT>);
-    constexpr size_t smem = ((I4_PART * (8 * NT + 1) * 4 + 15) & ~15) + (size_t)8 * NT * (I4_SEG<NT> * 64 + 32) * 2;
+    constexpr size_t smem = ((I4_PART * (8 * NT + 1) * 4 + 127) & ~127) + (size_t)8 * NT * I4_SEG<NT> * 64 * 2;
     static int ready[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "int4_linear: cannot tell the current device");
@@ -303,7 +310,7 @@ VAPI_EXPORT int vapi_int4_linear(const void* codes, const void* scales, int n, i
 }
 
 // ---- the weight as numbers --------------------------------------------------------------------------
-// A thread's 16 bytes are twice 8 columns of two rows.
+// A thread takes one word of each of four lanes: 16 columns of two rows.
 template <typename T>
 __global__ void int4_numbers_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales, int n, int k, int group, int chunks,
                                     T* __restrict__ out, long long pieces) {
@@ -313,30 +320,29 @@ __global__ void int4_numbers_kernel(const unsigned* __restrict__ codes, const un
         pdl_wait();
         return;
     }
-    const int lane = (int)(i & 31), g = lane >> 2, c = lane & 3;
-    const int tile = (int)(i / 32 / chunks), ch = (int)(i / 32 % chunks);
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(codes) + i);
-    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+    const int lane = (int)(i & 31), g = lane >> 2, j = lane & 3;
+    const int tile = (int)(i / 32 / chunks), col = (int)(i / 32 % chunks) * 64 + 16 * j;
+    unsigned words[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) words[c] = __ldg(codes + (i - j + c) * 4 + j);
     const int groups = group == 32 ? 2 * chunks : k / group;
     pdl_wait();                                    // (the weight is nobody's output, but `out` may still be read)
+    if (col >= k) return;
+    const uint2 sc = __ldg(reinterpret_cast<const uint2*>(scales) + ((size_t)tile * groups + col / group) * 8 + g);
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-        const int col = ch * 64 + 32 * a + 8 * c;
-        if (col >= k) break;
-        const uint2 sc = __ldg(reinterpret_cast<const uint2*>(scales) + ((size_t)tile * groups + col / group) * 8 + g);
+    for (int h = 0; h < 2; ++h) {
+        const int row = tile * 16 + g + 8 * h;
+        if (row >= n) continue;
+        const unsigned s = h ? sc.y : sc.x;
+        const float f = i4_scale(s), z = __uint_as_float(s & 0xffff0000u) - 128.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = tile * 16 + g + 8 * h;
-            if (row >= n) continue;
-            const unsigned s = h ? sc.y : sc.x;
-            const float f = i4_scale(s), z = __uint_as_float(s & 0xffff0000u) - 128.f;
-            T* dst = out + (size_t)row * k + col;
+        for (int p = 0; p < 2; ++p) {
+            T* dst = out + (size_t)row * k + col + 8 * p;
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)        // columns 4j + 2p + e: bits from 8p + 4h + 16e on of word 2a + j
-                    v[4 * j + e] = ((float)(words[2 * a + j] >> (8 * (e >> 1) + 4 * h + 16 * (e & 1)) & 15u) - z) * f;
+                for (int e = 0; e < 2; ++e) v[2 * c + e] = ((float)(words[c] >> (8 * p + 4 * h + 16 * e) & 15u) - z) * f;
             if (sizeof(T) == 4) {
                 reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
                 reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -383,17 +389,15 @@ __global__ void int4_pack_kernel(const unsigned char* __restrict__ codes, const 
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int row = tile * 16 + 8 * h + g, col = ch * 64 + 32 * a + 8 * c;
-                if (row >= n || col >= k) continue;
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)row * k + col));
-                over |= ((x.x | x.y) & 0xf0f0f0f0u) != 0u;
-                // columns 4b + 2p + e: byte 2p + e of word b, to bits from 8p + 4h + 16e on
-                const unsigned in[2] = {x.x & 0x0f0f0f0fu, x.y & 0x0f0f0f0fu};
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    w[2 * a + b] |= ((in[b] & 15u) | (in[b] >> 8 & 15u) << 16 | (in[b] >> 16 & 15u) << 8 | (in[b] >> 24) << 24) << (4 * h);
-            }
+                for (int p = 0; p < 2; ++p) {
+                    const int row = tile * 16 + 8 * h + g, col = ch * 64 + 16 * j + 8 * p + 2 * c;
+                    if (row >= n || col >= k) continue;
+                    const unsigned x = __ldg(reinterpret_cast<const unsigned short*>(codes + (size_t)row * k + col));
+                    over |= (x & 0xf0f0u) != 0u;
+                    w[j] |= ((x & 15u) | (x >> 8 & 15u) << 16) << (8 * p + 4 * h);
+                }
         reinterpret_cast<uint4*>(words)[i] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
         const long long j = i - pieces;            // [tile][group][g][h]

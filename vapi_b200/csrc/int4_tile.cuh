@@ -4,10 +4,11 @@
 // A block owns 128 features (for a gated product 64 of the gate and the same 64 of up) and N rows of x; the blocks of a cluster share out the
 // columns.  A chunk is 64 columns:
 //   warps 0..7  a tile row of codes each (int4.cu says how it lies), AHEAD chunks under way in registers; what they make of it goes to a ring of
-//               shared-memory stages in the layout of a K-major operand;
-//   warp 8      x, by TMA into the same stages (rows and columns behind the end are zeros);
+//               stages in tensor memory, where a product may have its first operand: the codes' order is that of a 16-lane store.  (Through
+//               shared memory W was written there and read again, 32 of a chunk's 56 KB at 64 rows, and that was what bounded the kernel.)
+//   warp 8      x, by TMA into a ring of shared-memory stages (rows and columns behind the end are zeros);
 //   warp 9      D[feature][row] += W X^T, issued by one lane of the whole warp; owns the tensor memory.
-// Then warps 0..7 bring D to shared memory, whose stages nobody reads any more, and all threads write what comes of it, four features at a time.
+// Then warps 0..7 bring D to shared memory, where x's stages were, and all threads write what comes of it, four features at a time.
 //
 // Every wait is bounded; a role that gives up marks the block, whose results are then NaN.
 #pragma once
@@ -17,16 +18,25 @@
 namespace vapi {
 
 constexpr int I4T_LOADERS = 8, I4T_THREADS = (I4T_LOADERS + 2) * 32, I4T_FEATURES = 128, I4T_AHEAD = 6;
-template <int N> constexpr int I4T_STAGES = N == 128 ? 3 : 4;
+template <int N> constexpr int I4T_STAGES = N == 64 ? 6 : 4;
 template <int N> constexpr int I4T_BLOCKS = N > 128 ? 1 : 2;                                  // a multiprocessor
-template <int N> constexpr int I4T_STAGE = I4T_FEATURES * 128 + N * 128;                      // W | X, bytes
+template <int N> constexpr int I4T_STAGE = N * 128;                                           // bytes of x
+template <int N> constexpr int I4T_COLUMNS = N > 128 ? 512 : 256;                             // of tensor memory: D, then 32 a stage of W
 template <int N> constexpr size_t I4T_SMEM = 1024 + (size_t)I4T_STAGES<N> * I4T_STAGE<N> + 256;
+
+// D += A B^T with A in tensor memory, a row a lane and two k a column
+__device__ __forceinline__ void i4t_mma(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
 
 template <int N, int GS, bool GLU>                 // GS: k-steps of 16 columns a group (2, 4, 8)
 __global__ void __launch_bounds__(I4T_THREADS, I4T_BLOCKS<N>)
 int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, const int splits) {
-    constexpr int STAGES = I4T_STAGES<N>, STAGE = I4T_STAGE<N>, W_BYTES = I4T_FEATURES * 128, AHEAD = I4T_AHEAD, GPC = GS < 4 ? 2 : 1, CPG = GS > 4 ? 2 : 1;
+    constexpr int STAGES = I4T_STAGES<N>, STAGE = I4T_STAGE<N>, COLUMNS = I4T_COLUMNS<N>, AHEAD = I4T_AHEAD, GPC = GS < 4 ? 2 : 1, CPG = GS > 4 ? 2 : 1;
     static_assert(N * I4T_FEATURES * 4 <= STAGES * STAGE, "D fits where the stages were");
+    static_assert(N + 32 * STAGES <= COLUMNS && COLUMNS * I4T_BLOCKS<N> <= 512, "D and W fit in tensor memory");
     extern __shared__ unsigned char i4t_smem[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(i4t_smem) + 1023) & ~(uintptr_t)1023);
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(base + (size_t)STAGES * STAGE);
@@ -36,7 +46,6 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
     const int rank = (int)blockIdx.x % splits, block = (int)blockIdx.x / splits, r0 = (int)blockIdx.y * N;
     const int from = (int)((long long)p.chunks * rank / splits), upto = (int)((long long)p.chunks * (rank + 1) / splits);
     const unsigned full = smem_u32(bars), empty = smem_u32(bars + STAGES), x_full = smem_u32(bars + 2 * STAGES), done = smem_u32(bars + 3 * STAGES);
-    pdl_trigger();
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(full + 8 * i, 8); mbar_init(empty + 8 * i, 1); mbar_init(x_full + 8 * i, 1); }
         mbar_init(done, 1);
@@ -44,18 +53,21 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == I4T_LOADERS + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((unsigned)N) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((unsigned)COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
+    pdl_trigger();                                 // (not before the allocation: a block of the next kernel that came between would be waited for, and wait)
     const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     if (warp < I4T_LOADERS) {
-        const int g = lane >> 2, c = lane & 3, tiles = (p.n + 15) / 16, groups = GS < 4 ? 2 * p.chunks : p.k / p.group;
-        const int mine = GLU ? (warp < 4 ? block * 4 + warp : tiles / 2 + block * 4 + warp - 4) : block * 8 + warp;
-        const bool real = GLU ? block * 4 + (warp & 3) < tiles / 2 : mine < tiles;
+        // (a warp reaches the lanes of one quarter of tensor memory: two tile rows)
+        const int g = lane >> 2, tiles = (p.n + 15) / 16, groups = GS < 4 ? 2 * p.chunks : p.k / p.group, tn = 2 * (warp & 3) + (warp >> 2);
+        const int mine = GLU ? (tn < 4 ? block * 4 + tn : tiles / 2 + block * 4 + tn - 4) : block * 8 + tn;
+        const bool real = GLU ? block * 4 + (tn & 3) < tiles / 2 : mine < tiles;
+        const unsigned to_w = tmem + N + ((unsigned)(16 * tn) << 16);
         const uint4* codes = reinterpret_cast<const uint4*>(p.codes) + (size_t)(real ? mine : 0) * p.chunks * 32 + lane;
         const uint2* scales = reinterpret_cast<const uint2*>(p.scales) + (size_t)(real ? mine : 0) * groups * 8 + g;
         uint4 w[AHEAD];
@@ -76,30 +88,28 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
                 const int ch = at + i;
                 if (ch >= upto) break;
                 if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * stage, parity))) { ok = false; break; }
-                unsigned char* dst = base + (size_t)stage * STAGE + (16 * warp + g) * 128;
-                // (odd rows the other half first: the eight lanes of a store's quarter then meet in no bank)
+                tc5_fence_after();
+                const unsigned words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                unsigned v[16];                    // word 2j + q of a row's 8 words a lane: of row g, of row g + 8
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const bool a = (s ^ g) & 1;
-                    const unsigned words[2] = {a ? w[i].z : w[i].x, a ? w[i].w : w[i].y};
-                    const uint2 of = a ? sc[i][GPC - 1] : sc[i][0];
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        const uint2 of = sc[i][GPC == 2 ? j >> 1 : 0];
                         const unsigned pair = h ? of.y : of.x, both = __byte_perm(pair, pair, 0x1010);
                         const __nv_bfloat162 zero = i4_zero(pair), scale = *reinterpret_cast<const __nv_bfloat162*>(&both);
-                        unsigned v[4];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const unsigned u = i4_pair(words[j], 8 * e + 4 * h, zero);
-                                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&u), scale);
-                                v[2 * j + e] = *reinterpret_cast<const unsigned*>(&y);
-                            }
-                        *reinterpret_cast<uint4*>(dst + h * 8 * 128 + ((((a ? 4 : 0) + c) ^ g) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int q = 0; q < 2; ++q) {
+                            const unsigned u = i4_pair(words[j], 8 * q + 4 * h, zero);
+                            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&u), scale);
+                            v[2 * (2 * j + q) + h] = *reinterpret_cast<const unsigned*>(&y);
+                        }
                     }
-                }
-                fence_proxy_async();
+                asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                             ::"r"(to_w + 32 * stage), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                               "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+                tmem_st_wait();
+                tc5_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + 8 * stage);
                 bring(ch + AHEAD, w[i], sc[i]);
@@ -131,7 +141,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
             for (int ch = from; ch < upto; ++ch, ++asked) {
                 if (!mbar_wait(empty + 8 * stage, parity)) { *failed = 1; break; }
                 mbar_expect_tx(x_full + 8 * stage, N * 128);
-                tma_load_2d(smem_u32(base) + stage * STAGE + W_BYTES, &tm_x, x_full + 8 * stage, ch * 64, r0);
+                tma_load_2d(smem_u32(base) + stage * STAGE, &tm_x, x_full + 8 * stage, ch * 64, r0);
                 if (++stage == STAGES) { stage = 0; parity ^= 1; }
             }
             // (the block does not leave, or use the stages for something else, while a copy is under way)
@@ -149,11 +159,11 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
         for (int ch = from; ch < upto; ++ch) {
             if (!mbar_wait_warp(full + 8 * stage, parity) || !mbar_wait_warp(x_full + 8 * stage, parity)) { ok = false; break; }
             tc5_fence_after();
-            const unsigned a = low + stage * (STAGE >> 4), b = a + (W_BYTES >> 4);
+            const unsigned a = tmem + N + 32 * stage, b = low + stage * (STAGE >> 4);
             if (leader) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    umma_f16(tmem, (unsigned long long)high << 32 | (a + 2 * k), (unsigned long long)high << 32 | (b + 2 * k), idesc, (ch > from || k > 0) ? 1u : 0u);
+                    i4t_mma(tmem, a + 8 * k, (unsigned long long)high << 32 | (b + 2 * k), idesc, (ch > from || k > 0) ? 1u : 0u);
                 umma_commit(empty + 8 * stage);
             }
             __syncwarp();
@@ -168,7 +178,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
     __syncthreads();
     if (warp == I4T_LOADERS + 1) {
         tc5_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)N) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)COLUMNS) : "memory");
     }
     if (splits > 1) cluster_sync();                // every block's sums are in place
     pdl_wait();                                    // (what is written may still be read)

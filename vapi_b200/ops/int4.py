@@ -77,9 +77,9 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.T
         part = codes[at * 16:(at + step) * 16]
         m = -(-part.shape[0] // 16)
         part = torch.nn.functional.pad(part, (0, chunks * 64 - k, 0, m * 16 - part.shape[0])).to(torch.int32)
-        # row 8h + g, column 64 ch + 32a + 8c + 4b + 2p + e  ->  lane 4g + c, word 2a + b, bits from 8p + 4h + 16e on
-        part = part.view(m, 2, 8, chunks, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 1, 7, 8)
-        got = torch.zeros((m, chunks, 8, 4, 2, 2), dtype=torch.int32, device=codes.device)
+        # row 8h + g, column 64 ch + 16j + 8p + 2c + e  ->  lane 4g + c, word j, bits from 8p + 4h + 16e on
+        part = part.view(m, 2, 8, chunks, 4, 2, 4, 2).permute(0, 3, 2, 6, 4, 1, 5, 7)
+        got = torch.zeros((m, chunks, 8, 4, 4), dtype=torch.int32, device=codes.device)
         for h in range(2):
             for p in range(2):
                 for e in range(2):
