@@ -15,10 +15,10 @@
 using namespace vapi;
 
 constexpr int I4_WARPS = 8;
-// Rows of int4_rows_kernel; more go to int4_tile_kernel, which takes the time of 64 for any number up to that.  us of the one with as many rows as it can
-// hold (32) and of the other: 2,048 x 2,048, 24 rows 5.4 / 6.0, 32 rows 8.5 / 6.2; 16,384 x 2,048 gated 12.3 / 12.8 and 14.2 / 12.8; 2,048 x 8,192 9.3 / 11.5
-// and 12.0 / 11.8; 13,824 x 1,536 gated 9.4 / 10.6 and 11.6 / 10.2.
-constexpr int I4_MOST_ROWS = 24;
+// Rows of int4_rows_kernel; more go to int4_tile_kernel, which takes the time of 32 for any number up to that.  us of the one and of the other: 2,048 x
+// 2,048, 16 rows 3.5 / 5.4, 24 rows 5.3 / 5.5; 6,144 x 2,048 5.3 / 6.5 and 7.5 / 6.8; 16,384 x 2,048 gated 9.0 / 9.8 and 11.8 / 10.0; 2,048 x 8,192 7.5 / 8.4
+// and 9.8 / 8.6; 1,536 x 6,912 6.4 / 7.5 and 8.7 / 7.7.
+constexpr int I4_MOST_ROWS = 16;
 constexpr int I4_TILE_WORDS = 128;                 // 16 x 64 codes
 
 struct I4Params {
@@ -63,17 +63,16 @@ __device__ __forceinline__ uint4 i4_pieces(unsigned addr) {
 // would be most of the traffic.  Partial results are added in the order of slices, then of blocks.
 constexpr int I4_PART = 8 * 16;                    // rows of partial results: eight warps x 16 features
 
-template <int NT> constexpr int I4_SEG = NT >= 3 ? 24 : 32;              // tiles of columns of x that shared memory holds at most
-template <int NT> constexpr int I4_AHEAD = NT >= 3 ? 4 : 6;
+constexpr int I4_SEG = 32, I4_AHEAD = 6;           // tiles of columns of x that shared memory holds at most; tiles of weights under way
 
 template <int NT, int GS, bool GLU>                // GS: k-steps of 16 columns a group (2, 4, 8)
 __global__ void __launch_bounds__(I4_WARPS * 32, 2)
 int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg) {
-    constexpr int AHEAD = I4_AHEAD<NT>, CPG = GS > 4 ? GS / 4 : 1, GPC = GS < 4 ? 4 / GS : 1;      // tiles a group; groups a tile
+    constexpr int AHEAD = I4_AHEAD, CPG = GS > 4 ? GS / 4 : 1, GPC = GS < 4 ? 4 / GS : 1;      // tiles a group; groups a tile
     extern __shared__ __align__(128) unsigned char i4_smem[];
     float (*part)[8 * NT + 1] = reinterpret_cast<float (*)[8 * NT + 1]>(i4_smem);
     __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(i4_smem + ((I4_PART * (8 * NT + 1) * 4 + 127) & ~127));
-    constexpr int PITCH = I4_SEG<NT> * 64;         // (a row's pieces of 16 bytes are turned by the row, so that eight rows' are in unlike banks)
+    constexpr int PITCH = I4_SEG * 64;         // (a row's pieces of 16 bytes are turned by the row, so that eight rows' are in unlike banks)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rank = (int)blockIdx.x % splits, block = (int)blockIdx.x / splits, r0 = blockIdx.y * 8 * NT;
     const int tiles = (p.n + 15) / 16, groups = GS < 4 ? p.chunks * GPC : p.k / p.group;
@@ -234,12 +233,12 @@ int4_rows_kernel(const I4Params p, const int splits, const int wn, const int seg
     if (splits > 1) cluster_sync();                // nobody reads this block's memory any more
 }
 
-// How the work falls to blocks: as many tile rows a block (1, 2, 4 or 8) as leave about two blocks a multiprocessor, and where K is long at least NT,
-// so that x is not read more often than the weights (of a short K, blocks are worth more: 16 rows, one tile row a block or two, 2,048 x 2,048 3.8 / 4.5
-// us, 2,048 x 8,192 8.5 / 7.4; 19 rows, two or four, 2,048 x 2,048 5.4 / 6.8, 2,048 x 8,192 9.2 / 9.3, 8,192 x 28,672 84 / 68); then, while there are fewer
-// blocks, a cluster of up to 8 shares the columns as long as each warp still has four tiles.
+// How the work falls to blocks: as many tile rows a block (1, 2, 4 or 8) as leave about two blocks a multiprocessor, and for more than 8 rows two where
+// K is long, so that x is not read more often than the weights (of a short K, blocks are worth more: 16 rows, one tile row a block or two, 2,048 x
+// 2,048 3.8 / 4.5 us, 2,048 x 8,192 8.5 / 7.4); then, while there are fewer blocks, a cluster of up to 8 shares the columns as long as each
+// warp still has four tiles.
 static void int4_shape(int tiles, int chunks, int nt, bool glu, int& wn, int& splits) {
-    const int least = nt == 1 ? 1 : nt == 2 ? (chunks > 48 ? 2 : 1) : (chunks > 128 ? 4 : 2);
+    const int least = nt > 1 && chunks > 48 ? 2 : 1;
     wn = glu ? 2 : 1;
     while (wn < 8 && (wn < least || (tiles + wn - 1) / wn > 2 * sm_count())) wn *= 2;
     const long long blocks = (tiles + wn - 1) / wn;
@@ -252,8 +251,8 @@ static int launch_int4_rows(const I4Params& p, cudaStream_t stream) {
     const int tiles = (p.n + 15) / 16;
     int wn, splits;
     int4_shape(tiles, p.chunks, NT, GLU, wn, splits);
-    const int each = (p.chunks + splits - 1) / splits + 1, seg = (each < I4_SEG<NT> ? each + (each & 1) : I4_SEG<NT>);
-    constexpr size_t smem = ((I4_PART * (8 * NT + 1) * 4 + 127) & ~127) + (size_t)8 * NT * I4_SEG<NT> * 64 * 2;
+    const int each = (p.chunks + splits - 1) / splits + 1, seg = (each < I4_SEG ? each + (each & 1) : I4_SEG);
+    constexpr size_t smem = ((I4_PART * (8 * NT + 1) * 4 + 127) & ~127) + (size_t)8 * NT * I4_SEG * 64 * 2;
     static int ready[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "int4_linear: cannot tell the current device");
@@ -281,8 +280,7 @@ static int launch_int4_rows(const I4Params& p, cudaStream_t stream) {
 template <int GS>
 static int int4_rows(const I4Params& p, bool glu, cudaStream_t stream) {
     if (p.rows <= 8) return glu ? launch_int4_rows<1, GS, true>(p, stream) : launch_int4_rows<1, GS, false>(p, stream);
-    if (p.rows <= 16) return glu ? launch_int4_rows<2, GS, true>(p, stream) : launch_int4_rows<2, GS, false>(p, stream);
-    return glu ? launch_int4_rows<3, GS, true>(p, stream) : launch_int4_rows<3, GS, false>(p, stream);
+    return glu ? launch_int4_rows<2, GS, true>(p, stream) : launch_int4_rows<2, GS, false>(p, stream);
 }
 
 // x [rows][k] bfloat16 with 16-byte aligned rows.  gated: W is [gate; up], y [rows][n / 2] = act(gate) * up, n / 2 a multiple of 16.

@@ -18,7 +18,7 @@
 namespace vapi {
 
 constexpr int I4T_LOADERS = 8, I4T_THREADS = (I4T_LOADERS + 2) * 32, I4T_FEATURES = 128, I4T_AHEAD = 6;
-template <int N> constexpr int I4T_STAGES = N == 64 ? 6 : 4;
+template <int N> constexpr int I4T_STAGES = N <= 64 ? 6 : 4;
 template <int N> constexpr int I4T_BLOCKS = N > 128 ? 1 : 2;                                  // a multiprocessor
 template <int N> constexpr int I4T_STAGE = N * 128;                                           // bytes of x
 template <int N> constexpr int I4T_COLUMNS = N > 128 ? 512 : 256;                             // of tensor memory: D, then 32 a stage of W
@@ -286,6 +286,7 @@ static int launch_int4_tile(const I4Params& p, cudaStream_t stream) {
 
 template <int GS>
 static int int4_tile(const I4Params& p, bool glu, cudaStream_t stream) {
+    if (p.rows <= 32) return glu ? launch_int4_tile<32, GS, true>(p, stream) : launch_int4_tile<32, GS, false>(p, stream);
     if (p.rows <= 64) return glu ? launch_int4_tile<64, GS, true>(p, stream) : launch_int4_tile<64, GS, false>(p, stream);
     if (p.rows <= 128) return glu ? launch_int4_tile<128, GS, true>(p, stream) : launch_int4_tile<128, GS, false>(p, stream);
     return glu ? launch_int4_tile<256, GS, true>(p, stream) : launch_int4_tile<256, GS, false>(p, stream);

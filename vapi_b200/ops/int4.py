@@ -12,12 +12,9 @@ from . import linear_swiglu as _linear_swiglu
 from . import swiglu as _swiglu
 
 INT4_GROUPS = (32, 64, 128)
-#: products of more bfloat16 rows than this take the weight as bfloat16 numbers through this package's and the library's products, and from
-#: _SMALL_ROWS rows on those of weights of fewer than _LARGE numbers do: writing a weight out costs 0.43 us for each million of its numbers, the
-#: kernel's lesser rate a fifth of the product.  us of the kernel and of the other form: 6,144 x 2,048, 128 rows 11 / 13, 256 rows 15 / 14; 16,384 x 2,048
-#: gated, 256 rows 20 / 33, 512 rows 38 / 43, 1,024 rows 74 / 66; 8,192 x 28,672, 512 rows 214 / 274
-INT4_MAX_ROWS = int(os.environ.get("VAPI_INT4_MAX_ROWS", "512"))
-_SMALL_ROWS, _LARGE = 128, 1 << 24
+#: products of more bfloat16 rows than this take the weight as bfloat16 numbers through this package's and the library's products (and of fewer,
+#: where :func:`_own` says so)
+INT4_MAX_ROWS = int(os.environ.get("VAPI_INT4_MAX_ROWS", "2048"))
 
 
 class Int4Weight:
@@ -160,8 +157,14 @@ def int4_dequantize(w: Int4Weight, dtype: torch.dtype) -> torch.Tensor:
 
 
 def _own(rows: int, w: Int4Weight) -> bool:
-    """Whether a product of so many bfloat16 rows is csrc/int4.cu's."""
-    return rows <= INT4_MAX_ROWS and (rows <= _SMALL_ROWS or w.n * w.k >= _LARGE)
+    """Whether a product of so many bfloat16 rows is csrc/int4.cu's.  Writing a weight out costs 0.43 us for each million of its numbers, and the
+    kernel's lesser rate a part of the product, which is the larger the shorter K is (a block's start and end).  us of the kernel and of the other
+    form: 2,048 x 2,048, 128 rows 8.0 / 8.7, 256 rows 11.3 / 9.0; 6,144 x 2,048, 256 rows 13.4 / 14.0, 512 rows 18.3 / 18.5, 1,024 rows 35 / 27;
+    16,384 x 2,048, 768 rows 53.6 / 54.0, 1,024 rows 70 / 64; 2,048 x 8,192, 512 rows 20 / 26, 2,048 rows 49 / 54; 28,672 x 8,192 gated, 2,048 rows
+    757 / 862."""
+    numbers = w.n * w.k
+    most = 128 if numbers < 1 << 23 else 512 if numbers < 1 << 24 else 768 if w.k < 4096 else 2048
+    return rows <= min(most, INT4_MAX_ROWS)
 
 
 def _rows(x: torch.Tensor, w: Int4Weight, bias, out: torch.Tensor, gated: int, act: int) -> torch.Tensor:
@@ -175,8 +178,8 @@ def _rows(x: torch.Tensor, w: Int4Weight, bias, out: torch.Tensor, gated: int, a
 def int4_linear(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """:func:`linear` with a 4-bit weight: ``x @ W.T (+ bias)`` for ``x`` [n, k], in ``out_dtype`` (the type of ``x``, or float32).
 
-    Up to 24 bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in float32, and the
-    result is rounded once.  More rows take the weight's numbers rounded to bfloat16, in the product itself up to INT4_MAX_ROWS rows, else,
+    Up to 16 bfloat16 rows the codes are multiplied as the whole numbers they are, a group's sum is put on its scale in float32, and the
+    result is rounded once.  More rows take the weight's numbers rounded to bfloat16, in the product itself up to 128 to INT4_MAX_ROWS rows (by the weight's size), else,
     as float32 ``x`` does with them in float32, through :func:`int4_dequantize` and :func:`linear`."""
     if type(w) is Int4Weight and x.is_cuda and x.dtype == torch.bfloat16 and _own(x.shape[0], w) and out_dtype in (None, torch.bfloat16, torch.float32):
         lib = _lib("int4")
