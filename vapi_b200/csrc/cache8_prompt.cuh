@@ -71,13 +71,6 @@ __device__ __forceinline__ void p8_numbers(const uint4& c, float f, uint4& lo, u
     hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
-// whether a phase has ended, without waiting for it
-__device__ __forceinline__ bool p8_ended(unsigned bar, unsigned parity) {
-    unsigned yes;
-    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes) : "r"(bar), "r"(parity) : "memory");
-    return yes != 0;
-}
-
 // JOIN: whether `splits` blocks of a cluster share a tile's keys.  (A kernel of its own: the registers of the join in the same one cost the
 // other 5%.)
 template <int HD, bool JOIN>
@@ -429,8 +422,8 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 if (c == 5) {                                       // (asked now, wanted when these are written)
-                    s_there = p8_ended(my_full + 8 * (sb ^ 1), ((i + 1) >> 1) & 1);
-                    kv_there = p8_ended(kv_full + 8 * ((i + 1) % STAGES), ((i + 1) / STAGES) & 1);
+                    s_there = mbar_ended(my_full + 8 * (sb ^ 1), ((i + 1) >> 1) & 1);
+                    kv_there = mbar_ended(kv_full + 8 * ((i + 1) % STAGES), ((i + 1) / STAGES) & 1);
                 }
                 unsigned w[4];
                 const float2 f2 = make_float2(f[c >> 1], f[c >> 1]);

@@ -10,6 +10,11 @@
 //   warp 9      D[feature][row] += W X^T, issued by one lane of the whole warp; owns the tensor memory.
 // Then warps 0..7 bring D to shared memory, where x's stages were, and all threads write what comes of it, four features at a time.
 //
+// What bounds it: making the numbers.  A chunk is 64 conversions a lane of eight warps beside barriers and the store, 430 cycles of a warp one after
+// the other, and about as many of a multiprocessor with two blocks on it; the products of 64 rows take 180, the bytes of a chunk's codes 190.  64
+// rows of 8,192 x 28,672 in 45 us (2.7 TB/s of codes; with 16-bit weights the product takes 76), of 16,384 x 2,048 gated in 11.0 (9.6), of 2,048 x
+// 8,192 in 11.4 (11.9); 2,048 rows of 2,048 x 8,192 in 48 us, 1.43 PFLOP/s.
+//
 // Every wait is bounded; a role that gives up marks the block, whose results are then NaN.
 #pragma once
 #include "cluster.cuh"
@@ -81,14 +86,17 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) bring(from + i, w[i], sc[i]);
         int stage = 0, parity = 1;
-        bool ok = true;
+        bool ok = true, free = true;               // (the first stages are)
         for (int at = from; at < upto && ok; at += AHEAD) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int ch = at + i;
                 if (ch >= upto) break;
-                if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * stage, parity))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, free) && !mbar_wait_warp(empty + 8 * stage, parity)) { ok = false; break; }
                 tc5_fence_after();
+                // (the next stage asked for before this one is made: 8,192 x 28,672, 64 rows 45.8 to 44.7 us; small ones the same)
+                const int next = stage + 1 == STAGES ? 0 : stage + 1;
+                free = mbar_ended(empty + 8 * next, next == 0 ? parity ^ 1 : parity);
                 const unsigned words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
                 unsigned v[16];                    // word 2j + q of a row's 8 words a lane: of row g, of row g + 8
 #pragma unroll
@@ -113,7 +121,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + 8 * stage);
                 bring(ch + AHEAD, w[i], sc[i]);
-                if (++stage == STAGES) { stage = 0; parity ^= 1; }
+                if (next == 0) parity ^= 1;
+                stage = next;
             }
         }
         if (ok && upto > from && !__all_sync(0xffffffffu, mbar_wait(done, 0))) ok = false;
@@ -259,12 +268,13 @@ static int launch_int4_tile(const I4Params& p, cudaStream_t stream) {
         ready[dev] = 1;
     }
     const long long blocks = ((p.n + 15) / 16 + 7) / 8;               // (a gated block's eight tile rows are four of each half)
-    // Columns shared out while every block has a place at once and at least 8 chunks; above 128 rows, where what is joined is larger, by 4 at most.
-    // us with 1, 2, 4 and 8 blocks: 2,048 x 2,048, 33 rows 13.0 / 8.6 / 6.5 / 6.4, 128 rows 16.7 / 10.9 / 9.1 / 10.9; 6,144 x 2,048, 64 rows 13.9 / 9.5 /
-    // 9.6 / 17.4; 2,048 x 8,192, 64 rows 47 / 26 / 16 / 14, 256 rows 62 / 35 / 22 / 34; 8,192 x 28,672, 64 rows 205 / 121 / 67.
+    // Columns shared out while every block has a place at once and at least 8 chunks (12 with 65 to 128 rows); above 128 rows, where what is joined is
+    // larger, by 4 at most.  us with 1, 2, 4 and 8 blocks: 2,048 x 2,048, 24 rows 8.5 / 6.6 / 5.5 / 5.4, 64 rows 9.4 / 7.3 / 6.5 / 7.5; 6,144 x 2,048, 64 rows
+    // 9.7 / 7.7 / 8.4 / 16.6, 128 rows 11.1 / 8.9 / 12.0 / 23.7; 2,048 x 8,192, 64 rows 32 / 18 / 12 / 11, 256 rows 43 / 26 / 18 / 31; 8,192 x 28,672, 64 rows
+    // 141 / 80 / 45.
     const long long all = blocks * ((p.rows + N - 1) / N), held = (long long)sm_count() * I4T_BLOCKS<N>;
     int splits = 1;
-    while (splits < (N > 128 ? 4 : 8) && 2 * splits * all <= held && p.chunks / (2 * splits) >= 8) splits *= 2;
+    while (splits < (N > 128 ? 4 : 8) && 2 * splits * all <= held && p.chunks / (2 * splits) >= (N == 128 ? 12 : 8)) splits *= 2;
     CUtensorMap tm;
     const int rc = kmajor_map(&tm, "int4_linear", p.x, p.rows, p.k, N, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, false);
     if (rc != 0) return rc;

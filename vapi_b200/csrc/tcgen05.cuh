@@ -30,7 +30,13 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
     }
     return false;
 }
-// the same by a whole warp, with one outcome
+// whether a phase has ended, without waiting for it
+__device__ __forceinline__ bool mbar_ended(unsigned bar, unsigned parity) {
+    unsigned yes;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes) : "r"(bar), "r"(parity) : "memory");
+    return yes != 0;
+}
+// a wait by a whole warp, with one outcome
 __device__ __forceinline__ bool mbar_wait_warp(unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 // one lane of a whole warp, the same every time
 __device__ __forceinline__ bool elect_lane() {
