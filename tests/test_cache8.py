@@ -382,6 +382,20 @@ def test_attention_on_the_general_kernel(nh, nkv, d, page, dtype, window):
 
 
 @gpu
+@pytest.mark.parametrize("splits", [None, 1, 3, 8, 16])
+@pytest.mark.parametrize("nh,nkv,d,dtype,rows", [(4, 1, 80, torch.float32, 1), (2, 2, 64, torch.float32, 7), (8, 1, 256, torch.bfloat16, 3)])
+def test_the_general_kernel_over_a_cluster(splits, nh, nkv, d, dtype, rows):
+    """Blocks with several tiles of keys, one and none; tokens before the first key beside others of their tile."""
+    c = _attention_case([2500, 9, 40], [rows, rows, rows], nh, nkv, d, 16, dtype, d + rows)
+    got = _run_attention(c, d ** -0.5, splits=splits, impl="general")
+    _check_attention(c, got, d ** -0.5, tensor_cores=False)
+    assert torch.equal(got, _run_attention(c, d ** -0.5, splits=splits, impl="general"))
+    c["kl"] = torch.tensor([2500, 0, rows - 1], dtype=torch.int32)
+    blind = _run_attention(c, d ** -0.5, splits=splits, impl="general")
+    assert torch.equal(blind[:rows], got[:rows]) and not blind[rows:2 * rows + 1].any() and torch.isfinite(blind).all()
+
+
+@gpu
 def test_queries_at_any_stride_and_place():
     for extra, tensor_cores in ((64, True), (8, True), (4, False), (1, False)):
         c = _attention_case([70, 30], [2, 30], 4, 2, 64, 64, torch.bfloat16, extra, extra)

@@ -393,116 +393,212 @@ VAPI_EXPORT int vapi_cache8_read(const void* codes, const void* exps, const int*
 }
 
 // ---- attention: the general kernel --------------------------------------------------------------
-// float32 activations, head sizes other than 64 and 128.  A block owns 16 rows (query token, q head of the group) of one (sequence,
-// kv head) and walks the keys 32 at a time; K and V of a tile stand in shared memory as floats, a warp owns four rows, a lane
-// one key of the scores and every 32nd element of the output.  One pass with a running maximum and sum per row, in float.
-constexpr int G8_ROWS = 16, G8_KEYS = 32, G8_WARPS = 4, G8_RPW = G8_ROWS / G8_WARPS;
+// float32 activations, head sizes other than 64 and 128, queries at any alignment; float FMAs.  A block owns R rows (query token, q head of the group) of
+// one (sequence, kv head); its eight warps, and those of the up to 8 blocks of its cluster, each take a run of the key tiles, 32 keys a tile,
+// a lane one key of the scores (a code is turned once for all rows) and every 32nd element of the output.  One pass with a running maximum and sum a
+// row, in float; the results are joined in the order of warps, then of blocks.  Bound by its loads of single codes and float operations.  32 / 8 heads
+// of 64, float32: one request of 4,090 keys 32 us, 64 of 128 to 2,048 146, 8 of 32,000 700 (in bfloat16 the mma.sync kernel takes 6, 20 and 48), 500 tokens
+// behind 100 245 (15).
+constexpr int G8_KEYS = 32, G8_WARPS = 8, G8_MAX_CLUSTER = 8;
 
-template <typename T, int DMAX>
+template <typename T, int DMAX, int R>
 __global__ void __launch_bounds__(G8_WARPS * 32)
-attention8_kernel(const C8Params p, const T* __restrict__ q, T* __restrict__ out) {
-    extern __shared__ float g8_smem[];
-    const int d = p.d, pitch = d + 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* sQ = g8_smem;
-    float* sK = sQ + G8_ROWS * pitch;
-    float* sV = sK + G8_KEYS * pitch;
-    const int s = blockIdx.z, g = blockIdx.y, n_rep = p.nh / p.nkv;
+attention8_kernel(const C8Params p, const T* __restrict__ q, T* __restrict__ out, const int splits) {
+    constexpr int C = DMAX / 32;
+    extern __shared__ __align__(16) float g8_smem[];
+    __shared__ float sM[G8_WARPS][R], sL[G8_WARPS][R], xM[R], xL[R];
+    const int d = p.d, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* sQ = g8_smem;                                            // [R][d]; then, in its place, the block's O
+    float* sO = g8_smem + R * d;                                    // [warp][R][d]
+    const int rank = (int)blockIdx.x % splits, s = blockIdx.z, g = blockIdx.y, n_rep = p.nh / p.nkv;
     pdl_trigger();
     pdl_wait();
     const int q0 = p.cu_q[s], qlen = p.cu_q[s + 1] - q0, klen = p.seqlens_k[s];
-    const int rows_total = qlen * n_rep, r0 = blockIdx.x * G8_ROWS;
-    if (r0 >= rows_total) return;
+    const int rows_total = qlen * n_rep, r0 = (int)blockIdx.x / splits * R;
+    if (r0 >= rows_total) return;                                   // (the same for the whole cluster)
     const int base = klen - qlen;
-    const int p_min = base + r0 / n_rep, p_max = base + (min(rows_total, r0 + G8_ROWS) - 1) / n_rep;
-    for (int i = threadIdx.x; i < G8_ROWS * d; i += blockDim.x) {
-        const int r = i / d, c = i - r * d, rr = r0 + r;
-        const int tok = rr / n_rep, head = g * n_rep + rr - tok * n_rep;
-        sQ[r * pitch + c] = rr < rows_total ? to_f32(q[(size_t)(q0 + tok) * p.q_row_stride + (size_t)head * d + c]) * p.scale_log2e : 0.f;
+    const int p_min = base + r0 / n_rep, p_max = base + (min(rows_total, r0 + R) - 1) / n_rep;
+    const int lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
+    for (int i = threadIdx.x; i < R * d; i += blockDim.x) {
+        const int r = i / d, c = i - r * d, rr = r0 + r, tok = rr / n_rep;
+        sQ[i] = rr < rows_total ? to_f32(q[(size_t)(q0 + tok) * p.q_row_stride + (size_t)(g * n_rep + rr - tok * n_rep) * d + c]) * p.scale_log2e : 0.f;
     }
-    float m[G8_RPW], l[G8_RPW], o[G8_RPW][DMAX / 32];
+    int pos[R];                                                     // -1: sees nothing
+    float m[R], l[R], o[R][C];
 #pragma unroll
-    for (int r = 0; r < G8_RPW; ++r) {
+    for (int r = 0; r < R; ++r) {
+        pos[r] = r0 + r < rows_total ? base + (r0 + r) / n_rep : -1;
         m[r] = -INFINITY;
         l[r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < DMAX / 32; ++c) o[r][c] = 0.f;
+        for (int c = 0; c < C; ++c) o[r][c] = 0.f;
     }
-    const int lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
+    __syncthreads();
     const int* bt = p.block_table + (size_t)s * p.table_stride;
-    for (int k0 = lo / G8_KEYS * G8_KEYS; k0 <= p_max; k0 += G8_KEYS) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * G8_KEYS * (d / 4); i += blockDim.x) {
-            const int kv = i / (G8_KEYS * (d / 4)), j = i - kv * G8_KEYS * (d / 4), r = j / (d / 4), c = j - r * (d / 4), key = k0 + r;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);            // keys behind the end may hold anything, and are not read
-            if (key < klen && key <= p_max && key >= lo) {
-                const int page = bt[key / p.page_size];
-                if (page < 0 || page >= p.num_pages) {
-                    if (p.status) atomicExch(p.status, 4);
-                } else {
-                    const size_t head = ((size_t)page * 2 + kv) * p.nkv + g;
-                    const int off = key % p.page_size;
-                    v = c8_floats(*reinterpret_cast<const unsigned*>(p.codes + (head * p.page_size + off) * d + 4 * c));
-                    const float f = c8_power(p.exps[head * (p.page_size / C8_BLOCK) + off / C8_BLOCK]);
-                    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-                }
+    const int t_lo = lo / G8_KEYS, unit = rank * G8_WARPS + warp, units = splits * G8_WARPS;
+    const long long tiles = p_max < lo ? 0 : p_max / G8_KEYS - t_lo + 1;
+    for (int t = t_lo + (int)(tiles * unit / units); t < t_lo + (int)(tiles * (unit + 1) / units); ++t) {
+        const int key = t * G8_KEYS + lane;
+        const bool there = key >= lo && key <= p_max;               // (keys that no row sees may hold anything, and are not read)
+        int page = there ? bt[key / p.page_size] : -1;
+        if (there && (page < 0 || page >= p.num_pages) && p.status) atomicExch(p.status, 4);
+        if (page >= p.num_pages) page = -1;
+        const int off = key % p.page_size;
+        const size_t head = ((size_t)max(page, 0) * 2) * p.nkv + g;
+        float x[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[r] = 0.f;
+        float fk = 0.f, fv = 0.f;                                   // (a page that is none: zeros)
+        if (page >= 0) {
+            const size_t e = head * (p.page_size / C8_BLOCK) + off / C8_BLOCK;
+            fk = c8_power(p.exps[e]);
+            fv = c8_power(p.exps[e + (size_t)p.nkv * (p.page_size / C8_BLOCK)]);
+            const uint4* k = reinterpret_cast<const uint4*>(p.codes + (head * p.page_size + off) * d);
+            for (int c = 0; c < d / 16; ++c) {
+                const uint4 v = k[c];
+                const float4 a[4] = {c8_floats(v.x), c8_floats(v.y), c8_floats(v.z), c8_floats(v.w)};
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 b = *reinterpret_cast<const float4*>(sQ + r * d + 16 * c + 4 * i);
+                        x[r] = fmaf(a[i].x, b.x, fmaf(a[i].y, b.y, fmaf(a[i].z, b.z, fmaf(a[i].w, b.w, x[r]))));
+                    }
             }
-            *reinterpret_cast<float4*>((kv ? sV : sK) + r * pitch + 4 * c) = v;
         }
-        __syncthreads();
+        unsigned seen[R], all = 0xffffffffu, any = 0u;              // keys of the tile that a row sees
 #pragma unroll
-        for (int r = 0; r < G8_RPW; ++r) {
-            const int rr = r0 + warp * G8_RPW + r;
-            if (rr >= rows_total) break;
-            const int pos = base + rr / n_rep, key = k0 + lane;
-            const float* qr = sQ + (warp * G8_RPW + r) * pitch;
-            float x = 0.f;
-            for (int c = 0; c < d; c += 4) {
-                const float4 a = *reinterpret_cast<const float4*>(qr + c), b = *reinterpret_cast<const float4*>(sK + lane * pitch + c);
-                x = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, x))));
-            }
-            const bool sees = key <= pos && key < klen && (p.window <= 0 || key > pos - p.window);
-            x = sees ? x : -INFINITY;
-            const unsigned seen = __ballot_sync(0xffffffffu, sees);
-            if (!seen) continue;
-            const float mx = fmaxf(m[r], warp_max(x)), use = mx == -INFINITY ? 0.f : mx;
-            const float alpha = exp2f(m[r] - use), w = sees ? exp2f(x - use) : 0.f;
+        for (int r = 0; r < R; ++r) {
+            const bool sees = there && key <= pos[r] && (p.window <= 0 || key > pos[r] - p.window);
+            seen[r] = __ballot_sync(0xffffffffu, sees);
+            x[r] = sees ? x[r] * fk : -INFINITY;
+            any |= seen[r];
+            if (r0 + r < rows_total) all &= seen[r];
+            if (!seen[r]) { x[r] = 0.f; continue; }
+            const float mx = fmaxf(m[r], warp_max(x[r])), use = mx == -INFINITY ? 0.f : mx;
+            const float alpha = exp2f(m[r] - use);
+            x[r] = sees ? exp2f(x[r] - use) : 0.f;                  // the weight
             m[r] = mx;
-            l[r] = l[r] * alpha + warp_sum(w);
+            l[r] = l[r] * alpha + x[r];                             // (a lane's share of the sum)
 #pragma unroll
-            for (int c = 0; c < DMAX / 32; ++c) o[r][c] *= alpha;
-            for (int k = 0; k < G8_KEYS; ++k) {
-                if (!(seen >> k & 1)) continue;                     // (a NaN behind the mask stays there)
-                const float wk = __shfl_sync(0xffffffffu, w, k);
+            for (int c = 0; c < C; ++c) o[r][c] *= alpha;
+        }
+#pragma unroll 4
+        for (int k = 0; k < G8_KEYS; ++k) {
+            if (!(any >> k & 1)) continue;
+            const int page_k = __shfl_sync(0xffffffffu, page, k);
+            const float f = __shfl_sync(0xffffffffu, fv, k);
+            const unsigned char* src = p.codes + ((((size_t)max(page_k, 0) * 2 + 1) * p.nkv + g) * p.page_size + (t * G8_KEYS + k) % p.page_size) * d;
+            float v[C];
 #pragma unroll
-                for (int c = 0; c < DMAX / 32; ++c)
-                    if (c * 32 + lane < d) o[r][c] = fmaf(wk, sV[k * pitch + c * 32 + lane], o[r][c]);
+            for (int c = 0; c < C; ++c) v[c] = page_k >= 0 && c * 32 + lane < d ? c8_floats(src[c * 32 + lane]).x * f : 0.f;
+            const bool every = all >> k & 1;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float w = __shfl_sync(0xffffffffu, x[r], k);
+                if (!every && !(seen[r] >> k & 1)) continue;        // (a NaN that a row does not see stays where it is)
+#pragma unroll
+                for (int c = 0; c < C; ++c) o[r][c] = fmaf(w, v[c], o[r][c]);
             }
         }
     }
 #pragma unroll
-    for (int r = 0; r < G8_RPW; ++r) {
-        const int rr = r0 + warp * G8_RPW + r;
-        if (rr >= rows_total) break;
-        const int tok = rr / n_rep, head = g * n_rep + rr - tok * n_rep;
-        const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];          // a row that sees nothing: zeros
+    for (int r = 0; r < R; ++r) {
+        const float sum = warp_sum(l[r]);
+        if (lane == 0) { sM[warp][r] = m[r]; sL[warp][r] = sum; }
 #pragma unroll
-        for (int c = 0; c < DMAX / 32; ++c)
-            if (c * 32 + lane < d) out[((size_t)(q0 + tok) * p.nh + head) * d + c * 32 + lane] = from_f32<T>(o[r][c] * inv);
+        for (int c = 0; c < C; ++c)
+            if (c * 32 + lane < d) sO[(warp * R + r) * d + c * 32 + lane] = o[r][c];
+    }
+    __syncthreads();
+    auto store = [&](int r, int c, float v, float sum) {
+        const int rr = r0 + r, tok = rr / n_rep;
+        if (rr >= rows_total) return;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;             // a row that sees nothing: zeros
+        out[((size_t)(q0 + tok) * p.nh + g * n_rep + rr - tok * n_rep) * d + c] = from_f32<T>(v * inv);
+    };
+    for (int i = threadIdx.x; i < R * d; i += G8_WARPS * 32) {
+        const int r = i / d, c = i - r * d;
+        float mx = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < G8_WARPS; ++w) mx = fmaxf(mx, sM[w][r]);
+        const float use = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int w = 0; w < G8_WARPS; ++w) {
+            const float f = exp2f(sM[w][r] - use);
+            sum = fmaf(sL[w][r], f, sum);
+            v = fmaf(sO[(w * R + r) * d + c], f, v);
+        }
+        if (splits == 1) {
+            store(r, c, v, sum);
+        } else {
+            sQ[i] = v;
+            if (c == 0) { xM[r] = mx; xL[r] = sum; }
+        }
+    }
+    if (splits > 1) {
+        cluster_sync();                                             // every block's result is in place
+        const int mine = (R * d + splits - 1) / splits;
+        for (int i = rank * mine + threadIdx.x; i < min((rank + 1) * mine, R * d); i += G8_WARPS * 32) {
+            const int r = i / d, c = i - r * d;
+            float ms[G8_MAX_CLUSTER], ls[G8_MAX_CLUSTER], vs[G8_MAX_CLUSTER], mx = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+            for (int j = 0; j < G8_MAX_CLUSTER; ++j) {              // (all under way together)
+                ms[j] = j < splits ? cluster_f32(cluster_peer(&xM[r], (unsigned)j)) : -INFINITY;
+                ls[j] = j < splits ? cluster_f32(cluster_peer(&xL[r], (unsigned)j)) : 0.f;
+                vs[j] = j < splits ? cluster_f32(cluster_peer(&sQ[i], (unsigned)j)) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < G8_MAX_CLUSTER; ++j) mx = fmaxf(mx, ms[j]);
+            const float use = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+            for (int j = 0; j < G8_MAX_CLUSTER; ++j) {
+                const float f = exp2f(ms[j] - use);
+                sum = fmaf(ls[j], f, sum);
+                v = fmaf(vs[j], f, v);
+            }
+            store(r, c, v, sum);
+        }
+        cluster_sync();                                             // nobody reads this block's memory any more
     }
 }
 
-template <typename T, int DMAX>
-static int launch_attention8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, cudaStream_t stream) {
-    const long long tiles = ((long long)max_q * (p.nh / p.nkv) + G8_ROWS - 1) / G8_ROWS;
-    if (tiles > 0x7fffffffLL || p.nkv > 65535 || num_seqs > 65535)
+template <typename T, int DMAX, int R>
+static int launch_attention8_of(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int max_k, int splits, cudaStream_t stream) {
+    const long long tiles = ((long long)max_q * (p.nh / p.nkv) + R - 1) / R;
+    if (tiles * G8_MAX_CLUSTER > 0x7fffffffLL || p.nkv > 65535 || num_seqs > 65535)
         return fail(-1, "paged_attention8: the step exceeds the grid (%lld row tiles, %d kv heads, %d sequences)", tiles, p.nkv, num_seqs);
-    const size_t smem = (size_t)(G8_ROWS + 2 * G8_KEYS) * (p.d + 4) * sizeof(float);
-    auto kern = attention8_kernel<T, DMAX>;
+    if (splits <= 0) {
+        // blocks to two a multiprocessor, while every warp has a tile
+        splits = 1;
+        while (splits < G8_MAX_CLUSTER && 2 * splits * tiles * p.nkv * num_seqs <= 2LL * sm_count() && 2LL * splits * G8_WARPS * G8_KEYS <= max_k) splits *= 2;
+    }
+    if (splits > G8_MAX_CLUSTER) splits = G8_MAX_CLUSTER;
+    const size_t smem = (size_t)(1 + G8_WARPS) * R * p.d * sizeof(float);
+    auto kern = attention8_kernel<T, DMAX, R>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     }
-    return check_launch("paged_attention8", launch(kern, dim3((unsigned)tiles, p.nkv, num_seqs), G8_WARPS * 32, smem, stream, p, (const T*)q, (T*)out));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * splits), p.nkv, num_seqs);
+    cfg.blockDim = dim3(G8_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return check_launch("paged_attention8", cudaLaunchKernelEx(&cfg, kern, p, (const T*)q, (T*)out, splits));
+}
+template <typename T, int DMAX>
+static int launch_attention8(const C8Params& p, const void* q, void* out, int num_seqs, int max_q, int max_k, int splits, cudaStream_t stream) {
+    if ((long long)max_q * (p.nh / p.nkv) <= 4) return launch_attention8_of<T, DMAX, 4>(p, q, out, num_seqs, max_q, max_k, splits, stream);
+    return launch_attention8_of<T, DMAX, 8>(p, q, out, num_seqs, max_q, max_k, splits, stream);
 }
 
 // How many blocks of the mma.sync kernel share the keys of one (sequence, kv head, tile of rows): a power of two up to a cluster's 16, while all
@@ -573,7 +669,7 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
         return d == 64 ? launch_decode8<64>(p, q, out, num_seqs, max_q, max_k, splits, most_q, stream)
                        : launch_decode8<128>(p, q, out, num_seqs, max_q, max_k, splits, most_q, stream);
     }
-#define VAPI_ATT8(T, DM) return launch_attention8<T, DM>(p, q, out, num_seqs, max_q, stream)
+#define VAPI_ATT8(T, DM) return launch_attention8<T, DM>(p, q, out, num_seqs, max_q, max_k, splits, stream)
     if (dtype == VAPI_F32) {
         if (d <= 64) VAPI_ATT8(float, 64); else if (d <= 128) VAPI_ATT8(float, 128); else VAPI_ATT8(float, 256);
     }
