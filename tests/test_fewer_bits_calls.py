@@ -129,3 +129,28 @@ def test_the_c_functions_own_refusals(ops):
     for slices in (3, 16, -1):
         with pytest.raises(ops.KernelError, match="power of two"):
             ops.token_logprobs(f(1, 10), i(0), 1, slices=slices)
+
+
+def test_operators_on_two_streams_at_once(ops):
+    """Kernels that hold tensor memory and wait for their cluster, beside one another and in turn."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(4)
+    cache = ops.cache8_empty(20, 8, 64, 64)
+    qkv = torch.randn(1280, 48 * 64, generator=g).bfloat16().cuda()
+    ops.qk_norm_rope_write8(qkv, 32, 8, 64, None, None, 0.0, None, None, 0, cache, torch.arange(1280, dtype=torch.int32, device="cuda"))
+    q, table, cu, kl = qkv[:200], torch.arange(20, dtype=torch.int32, device="cuda")[None], i32(0, 200), i32(1280)
+    w = ops.int4_quantize(torch.randn(2048, 2048, generator=g).cuda())
+    x, logits, tokens = torch.randn(64, 2048, generator=g).bfloat16().cuda(), torch.randn(8, 30000, generator=g).cuda(), i32(*range(8))
+    calls = [lambda: ops.paged_attention8(q, qkv.stride(0), cache, table, cu, kl, 200, 1, 200, 1280, 32, 8, 64, 0.125),
+             lambda: ops.int4_linear(x, w), lambda: ops.int4_linear_swiglu(x[:3], w), lambda: ops.token_logprobs(logits, tokens, 5).top_logprobs]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for turn in range(40):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append([calls[(j + 2 * i) % 4]() for j in range(4)])
+    torch.cuda.synchronize()
+    for n, outs in enumerate(got):
+        for j, o in enumerate(outs):
+            assert torch.equal(o, want[(j + 2 * (n % 2)) % 4]), (n, j)

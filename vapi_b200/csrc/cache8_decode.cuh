@@ -19,6 +19,9 @@
 //                to 2^15, float the sums), which no lane has to ask its neighbours for: a vote a chunk, and a reduction a few times
 //                a row.  P is turned about by movmatrix; the values of two tokens are paired by byte permutes.
 //
+// What bounds it: memory where keys are many (32 / 8 heads of 64, 8 requests of 32,000 keys 47 us, 5.6 TB/s; the 16-bit kernel 85), the integer
+// operations that turn codes to halves close behind; for one request of 4,090 keys (6.0 us) the way of table, exponents and codes after one another.
+//
 // Keys that a row does not see are masked by selection, and the values of those that no row of the block sees taken as zeros.  (A NaN among the
 // values that some of the block's rows see and others do not can reach the others through 0 * NaN; the step that wrote it was lost.)
 #pragma once

@@ -488,6 +488,16 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     }
     if constexpr (JOIN) {
         if (warp < 4 || warp == P8_THREADS / 32 - 1) __syncthreads();       // (with the softmax warps')
+    }
+    // (before the cluster's blocks wait for one another: what they hold meanwhile, another kernel's blocks may be waiting for)
+    tc5_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && flags[0] && p.status) atomicExch(p.status, 16);
+    if (warp == P8_THREADS / 32 - 1) {
+        tc5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((unsigned)P8_TMEM_COLS) : "memory");
+    }
+    if constexpr (JOIN) {
         cluster_sync();                                             // every block's result is in place
         const auto join = [&](auto blocks) {
             constexpr int C = decltype(blocks)::value;
@@ -530,13 +540,6 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         else if (splits == 4) join(std::integral_constant<int, 4>());
         else join(std::integral_constant<int, 8>());
         cluster_sync();                                             // nobody reads this block's memory any more
-    }
-    tc5_fence_before();
-    __syncthreads();
-    if (threadIdx.x == 0 && flags[0] && p.status) atomicExch(p.status, 16);
-    if (warp == P8_THREADS / 32 - 1) {
-        tc5_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((unsigned)P8_TMEM_COLS) : "memory");
     }
 }
 
