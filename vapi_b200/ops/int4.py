@@ -145,14 +145,14 @@ def _operands(x: torch.Tensor, w: Int4Weight) -> torch.Tensor:
 
 def int4_dequantize(w: Int4Weight, dtype: torch.dtype) -> torch.Tensor:
     """The numbers of a 4-bit weight, [n, k] in float32 (exactly) or bfloat16 (each rounded once: a scale times a whole number of
-    four bits has four bits more than bfloat16)."""
+    four bits has four bits more than bfloat16).  Any kernel launched behind the call may read them as a weight."""
     if dtype not in _DT:
         raise KernelError(f"dtype {dtype} is not supported by the kernels (float32, bfloat16)")
     _cuda(w.codes, w.scales)
     _here(w.codes, w.scales)
     out = torch.empty((w.n, w.k), dtype=dtype, device=w.device)
     lib = _lib("int4")
-    _check(lib, lib.vapi_int4_numbers(_p(w.codes), _p(w.scales), w.n, w.k, w.group, _p(out), _DT[dtype], _stream()))
+    _check(lib, lib.vapi_int4_numbers(_p(w.codes), _p(w.scales), w.n, w.k, w.group, _p(out), _DT[dtype], _stream()), launches=2)
     return out
 
 
