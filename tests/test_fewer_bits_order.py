@@ -5,7 +5,7 @@ import torch
 from test_int4 import _check, _random, _to_device
 
 pytestmark = pytest.mark.gpu
-BF, F32 = torch.bfloat16, torch.float32
+BF, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 
 
 @pytest.fixture
@@ -98,3 +98,96 @@ def test_a_product_with_a_weight_of_int4_dequantize(ops, dtype, rows):
     for got in _played(body):
         for i, y in enumerate(got):
             _check(x, hosts[i // 2], y, rounded=dtype == BF)
+
+# ---- a cache that is written -------------------------------------------------------------------------
+
+class Prompt:
+    """A prompt's rows, its cache, and what is done with them: 32 / 8 heads.  (Rows that are not 16-byte aligned are the general write's, a warp of which
+    takes 16 tokens one after the other: it ends late.)"""
+
+    def __init__(self, ops, d, n):
+        self.ops, self.d, self.n = ops, d, n
+        g = torch.Generator().manual_seed(4)
+        self.qkv = torch.randn(n * 48 * d + 1, generator=g).bfloat16().cuda()[1:].view(n, 48 * d)
+        self.cache = ops.cache8_empty(-(-n // 64), 8, 64, d)
+        self.slots = torch.arange(n, dtype=I32, device="cuda")
+        self.table = torch.arange(-(-n // 64), dtype=I32, device="cuda")[None]
+        self.lens = torch.tensor([n], dtype=I32, device="cuda")
+
+    def clear(self):
+        self.cache.codes.view(torch.uint8).fill_(0x7f)
+        self.cache.exps.zero_()
+
+    def write(self, a, b, rows=None):
+        return self.ops.qk_norm_rope_write8(self.qkv[a:b] if rows is None else rows, 32, 8, self.d, None, None, 0.0, None, None, 0, self.cache, self.slots[a:b])
+
+    def attend(self, q, ends, impl="auto"):
+        rows = q.shape[0]
+        return self.ops.paged_attention8(q, q.stride(0), self.cache, self.table, ends, self.lens, rows, 1, rows, self.n, 32, 8, self.d, self.d ** -0.5, impl=impl)
+
+
+def _ends(rows):
+    return torch.tensor([0, rows], dtype=I32, device="cuda")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,impl", [(1, "auto"), (7, "tensor_core"), (200, "tcgen05"), (200, "auto"), (1, "general")])
+def test_attention_of_the_last_tokens_of_what_was_just_written(ops, d, rows, impl):
+    """One write of a whole prompt, and attention of its last tokens straight behind it."""
+    n, ends = 6000, _ends(rows)
+    p = Prompt(ops, d, n)
+    q = p.write(0, n)[n - rows:]
+    torch.cuda.synchronize()
+    want = p.attend(q, ends, impl)
+    assert torch.isfinite(want).all()
+
+    def body():
+        p.clear()
+        return [p.attend(p.write(0, n)[n - rows:], ends, impl)]
+    for turn in range(5):
+        for got in _played(body):
+            assert torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 1000])
+def test_attention_behind_two_writes(ops, d, rows):
+    """A prompt in two portions, both written before the second's attention; and a portion, a token, the token's attention."""
+    n, ends = 7000, _ends(rows)
+    p = Prompt(ops, d, n)
+    p.write(0, n - rows)
+    torch.cuda.synchronize()
+    q = p.write(n - rows, n)
+    torch.cuda.synchronize()
+    want = p.attend(q, ends)
+    assert torch.isfinite(want).all()
+
+    def body():
+        p.clear()
+        p.write(0, n - rows)
+        return [p.attend(p.write(n - rows, n), ends)]
+    for turn in range(5):
+        for got in _played(body):
+            assert torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,impl", [(1, "auto"), (300, "tcgen05")])
+def test_settled_steps_read_their_own_tokens_when_they_are_written(ops, d, rows, impl):
+    """Within one_stream(settled=True), as in an engine's step: older keys ahead of the wait, the step's own behind its write."""
+    n, ends = 7000, _ends(rows)
+    p = Prompt(ops, d, n)
+    p.write(0, n - rows)
+    torch.cuda.synchronize()
+    q = p.write(n - rows, n)
+    torch.cuda.synchronize()
+    want = p.attend(q, ends, impl)
+    zeros = torch.zeros(rows, 48 * d, dtype=BF, device="cuda")
+    for turn in range(5):
+        p.write(n - rows, n, zeros)
+        torch.cuda.synchronize()
+        with ops.one_stream(settled=True):
+            assert ops._held.settled
+            p.write(n - rows, n)
+            got = p.attend(q, ends, impl)
+        assert torch.equal(got, want) and not ops._held.settled

@@ -637,10 +637,13 @@ static bool c8_portions(const C8Params& p, int n, int num_seqs, int max_q, int m
 // kernel; the general kernel for everything else.  1 = the general kernel; 2 = the mma.sync kernel, or an error;
 // 3 = the tcgen05 kernel for every sequence, or an error.  splits 0: as many as pay (max_k: the most keys
 // a sequence has); else those of the mma.sync kernel, up to 16, and at most 8, a power of two, of the tcgen05 kernel.
+// settled: no kernel that may still run when this one begins (the one before it, and those that it begins before the end of) writes keys before a sequence's
+// own tokens, as in an engine's step; else no key is read before every earlier kernel has ended.  us of one call after another, settled and not, 32 / 8
+// heads of 64: one request of 4,090 keys 6.0 / 6.4, 64 of 128 to 2,048 19.7 / 20.3, 8 of 32,000 47.0 / 49.0, 2,048 tokens behind 5,952 235.9 / 236.4.
 VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, const void* codes, const void* exps, int dtype, const int* block_table,
                                       int table_stride, const int* cu_q, const int* seqlens_k, void* out, int n, int num_seqs, int max_q,
                                       int max_k, int nh, int nkv, int d, int page_size, int num_pages, float scale, int window, int splits,
-                                      int impl, int* status, cudaStream_t stream) {
+                                      int impl, int settled, int* status, cudaStream_t stream) {
     if (n <= 0 || num_seqs <= 0 || max_q <= 0) return 0;
     if (d < 16 || d > 256 || d % 16 != 0) return fail(-1, "paged_attention8: head_dim %d is not a multiple of 16 in 16..256", d);
     if (nh <= 0 || nkv <= 0 || nh % nkv != 0) return fail(-1, "paged_attention8: %d heads are not a multiple of %d kv heads", nh, nkv);
@@ -650,7 +653,7 @@ VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, con
     C8Params p;
     p.q_row_stride = q_row_stride; p.codes = (const unsigned char*)codes; p.exps = (const signed char*)exps; p.block_table = block_table;
     p.table_stride = table_stride; p.cu_q = cu_q; p.seqlens_k = seqlens_k; p.nh = nh; p.nkv = nkv; p.d = d; p.page_size = page_size;
-    p.num_pages = num_pages; p.scale_log2e = scale * 1.4426950408889634f; p.window = window; p.status = status;
+    p.num_pages = num_pages; p.scale_log2e = scale * 1.4426950408889634f; p.window = window; p.settled = settled; p.status = status;
     const bool fast = dtype == VAPI_BF16 && (d == 64 || d == 128) && q_row_stride % 8 == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0;
     if (impl >= 2 && (!fast || (impl == 3 && !(scale > 0.f))))
         return fail(-3, "paged_attention8: the tensor-core kernels need bfloat16, head_dim 64 or 128, 16-byte aligned rows and, for portions, a "

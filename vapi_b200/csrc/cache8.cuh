@@ -16,6 +16,7 @@ struct C8Params {
     int nh, nkv, d, page_size, num_pages;
     float scale_log2e;
     int window;
+    int settled;                                   // keys before a sequence's own tokens were written by what has ended, whatever still runs
     int* status;
 };
 

@@ -117,7 +117,7 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     // Where 32 chunks at a time lie, one a lane, and their scales: looked up as the copies reach them, used as the products do.
     const int* bt = p.block_table + (size_t)s * p.table_stride;
     const int per_head = p.page_size / C8_BLOCK;
-    const int fresh = base < 0 ? 0 : base / C8_BLOCK;                       // the first chunk that this step's tokens may have changed
+    const int fresh = !p.settled || base < 0 ? 0 : base / C8_BLOCK;         // the first chunk that a kernel not yet waited for may have changed
     bool waited = false;
     int where = 0, scales_next = 0, scales = 0;
     auto look_up = [&](int from) {                                          // chunks begin + from ..

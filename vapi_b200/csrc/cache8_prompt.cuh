@@ -217,7 +217,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         constexpr int PER = 2 * P8_KEYS * HD / 16, EACH = (PER + P8_LOADERS - 1) / P8_LOADERS;       // 16-byte pieces of a tile, a thread
         const int* bt = p.block_table + (size_t)s * p.table_stride;
         const int per_head = p.page_size / C8_BLOCK;
-        const int fresh = base_pos < 0 ? 0 : base_pos / C8_BLOCK * C8_BLOCK;      // from here on the kernel before this one wrote
+        const int fresh = !p.settled || base_pos < 0 ? 0 : base_pos / C8_BLOCK * C8_BLOCK;      // from here on a kernel not yet waited for may have written
         bool waited = false;
         // Where the 32 blocks of eight tiles lie, one a lane, and their scales.  Looked up in two steps, both well before they are
         // wanted: a tile's codes are asked for two tiles ahead, and waiting for the table first would double the way.

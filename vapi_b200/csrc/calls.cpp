@@ -312,14 +312,14 @@ PyObject* read8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 }
 
 typedef int (*Attention8Fn)(const void*, long long, const void*, const void*, int, const int*, int, const int*, const int*, void*, int, int, int, int, int,
-                            int, int, int, int, float, int, int, int, int*, void*);
+                            int, int, int, int, float, int, int, int, int, int*, void*);
 
-// attention8(fn, q, q_row_stride, codes, exps, block_table, cu_q, seqlens_k, n, num_seqs, max_q, max_k, nh, nkv, d, scale, window, splits, impl, status,
-//            stream, device): ops.paged_attention8
+// attention8(fn, q, q_row_stride, codes, exps, block_table, cu_q, seqlens_k, n, num_seqs, max_q, max_k, nh, nkv, d, scale, window, splits, impl, settled,
+//            status, stream, device): ops.paged_attention8
 PyObject* attention8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-    return guarded(nargs, 22, [&](bool& called) -> PyObject* {
+    return guarded(nargs, 23, [&](bool& called) -> PyObject* {
         const auto fn = reinterpret_cast<Attention8Fn>(address(a[0]));
-        const int device = integer(a[21]), n = integer(a[8]), seqs = integer(a[9]), max_q = integer(a[10]), max_k = integer(a[11]);
+        const int device = integer(a[22]), n = integer(a[8]), seqs = integer(a[9]), max_q = integer(a[10]), max_k = integer(a[11]);
         const int nh = integer(a[12]), nkv = integer(a[13]), d = integer(a[14]);
         const int64_t stride = integer(a[2]);
         const at::Tensor* q = on(tensor(a[1]), device);
@@ -332,16 +332,16 @@ PyObject* attention8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         if (!table || table->scalar_type() != at::kInt || table->dim() != 2 || table->stride(1) != 1 || table->size(0) < seqs) throw Bad{};
         const int *cu = ints_on(a[6], seqs + 1LL, device), *kl = ints_on(a[7], seqs, device);
         const float scale = real(a[15]);
-        const int window = integer(a[16]), splits = integer(a[17]), impl = integer(a[18]), table_stride = size32(table->stride(0));
-        int* status = static_cast<int*>(address(a[19]));
-        void* stream = address(a[20]);
+        const int window = integer(a[16]), splits = integer(a[17]), impl = integer(a[18]), settled = integer(a[19]), table_stride = size32(table->stride(0));
+        int* status = static_cast<int*>(address(a[20]));
+        void* stream = address(a[21]);
         at::Tensor out = at::empty({n, (int64_t)nh * d}, q->options());
         int rc;
         called = true;
         {
             Unlocked unlocked;
             rc = fn(q->data_ptr(), stride, c.codes->data_ptr(), c.exps->data_ptr(), type, static_cast<const int*>(table->data_ptr()), table_stride, cu, kl,
-                    out.data_ptr(), n, seqs, max_q, max_k, nh, nkv, d, c.page_size, c.pages, scale, window, splits, impl, status, stream);
+                    out.data_ptr(), n, seqs, max_q, max_k, nh, nkv, d, c.page_size, c.pages, scale, window, splits, impl, settled, status, stream);
         }
         return rc != 0 ? PyLong_FromLong(rc) : wrap(out);
     });

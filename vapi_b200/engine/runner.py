@@ -207,7 +207,7 @@ class ModelRunner:
         """Device work of a step for a prepared context; returns float32 logits [rows, vocab]
         or None when no logits are wanted (the caches are written either way)."""
         if self.device.type == "cuda":
-            with ops.one_stream(self.status):
+            with ops.one_stream(self.status, settled=True):      # (what came before is a copy's, or an earlier graph's)
                 return self._forward(ctx)
         return self._forward(ctx)
 

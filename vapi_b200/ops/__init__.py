@@ -198,6 +198,7 @@ class _Held(threading.local):
     """What the running step of a thread holds for its kernels (class attributes: a lookup with a default costs every launch)."""
     stream: Optional[int] = None
     status: Optional[int] = None
+    settled: bool = False
 
 
 _held = _Held()
@@ -217,19 +218,22 @@ class one_stream:
     """Within the block every kernel of this module launches on the stream that is current at its
     entry, looked up once instead of once per kernel (a step launches a few hundred).  The caller
     must not switch streams inside the block.  ``status``: the step's status word, into which the
-    products record a bounded wait that ran out (their callers, the parts of a model, do not carry it)."""
+    products record a bounded wait that ran out (their callers, the parts of a model, do not carry it).  ``settled``: the
+    caller's word that when the block's first kernel begins, the caches hold for good what attention finds before a sequence's own tokens (the last
+    ``cu_q[s + 1] - cu_q[s]`` of its ``seqlens_k[s]``), as in a step of an engine; :func:`paged_attention8` then reads it while the kernel
+    before it still runs."""
 
-    def __init__(self, status: Optional[torch.Tensor] = None):
-        self.status = status
+    def __init__(self, status: Optional[torch.Tensor] = None, settled: bool = False):
+        self.status, self.settled = status, settled
 
     def __enter__(self):
-        self.before = _held.stream, _held.status
+        self.before = _held.stream, _held.status, _held.settled
         _held.stream = torch.cuda.current_stream().cuda_stream if torch.cuda.is_available() else None
-        _held.status = _p(self.status)
+        _held.status, _held.settled = _p(self.status), self.settled
         return self
 
     def __exit__(self, *exc):
-        _held.stream, _held.status = self.before
+        _held.stream, _held.status, _held.settled = self.before
         return False
 
 

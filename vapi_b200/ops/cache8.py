@@ -5,7 +5,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import KernelError, _check, _contig, _cuda, _dt, _f32, _here, _i32, _least, _lib, _native, _p, _stream
+from . import KernelError, _check, _contig, _cuda, _dt, _f32, _held, _here, _i32, _least, _lib, _native, _p, _stream
 
 #: tokens of a head that share a scale
 CACHE8_BLOCK = 16
@@ -129,6 +129,9 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     request's end are not looked at.  A value that is not a number reaches the queries that see its token, and on the tensor cores also those
     of the same portion that stand before it in one tile, as with :func:`paged_attention`.
 
+    The cache may be the work of any kernel ahead on the stream.  Within ``one_stream(settled=True)`` what it holds before a sequence's own tokens of
+    the call is read while kernels ahead still run, and must be none of theirs.
+
     ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions (where rows and keys are enough for
     it), and the mma.sync kernel for the others, in both of which ``splits`` blocks (up to 16, and up to 8) share the keys as a cluster; the
     general kernel for every other type, head size (a multiple of 16 up to 256) and alignment.  "tcgen05", "tensor_core" and "general" force one (the first two raise where
@@ -141,7 +144,7 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     if q.is_cuda and code is not None:
         lib = _lib("cache8")
         got = _native("attention8", lib, "vapi_paged_attention8", q, q_row_stride, cache[0], cache[1], block_table, cu_q, seqlens_k, n, num_seqs,
-                      max_q, max_k, nh, nkv, d, scale, window, splits or 0, code, _p(status))
+                      max_q, max_k, nh, nkv, d, scale, window, splits or 0, code, int(_held.settled), _p(status))
         if got is not NotImplemented:
             _check(lib, got if type(got) is int else 0, kernels)
             return got
@@ -166,5 +169,5 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     lib = _lib("cache8")
     _check(lib, lib.vapi_paged_attention8(_p(q), q_row_stride, _p(cache.codes), _p(cache.exps), _dt(q), _p(block_table), block_table.stride(0),
                                           _p(cu_q), _p(seqlens_k), _p(out), n, num_seqs, max_q, max_k, nh, nkv, d, page_size, pages,
-                                          scale, window, splits or 0, code, _p(status), _stream()), launches=kernels)
+                                          scale, window, splits or 0, code, int(_held.settled), _p(status), _stream()), launches=kernels)
     return out
