@@ -191,3 +191,25 @@ def test_settled_steps_read_their_own_tokens_when_they_are_written(ops, d, rows,
             p.write(n - rows, n)
             got = p.attend(q, ends, impl)
         assert torch.equal(got, want) and not ops._held.settled
+
+
+# ---- a wait that is given up ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("gated", [0, 1])
+@pytest.mark.parametrize("n,k,splits", [(2048, 2048, 4), (256, 4096, 8), (40000, 256, 1)])
+def test_a_product_one_of_whose_blocks_gives_up_is_nan(ops, n, k, splits, gated):
+    """The blocks of one rank of their clusters take no wait: every result that their sums would have entered is NaN, and the next call is unaffected."""
+    w = _to_device(ops.int4_pack(*_random(n, k, 64, 7)))
+    x = torch.randn(50, k, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    call = ops.int4_linear_swiglu if gated else ops.int4_linear
+    want, lib = call(x, w), ops._lib("int4")
+    for trial in (-1, *range(splits), 8):
+        out = torch.zeros_like(want)
+        rc = lib.vapi_int4_linear(w.codes.data_ptr(), w.scales.data_ptr(), n, k, 64, x.data_ptr(), 50, None, out.data_ptr(), None, gated, 0, trial,
+                                  torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        if 0 <= trial < splits:
+            assert torch.isnan(out).all(), trial
+        else:
+            assert torch.equal(out, want)
+        assert torch.equal(call(x, w), want)

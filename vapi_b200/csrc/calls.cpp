@@ -347,7 +347,7 @@ PyObject* attention8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
-typedef int (*Int4Fn)(const void*, const void*, int, int, int, const void*, int, const float*, void*, float*, int, int, void*);
+typedef int (*Int4Fn)(const void*, const void*, int, int, int, const void*, int, const float*, void*, float*, int, int, int, void*);
 
 // int4(fn, codes, scales, n, k, group, x, bias, gated, act, float32 or not, stream, device): ops.int4_linear and int4_linear_swiglu of few rows.
 // (codes and scales are an Int4Weight's, laid out and checked by int4_pack)
@@ -370,7 +370,7 @@ PyObject* int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         {
             Unlocked unlocked;
             rc = fn(codes.data_ptr(), scales.data_ptr(), n, k, group, x.data_ptr(), rows, bias, f32 ? nullptr : out.data_ptr(),
-                    f32 ? static_cast<float*>(out.data_ptr()) : nullptr, gated, act, stream);
+                    f32 ? static_cast<float*>(out.data_ptr()) : nullptr, gated, act, -1, stream);
         }
         return rc != 0 ? PyLong_FromLong(rc) : wrap(out);
     });

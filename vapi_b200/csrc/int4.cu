@@ -30,6 +30,7 @@ struct I4Params {
     __nv_bfloat16* y;                              // [rows][n], or [rows][n / 2] for a gated product
     float* y32;                                    // instead of y
     int act;
+    int trial;                                     // a rank whose blocks give up at their first wait, or -1
 };
 
 // two codes, `shift` and 16 + shift bits up, less their row's zero
@@ -284,9 +285,10 @@ static int int4_rows(const I4Params& p, bool glu, cudaStream_t stream) {
 }
 
 // x [rows][k] bfloat16 with 16-byte aligned rows.  gated: W is [gate; up], y [rows][n / 2] = act(gate) * up, n / 2 a multiple of 16.
-// y32 instead of y for float32 results (not for a gated product).
+// y32 instead of y for float32 results (not for a gated product).  trial: -1; from 0 on, with 33 to 64 rows and groups of 64, the rank in its cluster of
+// blocks that take no wait.
 VAPI_EXPORT int vapi_int4_linear(const void* codes, const void* scales, int n, int k, int group, const void* x, int rows, const float* bias,
-                                 void* y, float* y32, int gated, int act, cudaStream_t stream) {
+                                 void* y, float* y32, int gated, int act, int trial, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (n <= 0 || k <= 0) return fail(-1, "int4_linear: a weight of %d x %d", n, k);
     if (group != 32 && group != 64 && group != 128) return fail(-1, "int4_linear: groups of %d columns are not 32, 64 or 128", group);
@@ -296,7 +298,7 @@ VAPI_EXPORT int vapi_int4_linear(const void* codes, const void* scales, int n, i
     if (rows > 65535 * 128) return fail(-1, "int4_linear: %d rows exceed the grid", rows);
     I4Params p;
     p.codes = (const unsigned*)codes; p.scales = (const unsigned*)scales; p.n = n; p.k = k; p.group = group; p.chunks = (k + 63) / 64;
-    p.x = (const __nv_bfloat16*)x; p.rows = rows; p.bias = bias; p.y = (__nv_bfloat16*)y; p.y32 = y32; p.act = act;
+    p.x = (const __nv_bfloat16*)x; p.rows = rows; p.bias = bias; p.y = (__nv_bfloat16*)y; p.y32 = y32; p.act = act; p.trial = trial;
     if (rows > I4_MOST_ROWS) {
         if (group == 32) return int4_tile<2>(p, gated != 0, stream);
         if (group == 64) return int4_tile<4>(p, gated != 0, stream);

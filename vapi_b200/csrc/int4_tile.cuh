@@ -15,7 +15,8 @@
 // rows of 8,192 x 28,672 in 45 us (2.7 TB/s of codes; with 16-bit weights the product takes 76), of 16,384 x 2,048 gated in 11.0 (9.6), of 2,048 x
 // 8,192 in 11.4 (11.9); 2,048 rows of 2,048 x 8,192 in 48 us, 1.43 PFLOP/s.
 //
-// Every wait is bounded; a role that gives up marks the block, whose results are then NaN.
+// Every wait is bounded; a role that gives up marks the block, whose sums are then NaN, and so is every result of its cluster, which adds them up.  The
+// products and copies that are under way are awaited first.
 #pragma once
 #include "cluster.cuh"
 #include "tcgen05.cuh"
@@ -36,7 +37,8 @@ __device__ __forceinline__ void i4t_mma(unsigned d, unsigned a, unsigned long lo
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
 }
 
-template <int N, int GS, bool GLU>                 // GS: k-steps of 16 columns a group (2, 4, 8)
+// GS: k-steps of 16 columns a group (2, 4, 8).  TRIAL: the blocks of one rank give up at their first wait (p.trial; for tests)
+template <int N, int GS, bool GLU, bool TRIAL>
 __global__ void __launch_bounds__(I4T_THREADS, I4T_BLOCKS<N>)
 int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, const int splits) {
     constexpr int STAGES = I4T_STAGES<N>, STAGE = I4T_STAGE<N>, COLUMNS = I4T_COLUMNS<N>, AHEAD = I4T_AHEAD, GPC = GS < 4 ? 2 : 1, CPG = GS > 4 ? 2 : 1;
@@ -66,6 +68,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
     tc5_fence_after();
     pdl_trigger();                                 // (not before the allocation: a block of the next kernel that came between would be waited for, and wait)
     const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const bool give_up = TRIAL && rank == p.trial;
 
     if (warp < I4T_LOADERS) {
         // (a warp reaches the lanes of one quarter of tensor memory: two tile rows)
@@ -92,7 +95,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
             for (int i = 0; i < AHEAD; ++i) {
                 const int ch = at + i;
                 if (ch >= upto) break;
-                if (!__all_sync(0xffffffffu, free) && !mbar_wait_warp(empty + 8 * stage, parity)) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, free) && (give_up || !mbar_wait_warp(empty + 8 * stage, parity))) { ok = false; break; }
                 tc5_fence_after();
                 // (the next stage asked for before this one is made: 8,192 x 28,672, 64 rows 45.8 to 44.7 us; small ones the same)
                 const int next = stage + 1 == STAGES ? 0 : stage + 1;
@@ -125,11 +128,12 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
                 stage = next;
             }
         }
-        if (ok && upto > from && !__all_sync(0xffffffffu, mbar_wait(done, 0))) ok = false;
-        tc5_fence_after();
+        if (ok && upto > from && !mbar_wait_warp(done, 0)) ok = false;
         if (!ok) *failed = 1;
         __syncthreads();
+        tc5_fence_after();
         // D to shared memory, [row][feature]: every product has ended, and so nothing reads the stages
+        const bool bad = *failed != 0;             // (of any role: all have been here)
         const int quarter = warp & 3, column = (warp >> 2) * (N / 2);
         float* d = reinterpret_cast<float*>(base) + quarter * 32 + lane;
         if (upto > from) {
@@ -138,7 +142,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
                 float v[16];
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + column + j, v);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) d[(column + j + e) * I4T_FEATURES] = v[e];
+                for (int e = 0; e < 16; ++e) d[(column + j + e) * I4T_FEATURES] = bad ? __int_as_float(0x7fc00000) : v[e];
             }
         } else {
             for (int j = 0; j < N / 2; ++j) d[(column + j) * I4T_FEATURES] = 0.f;
@@ -148,7 +152,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
             pdl_wait();                            // x comes from the kernel before this one
             int stage = 0, parity = 1, asked = 0;
             for (int ch = from; ch < upto; ++ch, ++asked) {
-                if (!mbar_wait(empty + 8 * stage, parity)) { *failed = 1; break; }
+                if (give_up || !mbar_wait(empty + 8 * stage, parity)) { *failed = 1; break; }
                 mbar_expect_tx(x_full + 8 * stage, N * 128);
                 tma_load_2d(smem_u32(base) + stage * STAGE, &tm_x, x_full + 8 * stage, ch * 64, r0);
                 if (++stage == STAGES) { stage = 0; parity ^= 1; }
@@ -166,7 +170,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
         int stage = 0, parity = 0;
         bool ok = true;
         for (int ch = from; ch < upto; ++ch) {
-            if (!mbar_wait_warp(full + 8 * stage, parity) || !mbar_wait_warp(x_full + 8 * stage, parity)) { ok = false; break; }
+            if (give_up || !mbar_wait_warp(full + 8 * stage, parity) || !mbar_wait_warp(x_full + 8 * stage, parity)) { ok = false; break; }
             tc5_fence_after();
             const unsigned a = tmem + N + 32 * stage, b = low + stage * (STAGE >> 4);
             if (leader) {
@@ -178,9 +182,11 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
             __syncwarp();
             if (++stage == STAGES) { stage = 0; parity ^= 1; }
         }
-        if (ok && leader && upto > from) umma_commit(done);
+        // (after giving up too: the block goes on when the products that were issued have ended)
         if (!ok) *failed = 1;
+        if (leader && upto > from) umma_commit(done);
         __syncwarp();
+        if (!ok) mbar_wait_warp(done, 0);
         __syncthreads();
     }
     tc5_fence_before();
@@ -195,7 +201,6 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
         constexpr int OUT = GLU ? I4T_FEATURES / 2 : I4T_FEATURES, QUADS = OUT / 4;
         const float* d = reinterpret_cast<const float*>(base);
         const int wide = GLU ? p.n / 2 : p.n, rows_here = min(N, p.rows - r0), items = rows_here * QUADS, mine = (items + splits - 1) / splits;
-        const bool bad = *failed != 0;
         // IN pieces of four features at a time, whose sums are asked for together; joined in the order of the blocks
         constexpr int IN = 4;
         const int last = min(items, (rank + 1) * mine);
@@ -239,7 +244,6 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += feature + e < wide ? p.bias[feature + e] : 0.f;
                 }
-                if (bad) v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fc00000);
                 if ((wide & 3) == 0) {             // (a whole piece, and aligned)
                     if (!GLU && p.y32) *reinterpret_cast<float4*>(p.y32 + to) = make_float4(v[0], v[1], v[2], v[3]);
                     else *reinterpret_cast<uint2*>(p.y + to) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
@@ -257,13 +261,13 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const I4Params p, con
     if (splits > 1) cluster_sync();                // nobody reads this block's memory any more
 }
 
-template <int N, int GS, bool GLU>
+template <int N, int GS, bool GLU, bool TRIAL = false>
 static int launch_int4_tile(const I4Params& p, cudaStream_t stream) {
     static int ready[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "int4_linear: cannot tell the current device");
     if (!ready[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(int4_tile_kernel<N, GS, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I4T_SMEM<N>);
+        const cudaError_t e = cudaFuncSetAttribute(int4_tile_kernel<N, GS, GLU, TRIAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I4T_SMEM<N>);
         if (e != cudaSuccess) return fail(-101, "int4_linear: cannot reserve %zu bytes of shared memory: %s", I4T_SMEM<N>, cudaGetErrorString(e));
         ready[dev] = 1;
     }
@@ -291,12 +295,14 @@ static int launch_int4_tile(const I4Params& p, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return check_launch("int4_linear (tcgen05)", cudaLaunchKernelEx(&cfg, int4_tile_kernel<N, GS, GLU>, tm, p, splits));
+    return check_launch("int4_linear (tcgen05)", cudaLaunchKernelEx(&cfg, int4_tile_kernel<N, GS, GLU, TRIAL>, tm, p, splits));
 }
 
 template <int GS>
 static int int4_tile(const I4Params& p, bool glu, cudaStream_t stream) {
     if (p.rows <= 32) return glu ? launch_int4_tile<32, GS, true>(p, stream) : launch_int4_tile<32, GS, false>(p, stream);
+    if constexpr (GS == 4)                         // (one form of the kernel has the trial)
+        if (p.trial >= 0 && p.rows <= 64) return glu ? launch_int4_tile<64, GS, true, true>(p, stream) : launch_int4_tile<64, GS, false, true>(p, stream);
     if (p.rows <= 64) return glu ? launch_int4_tile<64, GS, true>(p, stream) : launch_int4_tile<64, GS, false>(p, stream);
     if (p.rows <= 128) return glu ? launch_int4_tile<128, GS, true>(p, stream) : launch_int4_tile<128, GS, false>(p, stream);
     return glu ? launch_int4_tile<256, GS, true>(p, stream) : launch_int4_tile<256, GS, false>(p, stream);

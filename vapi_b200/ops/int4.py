@@ -171,7 +171,7 @@ def _rows(x: torch.Tensor, w: Int4Weight, bias, out: torch.Tensor, gated: int, a
     lib = _lib("int4")
     f32 = out.dtype == torch.float32
     _check(lib, lib.vapi_int4_linear(_p(w.codes), _p(w.scales), w.n, w.k, w.group, _p(x), x.shape[0], _p(bias), None if f32 else _p(out),
-                                     _p(out) if f32 else None, gated, act, _stream()), launches=int(x.shape[0] > 0))
+                                     _p(out) if f32 else None, gated, act, -1, _stream()), launches=int(x.shape[0] > 0))
     return out
 
 
