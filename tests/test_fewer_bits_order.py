@@ -1,4 +1,7 @@
 """Operators of serving in fewer bits straight behind the kernels whose results they read: launched without a pause, and captured."""
+import sys
+import threading
+
 import pytest
 import torch
 
@@ -213,3 +216,41 @@ def test_a_product_one_of_whose_blocks_gives_up_is_nan(ops, n, k, splits, gated)
         else:
             assert torch.equal(out, want)
         assert torch.equal(call(x, w), want)
+
+
+# ---- calls of several threads ---------------------------------------------------------------------------
+
+def test_threads_with_unlike_head_sizes(ops):
+    """Head sizes that share a kernel but not an amount of shared memory, from four threads at a time."""
+    i32 = lambda *v: torch.tensor(v, dtype=I32, device="cuda")
+
+    def case(d):
+        g = torch.Generator().manual_seed(d)
+        cache = ops.Cache8(torch.randn(4, 2, 1, 16, d, generator=g).to(torch.float8_e4m3fn).cuda(), torch.zeros(4, 2, 1, 1, dtype=torch.int8, device="cuda"))
+        q, table, cu, kl = torch.randn(2, 8 * d, generator=g).cuda(), i32(0, 1, 2, 3)[None], i32(0, 2), i32(50)
+        return lambda: ops.paged_attention8(q, 8 * d, cache, table, cu, kl, 2, 1, 2, 50, 8, 1, d, 0.1)
+    calls = [case(d) for d in (176, 256, 176, 256)]
+    want, wrong, interval = [f() for f in calls], [], sys.getswitchinterval()
+
+    def run(call, right, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(20000):
+                    got = call()
+                if not torch.equal(got, right):
+                    wrong.append("another result")
+        except Exception as e:
+            wrong.append(str(e))
+    torch.cuda.synchronize()
+    sys.setswitchinterval(1e-6)
+    try:
+        for _ in range(4):
+            threads = [threading.Thread(target=run, args=(f, y, torch.cuda.Stream())) for f, y in zip(calls, want)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    torch.cuda.synchronize()
+    assert not wrong, wrong

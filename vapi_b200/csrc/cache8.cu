@@ -575,10 +575,16 @@ static int launch_attention8_of(const C8Params& p, const void* q, void* out, int
     }
     if (splits > G8_MAX_CLUSTER) splits = G8_MAX_CLUSTER;
     const size_t smem = (size_t)(1 + G8_WARPS) * R * p.d * sizeof(float);
+    constexpr size_t most = (size_t)(1 + G8_WARPS) * R * DMAX * sizeof(float);
     auto kern = attention8_kernel<T, DMAX, R>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    // (the limit of the largest head size, once a device: a limit by the call's would be lowered between another thread's setting and its launch)
+    static int ready[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(-101, "paged_attention8: cannot tell the current device");
+    if (!ready[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        if (e != cudaSuccess) return fail(-101, "paged_attention8: cannot reserve %zu bytes of shared memory: %s", most, cudaGetErrorString(e));
+        ready[dev] = 1;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits), p.nkv, num_seqs);
