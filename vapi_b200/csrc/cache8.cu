@@ -309,6 +309,8 @@ VAPI_EXPORT int vapi_qk_norm_rope_write8(const void* qkv, int dtype, const float
     if (nh <= 0 || nkv <= 0) return fail(-1, "qk_norm_rope_write8: no heads");
     if (cosr && (rot <= 0 || rot > d || rot % 2 != 0)) return fail(-1, "qk_norm_rope_write8: rotation width %d does not fit head_dim %d", rot, d);
     if (page_size <= 0 || page_size % C8_BLOCK != 0 || num_pages <= 0) return fail(-1, "qk_norm_rope_write8: page size %d is not a multiple of 16, or there are no pages", page_size);
+    // (older codes of a block are read by words; the read and attention take pieces of 16 bytes)
+    if (((uintptr_t)codes & 15) != 0) return fail(-1, "qk_norm_rope_write8: the codes are not 16-byte aligned");
     // (16-byte rows of everything that is read or written by the piece)
     if (dtype == VAPI_BF16 && (d == 64 || d == 128) && (!cosr || rot == d) &&
         (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)codes | (uintptr_t)cosr | (uintptr_t)sinr) & 15) == 0)
