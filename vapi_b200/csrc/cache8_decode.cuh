@@ -173,7 +173,7 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         // largest element to [2^14, 2^15); the exponent kept where both factors are ordinary numbers
-        const int x = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120);
+        const int x = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
         const float up = c8_power(14 - x), down = c8_power(x - 14) * p.scale_log2e;
         const int pos = ok ? base + tok : -1;                               // -1: sees nothing
 #pragma unroll

@@ -333,7 +333,7 @@ prompt8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
 #pragma unroll
                 for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
             }
-            const int x = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120);
+            const int x = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
             const float up = c8_power(14 - x);
             row_f = c8_power(x - 14) * p.scale_log2e;
 #pragma unroll
