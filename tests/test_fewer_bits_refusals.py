@@ -39,3 +39,45 @@ def test_the_write_refuses_codes_off_16_bytes(ops, dtype):
             assert ops.launch_count == before
         else:
             call()
+
+
+# ---- a plan that several runners use, one after the other ------------------------------------------------
+
+def _plan_and_tensors(cfg, seed=3):
+    from vapi_b200.config.model import resolve_architecture
+    from vapi_b200.weights.random import random_tensors
+    arch = resolve_architecture(cfg)
+    plan = arch.plan(arch.parse(cfg))
+    return plan, random_tensors(plan, seed, 0.1, "ones", F32, device="cpu")
+
+
+def _runner(plan, tensors, **kw):
+    from vapi_b200.engine.runner import ModelRunner
+    return ModelRunner(plan, tensors, dtype="float32", device="cpu", num_pages=8, max_requests=2, max_batched_tokens=64, page_size=16, **kw)
+
+
+def _paged(runner):
+    return [(g.spec.eight_bit, g.tensor.dtype, g.exps is not None) for g in runner.cache.paged]
+
+
+def test_a_runner_with_the_plan_of_an_eight_bit_one_keeps_numbers():
+    from conftest import TINY_A
+    plan, tensors = _plan_and_tensors(TINY_A)
+    numbers, codes = [(False, F32, False)], [(True, torch.float8_e4m3fn, True)]
+    for kind, want in (("auto", numbers), ("fp8", codes), ("auto", numbers), ("fp8", codes)):
+        r = _runner(plan, tensors, kv_cache_dtype=kind)
+        assert _paged(r) == want and all(getattr(b.mixer, "cache8", False) == (kind == "fp8") for b in plan.layers if hasattr(b.mixer, "nkv"))
+
+
+def test_a_refusal_leaves_the_plan_as_it_was():
+    from conftest import TINY_A
+    plan, tensors = _plan_and_tensors(TINY_A)
+    with pytest.raises(ValueError, match="groups of 128"):
+        _runner(plan, tensors, kv_cache_dtype="fp8", weight_dtype="int4", weight_group=128)
+    assert not any(getattr(b.mixer, "cache8", False) for b in plan.layers)
+    last = [b.mixer for b in plan.layers if hasattr(b.mixer, "nkv")][-1]
+    last.general = True
+    with pytest.raises(ValueError, match="no form with a cache in 8 bits"):
+        _runner(plan, tensors, kv_cache_dtype="fp8")
+    last.general = False
+    assert not any(getattr(b.mixer, "cache8", False) for b in plan.layers) and _paged(_runner(plan, tensors)) == [(False, F32, False)]

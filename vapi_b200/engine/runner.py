@@ -69,12 +69,16 @@ class ModelRunner:
         #: keys and values "auto": in the activations' type; "fp8": e4m3 codes, a scale for each 16 tokens of a head.  The layers'
         #: matrices "auto": in the activations' type; "int4": 4-bit codes, a scale and a zero for each ``weight_group`` columns of a row
         self.kv_cache_dtype, self.weight_dtype = check_fewer_bits(kv_cache_dtype, weight_dtype, weight_group)
-        if self.kv_cache_dtype == "fp8":
+        try:
+            for blk in plan.layers:          # (the plan may have been another runner's)
+                blk.mixer.use_cache8(self.kv_cache_dtype == "fp8")
+            plan.bind(tensors, self.dtype)
+            if self.weight_dtype == "int4":
+                plan.quantize4(int(weight_group))
+        except BaseException:
             for blk in plan.layers:
-                blk.mixer.use_cache8()
-        plan.bind(tensors, self.dtype)
-        if self.weight_dtype == "int4":
-            plan.quantize4(int(weight_group))
+                blk.mixer.use_cache8(False)
+            raise
         self.vocab_size = plan.vocab_size
         self.max_context = min(int(max_context or plan.max_positions), plan.max_positions)
         if num_pages is not None:            # no request can hold more tokens than the pool has

@@ -111,10 +111,10 @@ class GQAttention(Mixer):
         return PagedSpec((PagedBuffer("k", self.nkv, self.d), PagedBuffer("v", self.nkv, self.dv)),
                          0 if self.keep_first > 0 else self.window, self.cache8)
 
-    def use_cache8(self):
-        if self.general:
+    def use_cache8(self, on=True):
+        if on and self.general:
             raise ValueError("attention with unlike widths, a chunk, a sink, gates or another of its options has no form with a cache in 8 bits")
-        self.cache8 = True
+        self.cache8 = bool(on)
 
     def quantize4(self, group):
         self.w_qkv, self.w_o = ops.int4_quantize(self.w_qkv, group), ops.int4_quantize(self.w_o, group)

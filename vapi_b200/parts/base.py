@@ -308,11 +308,11 @@ class Mixer(Part):
         the answer comes back to the mixer as ``cache.group.splits``.  1: no cutting."""
         return 1
 
-    def use_cache8(self) -> None:
-        """Keep what the mixer caches per token in 8 bits (asked before the cache is laid out).  A mixer without pages has nothing
-        to do; one whose pages have no such form refuses."""
+    def use_cache8(self, on: bool = True) -> None:
+        """Keep what the mixer caches per token in 8 bits, or (``on`` False) as numbers again (asked before the cache is laid out).  A mixer
+        without pages has nothing to do; one whose pages have no such form refuses."""
         spec = self.cache_spec()
-        if any(isinstance(s, PagedSpec) for s in (spec if isinstance(spec, tuple) else (spec,))):
+        if on and any(isinstance(s, PagedSpec) for s in (spec if isinstance(spec, tuple) else (spec,))):
             raise ValueError(f"{type(self).__name__} has no form with a cache in 8 bits")
 
     # A mixer of the form ``W_out inner(W_in a + b_in) + b_out`` may offer itself in pieces, so that a mixer made of
