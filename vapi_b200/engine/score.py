@@ -27,11 +27,12 @@ class TextScore:
 
     @property
     def perplexity(self) -> float:
-        """exp of the mean negative log probability (NaN for a text of one token)."""
+        """exp of the mean negative log probability (NaN for a text of one token, and where a log probability is NaN; infinity where a
+        token had none)."""
         if not self.logprobs:
             return math.nan
         mean = -sum(self.logprobs) / len(self.logprobs)
-        return math.exp(mean) if mean < 700 else math.inf
+        return math.inf if mean >= 700 else math.exp(mean)
 
 
 def score_texts(runner: ModelRunner, texts: Sequence[Sequence[int]], top: int = 0, portion: int = 2048) -> List[TextScore]:
