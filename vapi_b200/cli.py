@@ -124,11 +124,13 @@ def main(argv: Optional[List[str]] = None) -> int:
         except ValueError as e:
             print(f"vapi_b200: {e}", file=sys.stderr)
             return 2
+        number = lambda x: x if math.isfinite(x) else None              # (JSON has no other)
         for i, s in enumerate(scores):
-            rec = {"request": i, "tokens": len(s.tokens), "perplexity": s.perplexity if math.isfinite(s.perplexity) else None, "logprobs": s.logprobs, "entropies": s.entropies}
+            rec = {"request": i, "tokens": len(s.tokens), "perplexity": number(s.perplexity), "logprobs": [number(x) for x in s.logprobs],
+                   "entropies": [number(x) for x in s.entropies]}
             if args.logprobs:
-                rec["top"] = s.top
-            print(json.dumps(rec), flush=True)
+                rec["top"] = [[(t, number(x)) for t, x in place] for place in s.top]
+            print(json.dumps(rec, allow_nan=False), flush=True)
         return 0
     params = SamplingParams(
         temperature=args.temperature, top_p=args.top_p, top_k=args.top_k, min_p=args.min_p,
