@@ -647,7 +647,8 @@ static bool c8_portions(const C8Params& p, int n, int num_seqs, int max_q, int m
 // a sequence has); else those of the mma.sync kernel, up to 16, and at most 8, a power of two, of the tcgen05 kernel.
 // settled: no kernel that may still run when this one begins (the one before it, and those that it begins before the end of) writes keys before a sequence's
 // own tokens, as in an engine's step; else no key is read before every earlier kernel has ended.  us of one call after another, settled and not, 32 / 8
-// heads of 64: one request of 4,090 keys 6.0 / 6.4, 64 of 128 to 2,048 19.7 / 20.3, 8 of 32,000 47.0 / 49.0, 2,048 tokens behind 5,952 235.9 / 236.4.
+// heads of 64, over one cache: one request of 4,090 keys 5.9 / 6.2, 64 of 128 to 2,048 19.6 / 20.7, 8 of 32,000 47.0 / 48.8, 2,048 tokens behind 5,952
+// 235.7 / 235.7; over three caches in turn 6.5 / 7.1, 20.3 / 21.7 (22.9 without asking for the first chunks ahead of the wait), 51.6 / 52.8, 236.1 / 235.5.
 VAPI_EXPORT int vapi_paged_attention8(const void* q, long long q_row_stride, const void* codes, const void* exps, int dtype, const int* block_table,
                                       int table_stride, const int* cu_q, const int* seqlens_k, void* out, int n, int num_seqs, int max_q,
                                       int max_k, int nh, int nkv, int d, int page_size, int num_pages, float scale, int window, int splits,

@@ -63,6 +63,9 @@ __device__ __forceinline__ void d8_copy(unsigned dst, const void* src, unsigned 
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void d8_prefetch(const void* src, unsigned bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ uint4 d8_lds16(unsigned addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -118,11 +121,11 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
     const int* bt = p.block_table + (size_t)s * p.table_stride;
     const int per_head = p.page_size / C8_BLOCK;
     const int fresh = !p.settled || base < 0 ? 0 : base / C8_BLOCK;         // the first chunk that a kernel not yet waited for may have changed
+    const size_t to_values = (size_t)p.nkv * per_head * CHUNK;
     bool waited = false;
     int where = 0, scales_next = 0, scales = 0;
     auto look_up = [&](int from) {                                          // chunks begin + from ..
         const int last = min(end, begin + from + 32) - 1;
-        if (!waited && last >= fresh) { pdl_wait(); waited = true; }
         const int key = min(begin + from + lane, last) * C8_BLOCK;
         int page = bt[key / p.page_size];
         if (page < 0 || page >= p.num_pages) {
@@ -130,9 +133,17 @@ decode8_kernel(const C8Params p, const __nv_bfloat16* __restrict__ q, __nv_bfloa
             page = 0;
         }
         where = (page * 2 * p.nkv + g) * per_head + key % p.page_size / C8_BLOCK;
+        if (!waited && last >= fresh) {
+            // (what the ring takes first is on its way to L2 meanwhile)
+            if (lane < min(nt, 2 * D8_STAGES)) {
+                d8_prefetch(p.codes + (size_t)where * CHUNK, CHUNK);
+                d8_prefetch(p.codes + (size_t)where * CHUNK + to_values, CHUNK);
+            }
+            pdl_wait();
+            waited = true;
+        }
         scales_next = c8_scales(p, where, per_head);
     };
-    const size_t to_values = (size_t)p.nkv * per_head * CHUNK;
     auto bring = [&](int it, int stage) {                                   // chunks begin + 2 it and the next into a place of the ring: K, K, V, V
         if ((it & 15) == 0) look_up(2 * it);
         const int at = __shfl_sync(0xffffffffu, where, (2 * it + (lane & 1)) & 31);
