@@ -196,6 +196,32 @@ def test_settled_steps_read_their_own_tokens_when_they_are_written(ops, d, rows,
         assert torch.equal(got, want) and not ops._held.settled
 
 
+@pytest.mark.parametrize("d,rows,impl", [(64, 1, "auto"), (128, 1, "tensor_core"), (64, 40, "tcgen05"), (64, 1, "general")])
+def test_index_data_of_the_kernel_just_before(ops, d, rows, impl):
+    """Lengths and pages that another library's kernels write right ahead of the call, other ones each time."""
+    n, ends = 1536, _ends(rows)                              # (whole pages: in another order they hold numbers too)
+    p = Prompt(ops, d, n)
+    q = p.write(0, n)[n - rows:]
+    lengths = [torch.tensor([k], dtype=I32, device="cuda") for k in (n, 700, 64, n - 1)]
+    tables = [p.table.clone(), p.table.flip(1).contiguous()]
+    torch.cuda.synchronize()
+
+    def body(between=lambda: None):
+        out = []
+        for table in tables:
+            for length in lengths:
+                torch.add(table, 0, out=p.table)
+                torch.mul(length, 1, out=p.lens)
+                between()
+                out.append(p.attend(q, ends, impl))
+        return out
+    want = body(torch.cuda.synchronize)
+    assert all(torch.isfinite(y).all() for y in want)
+    for turn in range(20):
+        for got in _played(body):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---- a wait that is given up ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("gated", [0, 1])

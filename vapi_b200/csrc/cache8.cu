@@ -285,7 +285,8 @@ write8_vec_kernel(const __nv_bfloat16* __restrict__ qkv, const float* __restrict
     }
 }
 
-// Tokens of a step from which on a warp takes 16 of them: no step of single tokens is as large.  us of one and of 16 a warp, 32 / 8 heads of 64: runs of
+// Tokens of a step from which on a warp takes 16 of them: steps as large are a portion's.  (Single tokens beside it then take turns in a warp; the rule goes by
+// the step and not by its runs.)  us of one and of 16 a warp, 32 / 8 heads of 64: runs of
 // 128 tokens 3.3 / 3.2, 256 3.9 / 3.5, 512 5.4 / 3.8, 2,048 14.6 / 7.6; single tokens, 8 of them 2.8 / 14.3, 64 3.4 / 28.6.
 constexpr int W8_GROUP_TOKENS = 512;
 

@@ -13,7 +13,7 @@
 // What bounds it: making the numbers.  A chunk is 64 conversions a lane of eight warps beside barriers and the store, 430 cycles of a warp one after
 // the other, and about as many of a multiprocessor with two blocks on it; the products of 64 rows take 180, the bytes of a chunk's codes 190.  64
 // rows of 8,192 x 28,672 in 45 us (2.7 TB/s of codes; with 16-bit weights the product takes 76), of 16,384 x 2,048 gated in 11.0 (9.6), of 2,048 x
-// 8,192 in 11.4 (11.9); 2,048 rows of 2,048 x 8,192 in 48 us, 1.43 PFLOP/s.
+// 8,192 in 11.4 (11.9); 2,048 rows of 2,048 x 8,192 in 48 us, 1.43 PFLOP/s, and in 61 where one pass follows another (the power cap).
 //
 // Every wait is bounded; a role that gives up marks the block, whose sums are then NaN, and so is every result of its cluster, which adds them up.  The
 // products and copies that are under way are awaited first.

@@ -1114,6 +1114,9 @@ def paged_attention(q: torch.Tensor, q_row_stride: int, cache_layer: torch.Tenso
     128, page size a multiple of 64) and the general kernel elsewhere; "general" and
     "tensor_core" force one (the latter raises where it does not apply); "decode" forces the
     TMA-fed decode kernel (bfloat16, head_dim 64, at most 16 rows per sequence and kv head).
+
+    The bfloat16 kernels read the keys before a sequence's own tokens of the call (its last ``cu_q[s + 1] - cu_q[s]``) ahead of the wait for the
+    kernel before: no kernel still on its way may write them, as in a step of an engine (:class:`one_stream`, ``settled``).
     """
     _cuda(q, cache_layer, block_table, cu_q, seqlens_k)
     _i32(block_table, "block table")
@@ -1182,7 +1185,7 @@ def decode_attention_fused(qkv: torch.Tensor, nh: int, nkv: int, d: int,
     ``cache_layer`` (``write_kv``) at the places the block table gives for the sequences' last
     ``q`` positions, and attention over the cache.  ``qkv`` [n, (nh+2nkv)*d] is left as it was.
     bfloat16, head_dim 64, pages of 64n, at most 16 rows per sequence and kv head.  Gives exactly
-    what the two calls give."""
+    what the two calls give, and like :func:`paged_attention` reads older keys ahead."""
     _cuda(qkv, q_weight, k_weight, cos, sin, cache_layer, block_table, cu_q, seqlens_k)
     _contig(qkv, "qkv")
     _contig(cache_layer, "cache layer")
@@ -1743,7 +1746,8 @@ def masked_attention(q: torch.Tensor, q_row_stride: int, cache_layer: torch.Tens
     of its own row (latent attention).  ``softcap`` > 0: a score passes ``softcap * tanh(score / softcap)``;
     ``score_bias`` [nh] float32 is added to head h's scores behind the cap; ``weights`` "sigmoid": a visible key's weight
     is the sigmoid of its score and nothing is normalised over the keys (no sink then).  The output is multiplied by
-    ``out_scale`` and may go into ``out`` [n, nh*dv] with unit inner stride, e.g. a part of a wider buffer."""
+    ``out_scale`` and may go into ``out`` [n, nh*dv] with unit inner stride, e.g. a part of a wider buffer.  Keys before a sequence's own tokens
+    may be read ahead of the kernel before, as by :func:`paged_attention`."""
     _cuda(q, cache_layer, block_table, cu_q, seqlens_k, sinks, gate, score_bias)
     _f32(score_bias, "score bias")
     if weights not in ("softmax", "sigmoid"):

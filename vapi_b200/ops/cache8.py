@@ -53,7 +53,8 @@ def qk_norm_rope_write8(qkv: torch.Tensor, nh: int, nkv: int, d: int, q_weight: 
     Tokens of one block of 16 must follow one another in the step, as a request's do, and no two name one slot (what such a block then
     holds is not said: its tokens may be on another's scale).  A block whose first token (place 0) is
     among them begins afresh; the older tokens of another one are rounded again when a new token needs a larger scale.  What
-    is not finite is kept as NaN."""
+    is not finite is kept as NaN.  ``slot_mapping`` is index data: it is read ahead of the wait for the kernel before, and none of this package's
+    kernels on its way may write it."""
     if qkv.is_cuda:
         lib = _lib("cache8")
         got = _native("write8", lib, "vapi_qk_norm_rope_write8", qkv, nh, nkv, d, q_weight, k_weight, eps, cos, sin, rot, cache[0], cache[1],
@@ -130,7 +131,8 @@ def paged_attention8(q: torch.Tensor, q_row_stride: int, cache: Cache8, block_ta
     of the same portion that stand before it in one tile, as with :func:`paged_attention`.
 
     The cache may be the work of any kernel ahead on the stream.  Within ``one_stream(settled=True)`` what it holds before a sequence's own tokens of
-    the call is read while kernels ahead still run, and must be none of theirs.
+    the call is read while kernels ahead still run, and must be none of theirs.  ``block_table``, ``cu_q`` and ``seqlens_k`` are index data, read
+    ahead of that wait always: none of this package's kernels on its way may write them.
 
     ``impl``: "auto" picks: for bfloat16 and head size 64 or 128 the tcgen05 kernel for prompt portions (where rows and keys are enough for
     it), and the mma.sync kernel for the others, in both of which ``splits`` blocks (up to 16, and up to 8) share the keys as a cluster; the
