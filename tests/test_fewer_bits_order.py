@@ -280,3 +280,32 @@ def test_threads_with_unlike_head_sizes(ops):
         sys.setswitchinterval(interval)
     torch.cuda.synchronize()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("d,dtype", [(64, BF), (128, BF), (64, F32), (48, BF)])
+@pytest.mark.parametrize("requests,tokens", [(64, 1), (3, 5), (1, 40)])
+def test_writes_one_after_the_other(ops, d, dtype, requests, tokens):
+    """Steps of the same requests without a pause, each larger than the last, so that blocks' exponents, which lie side by side, keep growing; then the read."""
+    nkv, nh, page, steps = 8, 8, 64, 20
+    per = -(-steps * tokens // page)
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(steps, requests * tokens, (nh + 2 * nkv), d, generator=g)
+    grow = torch.rand(steps, requests * tokens, nh + 2 * nkv, 1, generator=g).cumsum(0)
+    x = (x * torch.exp2(2 * grow)).view(steps, requests * tokens, -1).to(dtype).cuda()
+    order = torch.randperm(requests * per, generator=g).view(requests, per)
+    pos = torch.arange(steps * tokens)
+    slots = (order[:, pos // page] * page + pos % page).view(requests, steps, tokens).transpose(0, 1).reshape(steps, -1).to(I32).contiguous().cuda()
+    cache, pages = ops.cache8_empty(requests * per, nkv, page, d), torch.arange(requests * per, dtype=I32, device="cuda")
+
+    def body(between=lambda: None):
+        cache.codes.view(torch.uint8).zero_()
+        cache.exps.fill_(-110)
+        for i in range(steps):
+            between()
+            ops.qk_norm_rope_write8(x[i], nh, nkv, d, None, None, 0.0, None, None, 0, cache, slots[i])
+        between()
+        return [ops.cache8_read(cache, pages, F32), cache.exps.clone()]
+    want = body(torch.cuda.synchronize)
+    for turn in range(10):
+        for got in _played(body):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
